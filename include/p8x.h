@@ -268,6 +268,105 @@ void p8x_gemv_batch_release(p8x_gemv_batch *b);
 typedef struct p8x_batch_info { int njobs, ncols, class_set, units, split_jobs, small_launch, waves, matrix_cores; } p8x_batch_info;
 int p8x_gemv_batch_info(const p8x_gemv_batch *b, p8x_batch_info *out);
 
+/* ---- between the linears: norms, cache, attention of drafted tokens ---------------------------------------- */
+/* No counterpart in the reference (ggml's own kernels run there): what a decode step over drafted tokens needs beside
+ * p8x_mul_mat_vec and p8x_mul_mat, for hosts that have no other kernels for it. All calls are asynchronous on the
+ * stream, allocate nothing, record kernel launches only and are deterministic; they keep nothing between calls. The
+ * structs are read during the call, what they point to is device memory. Fields left 0 / NULL take the stated default. */
+enum { P8X_NORM_NONE = 0, P8X_NORM_RMS = 1, P8X_NORM_LAYER = 2 };
+enum { P8X_GATE_LINEAR = 0, P8X_GATE_SIGMOID = 1 };
+#define P8X_NORM_MAX_C 32768
+
+/* The end of one block and the start of the next, row by row (n rows of C elements, strides in elements):
+ *   u  = N_post(y), N_RMS(v) = v / sqrt(mean(v^2) + eps) w (+ b), N_LAYER the same of v - mean(v), N_NONE(v) = v
+ *   h' = h + alpha a(gate) u        -> h_out (h_out may be h)
+ *   x  = N_pre(h')                  -> x (of the unrounded h')
+ * Types P8X_F32 | P8X_F16 | P8X_BF16 for each of y, h (and h_out), x and gate; sums in f32. */
+typedef struct p8x_norm_args {
+    int n, C;                       /* n >= 0, 1 <= C <= P8X_NORM_MAX_C */
+    const void *y; int y_dtype; size_t ldy;          /* the block's output; NULL: h' = h */
+    const void *h; int h_dtype; size_t ldh;          /* the residual */
+    void *h_out; size_t ldho;                        /* NULL: not stored */
+    void *x; int x_dtype; size_t ldx;                /* NULL: not stored; overlaps no input */
+    int post; const float *w_post, *b_post; float eps_post;   /* w, b [C]; NULL: 1, 0 */
+    int pre;  const float *w_pre,  *b_pre;  float eps_pre;
+    const void *gate; int gate_dtype; size_t ld_gate; int gate_act;   /* NULL: no gate; ld_gate 0: one row for all */
+    float alpha;                    /* residual scale (no default: 0 drops the block) */
+} p8x_norm_args;
+int p8x_norm_residual(const p8x_norm_args *a, void *stream);
+
+/* A key/value cache in the caller's memory: rows of head_dim elements, K and V with the same strides (elements, multiples
+ * of 8; K and V 16-byte aligned). Slot i of sequence s lies in page pages[s ld_pages + i / page_size], place i % page_size.
+ * A table entry outside 0 .. n_pages - 1 holds no slots: reads see them masked, writes to them are dropped. A slot is
+ * a place, not a position: keys carry their rotation, and attention does not ask for the slots' order. */
+typedef struct p8x_kv_cache {
+    int dtype;                      /* P8X_F16 | P8X_BF16 */
+    int n_seq, n_kv, head_dim;      /* head_dim 64, 128 or 256 */
+    void *k, *v;
+    size_t page_stride, head_stride, slot_stride;
+    int page_size, n_pages;         /* page_size a multiple of 16 (any size with pages NULL) */
+    const int32_t *pages; size_t ld_pages;   /* NULL: sequence s lies in page s */
+    const int32_t *len;             /* [n_seq] slots in use, clamped to 0 .. max_len */
+    int max_len;                    /* slots a sequence can hold; also the row length of score and pos arrays */
+} p8x_kv_cache;
+
+/* Drafted tokens as a layer's products leave them: sequence s has tokens first[s] .. first[s + 1] - 1 (at most
+ * max_tokens, further ones are ignored). Token rows ld_* elements apart, heads head_stride_* apart (0: head_dim). k and v
+ * in the cache's type, or in P8X_F32 and then rounded to it (to nearest even), as p8x_kv_append stores them. Rows and
+ * heads 16-byte aligned (strides multiples of 8, or of 4 for P8X_F32). */
+typedef struct p8x_drafts {
+    int n_tokens, max_tokens;
+    const int32_t *first;           /* [n_seq + 1] */
+    const void *k, *v; int kv_dtype; size_t ld_kv, head_stride_kv;
+    const uint64_t *mask;           /* [n_tokens] bit j: the token sees token j of its sequence; NULL: itself and those before */
+    int n_heads;                    /* query heads, a multiple of n_kv; consecutive ones share a key/value head */
+    const void *q; int q_dtype; size_t ld_q, head_stride_q;   /* P8X_F32, or the cache's type */
+    float scale;                    /* of q . k */
+} p8x_drafts;
+
+/* out = softmax(scale q k) v over the slots of the token's sequence and the drafted tokens its mask shows, out in q's
+ * type, lse [n_tokens][n_heads] = log of the sum of exp (NULL: not stored). A token that sees nothing gets 0 and
+ * lse -inf; what a mask hides does not reach the token, be it infinite or NaN. At most P8X_MAX_DRAFT tokens a sequence.
+ * P8X_F32 queries are multiplied in f32 accuracy (as sums of 16-bit parts), 16-bit ones as they are; the weights are
+ * rounded to no less than 16 bits either way, sums are f32.
+ * workspace: device memory that splits a sequence over workgroups (NULL or too little: fewer of them), zeroed
+ * once by the caller before its first use and left zeroed where it has to be; calls that may overlap need one each.
+ * p8x_attn_workspace: bytes beyond which more do not help for this shape. */
+#define P8X_MAX_DRAFT 64
+int p8x_attn_tree(const p8x_kv_cache *c, const p8x_drafts *d, void *out, size_t ld_out, size_t head_stride_out, float *lse,
+                  void *workspace, size_t workspace_bytes, void *stream);
+size_t p8x_attn_workspace(const p8x_kv_cache *c, const p8x_drafts *d);
+
+/* Attention weight that the accepted tokens gave, for each key/value head (lse from p8x_attn_tree):
+ *   score_out[s][h][j] = decay score[s][h][j] + sum over accepted tokens i and the heads of h of exp(scale q_i k_j - lse_i)
+ * for the slots j < len[s], and the sum alone for accepted tokens, at slot len[s] + rank (where p8x_kv_append puts them).
+ * accept [n_seq]: bit j = token j of the sequence is accepted; NULL: all. Rows of max_len, score_out may be score; the rest
+ * of score_out is left as it is. Call it before p8x_kv_append when that updates len in place. */
+int p8x_kv_score(const p8x_kv_cache *c, const p8x_drafts *d, const uint64_t *accept, const float *lse, float decay, const float *score,
+                 float *score_out, void *stream);
+
+/* Keys and values of the accepted tokens (accept as above; NULL: all, then any number of tokens) to slots len[s] + rank of
+ * their sequence, in the cache's type; pos [n_seq][n_kv][max_len] at those slots = at[token] (either NULL: not stored);
+ * len_out[s] = len[s] + accepted (len_out may be c->len; NULL: not stored). Tokens past max_len are dropped. */
+int p8x_kv_append(const p8x_kv_cache *c, const p8x_drafts *d, const uint64_t *accept, const int32_t *at, int32_t *pos, int32_t *len_out,
+                  void *stream);
+
+/* Cuts every key/value head of a sequence with more than `budget` slots to the budget. Kept are, in this order, slots with
+ * pos < n_sink or pos >= 1 + max(pos) - n_recent, then the highest scores (NaN lowest); equal ones by lower slot. The i-th kept slot
+ * >= budget moves into the i-th freed slot < budget: K and V in place, and score, pos into score_out, pos_out (either
+ * may be its input), whose slots < min(len, budget) are written; len_out = min(len, budget). No other slot changes. pos
+ * may be NULL when n_sink and n_recent are 0. Rows of max_len. n_sink + n_recent <= budget.
+ * workspace: at least p8x_kv_evict_workspace bytes, any contents. */
+typedef struct p8x_evict_args {
+    int budget, n_sink, n_recent;
+    const float *score; float *score_out;
+    const int32_t *pos; int32_t *pos_out;
+    int32_t *len_out;
+    void *workspace; size_t workspace_bytes;
+} p8x_evict_args;
+int p8x_kv_evict(const p8x_kv_cache *c, const p8x_evict_args *a, void *stream);
+size_t p8x_kv_evict_workspace(const p8x_kv_cache *c, int budget);
+
 /* ---- native model files (GGUF): slot bytes for p8x_prepare ----------------------------------------------- */
 /* The host side of the reference's model loader for VR tensors (llama_model_loader::vr_native_init and
  * vr_native_load, CPU.patch:4700-4869): p8x_vr_open parses one GGUF file (or the shards of one model, metadata from

@@ -17,6 +17,9 @@ P8X_OK, P8X_ERR_ARG, P8X_ERR_FORMAT, P8X_ERR_HIP, P8X_ERR_UNSUPPORTED, P8X_ERR_N
 F32, F16, BF16, I16 = 0, 1, 2, 3
 ACT_Q8_128, ACT_Q8_1, ACT_X16 = 0, 1, 2
 MM_NONE, MM_ROW_GROUP, MM_FUSED, MM_DECODED = 0, 1, 2, 3   # kernels of a prompt GEMM (mul_mat_plan)
+NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2
+GATE_LINEAR, GATE_SIGMOID = 0, 1
+MAX_DRAFT = 64   # drafted tokens of a sequence
 GEMV_KERNEL_AUTO, GEMV_KERNEL_DOT4, GEMV_KERNEL_MFMA = 0, 1, 2   # p8x_gemv_batch_create_ex
 MAX_COLS = 8
 VR3_TAG = 0x56523300
@@ -33,7 +36,8 @@ EXPORTS = [
     "p8x_mul_mat_vec_glu_act", "p8x_gemv_batch_create_act", "p8x_gemv_batch_create_ex", "p8x_graph_begin", "p8x_decode_tiles",
     "p8x_dequantize_rows", "p8x_vec_dot_rows", "p8x_encode_defaults", "p8x_encode_tensor", "p8x_encode_free",
     "p8x_encode_factor", "p8x_encode_alloc", "p8x_step_create", "p8x_step_create_act", "p8x_step_run", "p8x_step_check", "p8x_step_info",
-    "p8x_step_release",
+    "p8x_step_release", "p8x_norm_residual", "p8x_attn_tree", "p8x_attn_workspace", "p8x_kv_score", "p8x_kv_append", "p8x_kv_evict",
+    "p8x_kv_evict_workspace",
 ]
 
 
@@ -79,6 +83,39 @@ class EncodeParams(ctypes.Structure):
 class StepStageC(ctypes.Structure):
     _fields_ = [("n", ctypes.c_int), ("tensors", ctypes.c_void_p * 4), ("x", ctypes.c_void_p), ("y", ctypes.c_void_p * 4),
                 ("glu_out", ctypes.c_void_p)]
+
+
+class NormArgs(ctypes.Structure):
+    _fields_ = [("n", ctypes.c_int), ("C", ctypes.c_int),
+                ("y", ctypes.c_void_p), ("y_dtype", ctypes.c_int), ("ldy", ctypes.c_size_t),
+                ("h", ctypes.c_void_p), ("h_dtype", ctypes.c_int), ("ldh", ctypes.c_size_t),
+                ("h_out", ctypes.c_void_p), ("ldho", ctypes.c_size_t),
+                ("x", ctypes.c_void_p), ("x_dtype", ctypes.c_int), ("ldx", ctypes.c_size_t),
+                ("post", ctypes.c_int), ("w_post", ctypes.c_void_p), ("b_post", ctypes.c_void_p), ("eps_post", ctypes.c_float),
+                ("pre", ctypes.c_int), ("w_pre", ctypes.c_void_p), ("b_pre", ctypes.c_void_p), ("eps_pre", ctypes.c_float),
+                ("gate", ctypes.c_void_p), ("gate_dtype", ctypes.c_int), ("ld_gate", ctypes.c_size_t), ("gate_act", ctypes.c_int),
+                ("alpha", ctypes.c_float)]
+
+
+class KvCacheC(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int), ("n_seq", ctypes.c_int), ("n_kv", ctypes.c_int), ("head_dim", ctypes.c_int),
+                ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("page_stride", ctypes.c_size_t), ("head_stride", ctypes.c_size_t), ("slot_stride", ctypes.c_size_t),
+                ("page_size", ctypes.c_int), ("n_pages", ctypes.c_int), ("pages", ctypes.c_void_p), ("ld_pages", ctypes.c_size_t),
+                ("len", ctypes.c_void_p), ("max_len", ctypes.c_int)]
+
+
+class DraftsC(ctypes.Structure):
+    _fields_ = [("n_tokens", ctypes.c_int), ("max_tokens", ctypes.c_int), ("first", ctypes.c_void_p),
+                ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("kv_dtype", ctypes.c_int), ("ld_kv", ctypes.c_size_t), ("head_stride_kv", ctypes.c_size_t),
+                ("mask", ctypes.c_void_p), ("n_heads", ctypes.c_int),
+                ("q", ctypes.c_void_p), ("q_dtype", ctypes.c_int), ("ld_q", ctypes.c_size_t), ("head_stride_q", ctypes.c_size_t), ("scale", ctypes.c_float)]
+
+
+class EvictArgs(ctypes.Structure):
+    _fields_ = [("budget", ctypes.c_int), ("n_sink", ctypes.c_int), ("n_recent", ctypes.c_int),
+                ("score", ctypes.c_void_p), ("score_out", ctypes.c_void_p), ("pos", ctypes.c_void_p), ("pos_out", ctypes.c_void_p),
+                ("len_out", ctypes.c_void_p), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)]
 
 
 _lib = None
@@ -152,6 +189,14 @@ def lib():
     L.p8x_gemv_batch_run_stage_timed.argtypes = [vp, i, vp, vp, vp]
     L.p8x_gemv_batch_release.argtypes = [vp]; L.p8x_gemv_batch_release.restype = None
     L.p8x_gemv_batch_info.argtypes = [vp, ctypes.POINTER(BatchInfo)]
+    cache, drafts, f = ctypes.POINTER(KvCacheC), ctypes.POINTER(DraftsC), ctypes.c_float
+    L.p8x_norm_residual.argtypes = [ctypes.POINTER(NormArgs), vp]
+    L.p8x_attn_tree.argtypes = [cache, drafts, vp, sz, sz, vp, vp, sz, vp]
+    L.p8x_attn_workspace.argtypes = [cache, drafts]; L.p8x_attn_workspace.restype = sz
+    L.p8x_kv_score.argtypes = [cache, drafts, vp, vp, f, vp, vp, vp]
+    L.p8x_kv_append.argtypes = [cache, drafts, vp, vp, vp, vp, vp]
+    L.p8x_kv_evict.argtypes = [cache, ctypes.POINTER(EvictArgs), vp]
+    L.p8x_kv_evict_workspace.argtypes = [cache, i]; L.p8x_kv_evict_workspace.restype = sz
     _lib = L
     return L
 
@@ -876,3 +921,101 @@ class GemvBatch:
             self.release()
         except Exception:
             pass
+
+
+# --------------------------------------------------------------------------------------------------- between the linears
+# Calls with their arguments filled in once (a decode loop runs them on the same buffers every step): run(stream) is one
+# library call. Buffers are DeviceBuffers or device addresses; they are kept alive here only where they are DeviceBuffers.
+def _address(x):
+    return x.addr if isinstance(x, DeviceBuffer) else x
+
+
+class _Call:
+    """a library function, its arguments but the stream, and what they point to"""
+
+    def __init__(self, name, args, keep):
+        self._fn, self._args, self._name, self._keep = getattr(lib(), name), args, name, keep
+
+    def run(self, stream=None):
+        rc = self._fn(*self._args, stream.h if stream else None)
+        if rc:
+            check(rc, self._name)
+
+
+class NormResidual(_Call):
+    """h_out = h + alpha a(gate) N_post(y), x = N_pre(h_out) on n rows of C (p8x_norm_residual). Row strides default to C;
+    ld_gate 0: one gate row for all."""
+
+    def __init__(self, n, C, h, y=None, h_out=None, x=None, y_dtype=F32, h_dtype=F32, x_dtype=F32, ldy=None, ldh=None, ldho=None, ldx=None,
+                 post=NORM_NONE, w_post=None, b_post=None, eps_post=1e-6, pre=NORM_RMS, w_pre=None, b_pre=None, eps_pre=1e-6,
+                 gate=None, gate_dtype=F32, ld_gate=None, gate_act=GATE_LINEAR, alpha=1.0):
+        a = NormArgs(n, C, _address(y), y_dtype, ldy or C, _address(h), h_dtype, ldh or C, _address(h_out), ldho or C, _address(x), x_dtype, ldx or C,
+                     post, _address(w_post), _address(b_post), eps_post, pre, _address(w_pre), _address(b_pre), eps_pre,
+                     _address(gate), gate_dtype, C if ld_gate is None else ld_gate, gate_act, alpha)
+        super().__init__("p8x_norm_residual", (ctypes.byref(a),), (a, y, h, h_out, x, w_post, b_post, w_pre, b_pre, gate))
+
+
+class KvCache:
+    """A key/value cache in the caller's memory (p8x_kv_cache): strides in elements; pages None: sequence s in page s."""
+
+    def __init__(self, dtype, n_seq, n_kv, head_dim, k, v, page_stride, head_stride, slot_stride, page_size, n_pages, len, max_len, pages=None,
+                 ld_pages=0):
+        self.n_seq, self.n_kv, self.head_dim, self.max_len = n_seq, n_kv, head_dim, max_len
+        self.c = KvCacheC(dtype, n_seq, n_kv, head_dim, _address(k), _address(v), page_stride, head_stride, slot_stride, page_size, n_pages,
+                          _address(pages), ld_pages, _address(len), max_len)
+        self._keep = (k, v, pages, len)
+
+
+def _drafts(cache, n_tokens, max_tokens, first, k=None, v=None, kv_dtype=F32, ld_kv=None, head_stride_kv=0, mask=None, n_heads=0, q=None,
+            q_dtype=F32, ld_q=None, head_stride_q=0, scale=1.0):
+    D = cache.head_dim
+    return DraftsC(n_tokens, max_tokens, _address(first), _address(k), _address(v), kv_dtype, cache.n_kv * D if ld_kv is None else ld_kv, head_stride_kv,
+                   _address(mask), n_heads, _address(q), q_dtype, n_heads * D if ld_q is None else ld_q, head_stride_q, scale)
+
+
+class AttnTree(_Call):
+    """Attention of drafted tokens over the cache and each other (p8x_attn_tree); drafts: the fields of p8x_drafts by
+    name. Without a workspace of the caller's it keeps one of its own."""
+
+    def __init__(self, cache, out, lse=None, ld_out=None, head_stride_out=0, workspace=None, workspace_bytes=0, **drafts):
+        d = _drafts(cache, **drafts)
+        if workspace is None:
+            workspace_bytes = lib().p8x_attn_workspace(ctypes.byref(cache.c), ctypes.byref(d))
+            if workspace_bytes:
+                workspace = DeviceBuffer(workspace_bytes)
+                workspace.fill(0)
+                synchronize()
+        super().__init__("p8x_attn_tree", (ctypes.byref(cache.c), ctypes.byref(d), _address(out), d.n_heads * cache.head_dim if ld_out is None else ld_out,
+                                           head_stride_out, _address(lse), _address(workspace), workspace_bytes), (cache, d, drafts, out, lse, workspace))
+
+
+class KvScore(_Call):
+    """Attention weight of the accepted tokens added to the slots' scores (p8x_kv_score)."""
+
+    def __init__(self, cache, lse, score, score_out=None, accept=None, decay=1.0, **drafts):
+        d = _drafts(cache, **drafts)
+        score_out = score if score_out is None else score_out
+        super().__init__("p8x_kv_score", (ctypes.byref(cache.c), ctypes.byref(d), _address(accept), _address(lse), decay, _address(score),
+                                          _address(score_out)), (cache, d, drafts, accept, lse, score, score_out))
+
+
+class KvAppend(_Call):
+    """Keys and values of accepted tokens into the cache (p8x_kv_append)."""
+
+    def __init__(self, cache, accept=None, at=None, pos=None, len_out=None, **drafts):
+        d = _drafts(cache, **drafts)
+        super().__init__("p8x_kv_append", (ctypes.byref(cache.c), ctypes.byref(d), _address(accept), _address(at), _address(pos), _address(len_out)),
+                         (cache, d, drafts, accept, at, pos, len_out))
+
+
+class KvEvict(_Call):
+    """The cache cut to a budget (p8x_kv_evict). Without a workspace of the caller's it keeps one of its own."""
+
+    def __init__(self, cache, budget, score, len_out, score_out=None, pos=None, pos_out=None, n_sink=0, n_recent=0, workspace=None,
+                 workspace_bytes=0):
+        if workspace is None:
+            workspace_bytes = lib().p8x_kv_evict_workspace(ctypes.byref(cache.c), budget)
+            workspace = DeviceBuffer(workspace_bytes)
+        a = EvictArgs(budget, n_sink, n_recent, _address(score), _address(score if score_out is None else score_out), _address(pos),
+                      _address(pos if pos_out is None else pos_out), _address(len_out), _address(workspace), workspace_bytes)
+        super().__init__("p8x_kv_evict", (ctypes.byref(cache.c), ctypes.byref(a)), (cache, a, score, score_out, pos, pos_out, len_out, workspace))
