@@ -85,6 +85,8 @@ struct AttnJob {
     float *part;       // two records a workgroup: rows x D sums, then rows m, rows l
     int rw, rt, least; // row waves of a workgroup; row tiles of a sequence at most; units a workgroup takes at least
     int split;         // unit: a tile; 0: a whole segment (no records)
+    int join;          // records are joined by a launch of their own
+    int nwg;
 };
 
 // the units (32-slot tiles) of sequence s: tokens, slots, row tiles, tiles
@@ -274,6 +276,94 @@ __device__ __forceinline__ uint4v draft8(const void *p, size_t at, int f32, int 
         o[e + 2] = to16(hi[2 * e], bf16) | (uint32_t)to16(hi[2 * e + 1], bf16) << 16;
     }
     return o;
+}
+
+__device__ __forceinline__ float2 load2_agent(const float *p) {
+    const uint64_t v = __hip_atomic_load((const uint64_t *)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return make_float2(__builtin_bit_cast(float, (uint32_t)v), __builtin_bit_cast(float, (uint32_t)(v >> 32)));
+}
+__device__ __forceinline__ void store2_agent(float *p, float a, float b) {
+    __hip_atomic_store((uint64_t *)p, (uint64_t)__builtin_bit_cast(uint32_t, b) << 32 | __builtin_bit_cast(uint32_t, a), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// A record: [row][D] sums, then [row] (m, l). Elements e .. e + 3 of row r over the np records of a segment, in order, eight
+// loads in flight at a time; AGENT: written in this launch by other workgroups.
+template <int D, bool AGENT>
+__device__ __forceinline__ void join_records(const float *part, size_t rec, int rows_wg, int p0, int np, int r, int e, float4v &v, float &m, float &l) {
+    m = -INFINITY, l = 0.0f, v = float4v{0, 0, 0, 0};
+    for (int b = 0; b < np; b += 8) {
+        float2 ml[8];
+        float4v x[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int p = min(b + k, np - 1);
+            const float *q = part + (2 * (size_t)(p0 + p) + (p == 0 ? 1 : 0)) * rec;
+            if constexpr (AGENT) {
+                ml[k] = load2_agent(q + (size_t)rows_wg * D + 2 * r);
+                const float2 a = load2_agent(q + (size_t)r * D + e), c = load2_agent(q + (size_t)r * D + e + 2);
+                x[k] = float4v{a.x, a.y, c.x, c.y};
+            } else {
+                ml[k] = *(const float2 *)(q + (size_t)rows_wg * D + 2 * r);
+                x[k] = *(const float4v *)(q + (size_t)r * D + e);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            if (b + k >= np) break;
+            const float mn = fmaxf(m, ml[k].x), mb = mn == -INFINITY ? 0.0f : mn;
+            const float f0 = exp2f(m - mb), f1 = exp2f(ml[k].x - mb);
+            m = mn;
+            l = l * f0 + ml[k].y * f1;
+            v = v * f0 + x[k] * f1;
+        }
+    }
+}
+
+template <int D, bool BF, bool QF>
+__device__ __forceinline__ void store_row(const AttnJob &J, int first, int h, int row, int e, float4v v, float m, float l) {
+    constexpr float bias = BF ? 0.0f : 7.0f;
+    v *= l == 0.0f ? 0.0f : 1.0f / l;
+    const int G = J.d.G, i = row / G, head = h * G + row - i * G;
+    const size_t at = (size_t)(first + i) * J.ldo + (size_t)head * J.hso + e;
+    if constexpr (QF) *(float4v *)((float *)J.out + at) = v;
+    else {
+        const uint2v p = {pack2<BF>(v[0], v[1]), pack2<BF>(v[2], v[3])};
+        *(uint2v *)((uint16_t *)J.out + at) = p;
+    }
+    if (e == 0 && J.lse) J.lse[(size_t)(first + i) * J.c.n_kv * G + head] = l == 0.0f ? -INFINITY : (m - bias + __log2f(l)) * kLn2;
+}
+
+// The records of split segments in a launch of their own: a thread four elements of a row.
+template <int D, bool BF, bool QF>
+__global__ __launch_bounds__(256) void k_attn_join(AttnJob J, int rows_wg) {
+    const int lane = threadIdx.x & 63, s = blockIdx.z / J.c.n_kv, h = blockIdx.z % J.c.n_kv, rt = blockIdx.y;
+    const int x4 = blockIdx.x * 256 + threadIdx.x, r = x4 / (D / 4), e = x4 % (D / 4) * 4;
+    int total = 0, base = 0;
+    for (int s0 = 0; s0 < J.c.n_seq; s0 += 64) {
+        int v = 0;
+        if (s0 + lane < J.c.n_seq) {
+            const SeqUnits u = seq_units(J, s0 + lane, rows_wg);
+            v = J.c.n_kv * u.rts * u.per_seg;
+        }
+        int b = s0 + lane < s ? v : 0;
+        if (J.c.n_seq > 1)
+            for (int o = 32; o; o >>= 1) {
+                v += __shfl_xor(v, o);
+                b += __shfl_xor(b, o);
+            }
+        else v = __builtin_amdgcn_readfirstlane(v);
+        total += v;
+        base += J.c.n_seq > 1 ? b : 0;
+    }
+    const int per = max(J.least, (total + J.nwg - 1) / J.nwg);
+    const SeqUnits q = seq_units(J, s, rows_wg);
+    if (rt >= q.rts || rt * rows_wg + r >= q.nt * J.d.G || r >= rows_wg) return;
+    const int sa = base + (h * q.rts + rt) * q.tiles, sb = sa + q.tiles, p0 = sa / per, np = (sb - 1) / per - p0 + 1;
+    if (np < 2) return;
+    float4v v;
+    float m, l;
+    join_records<D, false>(J.part, (size_t)rows_wg * (D + 2), rows_wg, p0, np, r, e, v, m, l);
+    store_row<D, BF, QF>(J, q.first, h, rt * rows_wg + r, e, v, m, l);
 }
 
 template <int D, bool BF, bool QF, int NT>
@@ -526,20 +616,6 @@ __global__ __launch_bounds__(64 * attn_waves(D)) void k_attn(AttnJob J) {
         const int p0 = sa / per, np = (sb - 1) / per - p0 + 1;   // the segment's workgroups p0 .. p0 + np - 1
         const size_t rec = (size_t)rows_wg * (D + 2);
         float *mine = whole ? nullptr : J.part + (2 * (size_t)wg + (sa < wg * per ? 0 : 1)) * rec;
-        auto store_out = [&](int r, int e, float4v v) {
-            const int i = (rt * rows_wg + r) / d.G;
-            const size_t at = (size_t)(q.first + i) * J.ldo + (size_t)(h * d.G + (rt * rows_wg + r) - i * d.G) * J.hso + e;
-            if constexpr (QF) *(float4v *)((float *)J.out + at) = v;
-            else {
-                const uint2v p = {pack2<BF>(v[0], v[1]), pack2<BF>(v[2], v[3])};
-                *(uint2v *)((uint16_t *)J.out + at) = p;
-            }
-        };
-        auto store_lse = [&](int r, float m, float l) {
-            if (!J.lse) return;
-            const int i = (rt * rows_wg + r) / d.G;
-            J.lse[(size_t)(q.first + i) * c.n_kv * d.G + h * d.G + (rt * rows_wg + r) - i * d.G] = l == 0.0f ? -INFINITY : (m - W::kBias + __log2f(l)) * kLn2;
-        };
         for (int x4 = threadIdx.x; x4 < here * (D / 4); x4 += 64 * kWaves) {
             const int r = x4 / (D / 4), e = x4 % (D / 4) * 4, rg = r / R16, rr = r % R16;
             float m = -INFINITY;
@@ -554,19 +630,17 @@ __global__ __launch_bounds__(64 * attn_waves(D)) void k_attn(AttnJob J) {
                 v += f * *(const float4v *)(sh + ((size_t)wv * R16 + rr) * LD + e);
             }
             if (whole) {
-                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-                store_out(r, e, v * inv);
-                if (e == 0) store_lse(r, m, l);
+                store_row<D, BF, QF>(J, q.first, h, rt * rows_wg + r, e, v, m, l);
+            } else if (J.join) {
+                *(float4v *)(mine + (size_t)r * D + e) = v;
+                if (e == 0) *(float2 *)(mine + (size_t)rows_wg * D + 2 * r) = make_float2(m, l);
             } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) __hip_atomic_store(mine + (size_t)r * D + e + i, v[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                if (e == 0) {
-                    __hip_atomic_store(mine + (size_t)rows_wg * D + r, m, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                    __hip_atomic_store(mine + (size_t)rows_wg * (D + 1) + r, l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                }
+                store2_agent(mine + (size_t)r * D + e, v[0], v[1]);
+                store2_agent(mine + (size_t)r * D + e + 2, v[2], v[3]);
+                if (e == 0) store2_agent(mine + (size_t)rows_wg * D + 2 * r, m, l);
             }
         }
-        if (!whole) {
+        if (!whole && !J.join) {
             // the segment's last workgroup adds the records in the workgroups' order
             unsigned *ctr = J.count + ((size_t)s * c.n_kv + h) * J.rt + rt;
             __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the wave's record stores complete before the arrival
@@ -577,26 +651,14 @@ __global__ __launch_bounds__(64 * attn_waves(D)) void k_attn(AttnJob J) {
                 if (last) __hip_atomic_store(ctr, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
             __syncthreads();
-            if (last) {
-                auto record = [&](int p) { return J.part + (2 * (size_t)(p0 + p) + (p == 0 ? 1 : 0)) * rec; };
+            if (last)
                 for (int x4 = threadIdx.x; x4 < here * (D / 4); x4 += 64 * kWaves) {
                     const int r = x4 / (D / 4), e = x4 % (D / 4) * 4;
-                    float m = -INFINITY;
-                    for (int p = 0; p < np; ++p) m = fmaxf(m, __hip_atomic_load(record(p) + (size_t)rows_wg * D + r, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-                    const float mb = m == -INFINITY ? 0.0f : m;
-                    float l = 0;
-                    float4v v = {0, 0, 0, 0};
-                    for (int p = 0; p < np; ++p) {
-                        const float *q0 = record(p);
-                        const float f = exp2f(__hip_atomic_load(q0 + (size_t)rows_wg * D + r, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) - mb);
-                        l += f * __hip_atomic_load(q0 + (size_t)rows_wg * (D + 1) + r, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) v[i] += f * __hip_atomic_load(q0 + (size_t)r * D + e + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                    }
-                    store_out(r, e, v * (l == 0.0f ? 0.0f : 1.0f / l));
-                    if (e == 0) store_lse(r, m, l);
+                    float4v v;
+                    float m, l;
+                    join_records<D, true>(J.part, rec, rows_wg, p0, np, r, e, v, m, l);
+                    store_row<D, BF, QF>(J, q.first, h, rt * rows_wg + r, e, v, m, l);
                 }
-            }
         }
         __syncthreads();   // sh and last are free again
     }
@@ -604,6 +666,7 @@ __global__ __launch_bounds__(64 * attn_waves(D)) void k_attn(AttnJob J) {
 
 // Rows a wave and row waves a workgroup: 16 rows while they hold all, else 32 (16 with queries of several parts or
 // wide rows, whose operands fill the registers).
+constexpr size_t kJoinBytes = 64 << 10;   // records of more bytes than this are joined by a launch of their own
 struct AttnPlan { int nt, rw, rows_wg, rt; size_t segs, rec_bytes, head_bytes; };
 static AttnPlan attn_plan(const KvDev &c, const DraftDev &d, int D) {
     const int kWaves = attn_waves(D);
@@ -626,21 +689,22 @@ size_t attn_workspace(const KvDev &c, const DraftDev &d, int D) {
 }
 
 template <int D, bool BF, bool QF, int NT>
-static int attn_run(const AttnJob &J, int nwg, hipStream_t st) {
+static int attn_run(const AttnJob &J, int rows_wg, hipStream_t st) {
     constexpr int kWaves = attn_waves(D), lds = kWaves * 16 * NT * (D + 4 + 2) * 4;
     static const hipError_t e = hipFuncSetAttribute((const void *)k_attn<D, BF, QF, NT>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e != hipSuccess) return hip_check(e, "p8x_attn_tree LDS");
-    k_attn<D, BF, QF, NT><<<nwg, 64 * kWaves, lds, st>>>(J);
+    k_attn<D, BF, QF, NT><<<J.nwg, 64 * kWaves, lds, st>>>(J);
+    if (J.join) k_attn_join<D, BF, QF><<<dim3((rows_wg * (D / 4) + 255) / 256, J.rt, J.c.n_seq * J.c.n_kv), 256, 0, st>>>(J, rows_wg);
     return hip_check(hipGetLastError(), "p8x_attn_tree launch");
 }
 
 template <int D>
-static int attn_types(const AttnJob &J, int nt, int nwg, hipStream_t st) {
+static int attn_types(const AttnJob &J, const AttnPlan &p, hipStream_t st) {
     const bool bf = J.c.bf16;
-    if (J.d.q_f32) return bf ? attn_run<D, true, true, 1>(J, nwg, st) : attn_run<D, false, true, 1>(J, nwg, st);
+    if (J.d.q_f32) return bf ? attn_run<D, true, true, 1>(J, p.rows_wg, st) : attn_run<D, false, true, 1>(J, p.rows_wg, st);
     if constexpr (D < 256)
-        if (nt == 2) return bf ? attn_run<D, true, false, 2>(J, nwg, st) : attn_run<D, false, false, 2>(J, nwg, st);
-    return bf ? attn_run<D, true, false, 1>(J, nwg, st) : attn_run<D, false, false, 1>(J, nwg, st);
+        if (p.nt == 2) return bf ? attn_run<D, true, false, 2>(J, p.rows_wg, st) : attn_run<D, false, false, 2>(J, p.rows_wg, st);
+    return bf ? attn_run<D, true, false, 1>(J, p.rows_wg, st) : attn_run<D, false, false, 1>(J, p.rows_wg, st);
 }
 
 int launch_attn_tree(const KvDev &c, const DraftDev &d, int D, void *out, size_t ldo, size_t hso, float *lse, void *ws, size_t ws_bytes,
@@ -649,7 +713,7 @@ int launch_attn_tree(const KvDev &c, const DraftDev &d, int D, void *out, size_t
     const size_t most = p.segs * ((size_t)(c.max_len + 31) / 32 + 2);   // units
     if (most >= (1u << 30)) return set_error(P8X_ERR_UNSUPPORTED, "p8x_attn_tree: %zu tiles of 32 slots (fewer than 2^30)", most);
     if (c.slot_stride >= (1u << 26)) return set_error(P8X_ERR_UNSUPPORTED, "p8x_attn_tree: slot_stride %zu (below 2^26)", c.slot_stride);
-    AttnJob J{c, d, out, ldo, hso, lse, (unsigned *)ws, (float *)((char *)ws + p.head_bytes), p.rw, p.rt, attn_waves(D) / p.rw, 1};
+    AttnJob J{c, d, out, ldo, hso, lse, (unsigned *)ws, (float *)((char *)ws + p.head_bytes), p.rw, p.rt, attn_waves(D) / p.rw, 1, 0, 0};
     const size_t room = ws_bytes > p.head_bytes ? (ws_bytes - p.head_bytes) / (2 * p.rec_bytes) : 0;   // workgroups with records
     int nwg = (int)std::min<size_t>(num_cus(), room);
     if (nwg < 16) {   // whole segments then
@@ -657,7 +721,11 @@ int launch_attn_tree(const KvDev &c, const DraftDev &d, int D, void *out, size_t
         J.split = 0, J.least = 1;
     }
     if (nwg >= 8) nwg = nwg / 8 * 8;
-    return D == 64 ? attn_types<64>(J, p.nt, nwg, st) : D == 128 ? attn_types<128>(J, p.nt, nwg, st) : attn_types<256>(J, p.nt, nwg, st);
+    J.nwg = nwg;
+    // records of a segment, about, that one workgroup would join
+    const size_t each = J.split ? nwg / p.segs * p.rec_bytes : 0;
+    J.join = each > kJoinBytes && p.segs / p.rt <= 65535;
+    return D == 64 ? attn_types<64>(J, p, st) : D == 128 ? attn_types<128>(J, p, st) : attn_types<256>(J, p, st);
 }
 
 // ---- scores -----------------------------------------------------------------------------------------------
