@@ -8,14 +8,6 @@
 
 namespace p8x {
 
-// 8 elements of a query or draft row as f32; drafts in f32 are rounded to the cache's type
-__device__ __forceinline__ void load8(const void *p, size_t i, bool f32, int bf16, bool round, float *o) {
-    for (int e = 0; e < 8; ++e) {
-        o[e] = f32 ? ((const float *)p)[i + e] : from16(((const uint16_t *)p)[i + e], bf16);
-        if (round) o[e] = from16(to16(o[e], bf16), bf16);
-    }
-}
-
 __device__ __forceinline__ uint64_t token_mask(const DraftDev &d, int tok, int i) {
     return d.mask ? d.mask[tok] : i == 63 ? ~0ull : (2ull << i) - 1;
 }
@@ -73,6 +65,36 @@ __device__ __forceinline__ void split8(const float *f, uint4v *o) {
 
 // waves of a workgroup, one of which a compute unit holds: 256 registers a lane, or 512 for rows of 256 elements
 __host__ __device__ constexpr int attn_waves(int D) { return D == 256 ? 4 : 8; }
+// A lane's pieces of an f32 query row, 8 elements at 32 k, for splitting: fp16 parts need the row scaled to 2^13 (the lanes
+// 16 apart hold the rest of the row). Returns the factor of a product, f with that power taken back out.
+template <int C, bool BF>
+__device__ __forceinline__ float load_split(const float *q, bool on, float f, float (&x)[C][8]) {
+    float mx = 0.0f;
+#pragma unroll
+    for (int k = 0; k < C; ++k) {
+        const float4v lo = on ? *(const float4v *)(q + 32 * k) : float4v{0, 0, 0, 0}, hi = on ? *(const float4v *)(q + 32 * k + 4) : float4v{0, 0, 0, 0};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            x[k][e] = lo[e];
+            x[k][e + 4] = hi[e];
+            mx = fmaxf(mx, fmaxf(fabsf(lo[e]), fabsf(hi[e])));
+        }
+    }
+    if constexpr (!BF) {
+        mx = fmaxf(mx, __shfl_xor(mx, 16));
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        const int ex = mx > 0.0f && mx < INFINITY ? 13 - (int)((__builtin_bit_cast(uint32_t, mx) >> 23) - 127) : 0;
+        const int e1 = min(ex, 100);   // in two steps: 2^ex may be beyond f32
+        const float s1 = ldexpf(1.0f, e1), s2 = ldexpf(1.0f, ex - e1);
+#pragma unroll
+        for (int k = 0; k < C; ++k)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[k][e] = x[k][e] * s1 * s2;
+        f = ldexpf(f, -ex);
+    }
+    return f;
+}
+
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kLazy = 8.0f;   // log2 of how far a weight may exceed 1 before its row's maximum moves
 
@@ -128,29 +150,13 @@ struct Wave {
             for (int t = 0; t < DV; ++t) o[a][t] = float4v{0, 0, 0, 0};
             if constexpr (QF) {
                 float f[C][8];
-                float mx = 0.0f;
-#pragma unroll
-                for (int k = 0; k < C; ++k) {
-                    const float4v lo = on ? *(const float4v *)((const float *)d.q + at + 32 * k) : float4v{0, 0, 0, 0};
-                    const float4v hi = on ? *(const float4v *)((const float *)d.q + at + 32 * k + 4) : float4v{0, 0, 0, 0};
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        f[k][e] = d.scale < 0 ? -lo[e] : lo[e];
-                        f[k][e + 4] = d.scale < 0 ? -hi[e] : hi[e];
-                        mx = fmaxf(mx, fmaxf(fabsf(lo[e]), fabsf(hi[e])));
-                    }
-                }
-                if constexpr (!BF) {
-                    mx = fmaxf(mx, __shfl_xor(mx, 16));
-                    mx = fmaxf(mx, __shfl_xor(mx, 32));
-                    const int ex = mx > 0.0f && mx < INFINITY ? 13 - (int)((__builtin_bit_cast(uint32_t, mx) >> 23) - 127) : 0;
-                    const int e1 = min(ex, 100), e2 = ex - e1;   // two steps: 2^ex may be beyond f32
-                    const float s1 = ldexpf(1.0f, e1), s2 = ldexpf(1.0f, e2);
+                c2[a] = load_split<C, BF>((const float *)d.q + at, on, d.scale < 0 ? -sc : sc, f);
+                if (d.scale < 0) {
+                    c2[a] = -c2[a];
 #pragma unroll
                     for (int k = 0; k < C; ++k)
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) f[k][e] = f[k][e] * s1 * s2;
-                    c2[a] = ldexpf(sc, -ex);
+                        for (int e = 0; e < 8; ++e) f[k][e] = -f[k][e];
                 }
 #pragma unroll
                 for (int k = 0; k < C; ++k) {
@@ -729,50 +735,187 @@ int launch_attn_tree(const KvDev &c, const DraftDev &d, int D, void *out, size_t
 }
 
 // ---- scores -----------------------------------------------------------------------------------------------
-// One thread a slot or accepted token of a key/value head.
-template <int D>
-__global__ __launch_bounds__(256) void k_score(KvDev c, DraftDev d, const uint64_t *accept, const float *lse, float decay, const float *score, float *score_out) {
-    const int s = blockIdx.z, h = blockIdx.y, j = blockIdx.x * 256 + threadIdx.x;
+// sum over the accepted tokens' rows of exp(scale q k - lse) per slot. S [row][slot] = Q K^T with K as the B operand (lane
+// n = slot) straight from memory, each slot's keys read by one wave once, and Q as A from LDS, where the workgroup
+// leaves its rows in operand order; a lane's four rows of every tile are added in place, the four lane groups at the end.
+constexpr int kScoreWaves = 4;
+// rows that LDS holds at a time; more of them take the slots again
+__host__ __device__ constexpr int score_rows(int D) { return D == 256 ? 32 : 64; }
+
+struct ScoreJob {
+    KvDev c;
+    DraftDev d;
+    const uint64_t *accept;
+    const float *lse, *score;
+    float *score_out;
+    float decay;
+};
+
+// token of accepted rank r
+__device__ __forceinline__ int nth_bit(uint64_t b, int r) {
+    for (; r; --r) b &= b - 1;
+    return __ffsll((unsigned long long)b) - 1;
+}
+
+template <int D, bool BF, bool QF>
+__global__ __launch_bounds__(64 * kScoreWaves) void k_score(ScoreJob J) {
+    constexpr int C = D / 32, QP = QF ? (BF ? 3 : 2) : 1, RB = score_rows(D);
+    __shared__ uint4v sq[RB / 16][QP][C][64];
+    __shared__ float4v sl[RB / 4], sc[RB / 4];   // lse and factor of a product, by row (rows that are not there: 0)
+    __shared__ uint64_t see[RB];
+    const KvDev &c = J.c;
+    const DraftDev &d = J.d;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, ln = lane & 15;
+    const int s = blockIdx.z, h = blockIdx.y;
     int first = 0;
-    const int nt = d.n_tokens ? seq_tokens(d, s, first) : 0, n = seq_len(c, s);
-    const uint64_t all = nt >= 64 ? ~0ull : (1ull << nt) - 1, acc = accept ? accept[s] & all : all;
-    const int cnt = __popcll(acc);
-    if (j >= min(n + cnt, c.max_len)) return;
-    int tj = -1;   // the accepted token that becomes slot j
-    if (j >= n) {
-        uint64_t b = acc;
-        for (int r = j - n; r; --r) b &= b - 1;
-        tj = __ffsll((unsigned long long)b) - 1;
-    }
-    const int64_t at = tj < 0 ? slot_offset(c, s, j) : 0;
-    float sum = 0;
-    if (at >= 0)
-        for (uint64_t b = acc; b; b &= b - 1) {
-            const int i = __ffsll((unsigned long long)b) - 1, tok = first + i;
-            if (tj >= 0 && !(token_mask(d, tok, i) >> tj & 1)) continue;
-            for (int g = 0; g < d.G; ++g) {
-                const int head = h * d.G + g;
-                float a = 0;
-                for (int k = 0; k < D; k += 8) {
-                    float q[8], r[8];
-                    load8(d.q, (size_t)tok * d.ld_q + head * d.hs_q + k, d.q_f32, c.bf16, false, q);
-                    if (tj < 0) load8(c.k, at + h * c.head_stride + k, false, c.bf16, false, r);
-                    else load8(d.k, (size_t)(first + tj) * d.ld_kv + h * d.hs_kv + k, d.kv_f32, c.bf16, d.kv_f32, r);
-                    for (int u = 0; u < 8; ++u) a = fmaf(q[u], r[u], a);
-                }
-                sum += expf(a * d.scale - lse[(size_t)tok * c.n_kv * d.G + head]);
+    const int nt = __builtin_amdgcn_readfirstlane(d.n_tokens ? seq_tokens(d, s, first) : 0), n = __builtin_amdgcn_readfirstlane(seq_len(c, s));
+    const uint64_t all = nt >= 64 ? ~0ull : (1ull << nt) - 1, acc = J.accept ? J.accept[s] & all : all;
+    const int cnt = __popcll(acc), rows = cnt * d.G;
+    // the workgroup's tiles of 32 slots; the drafts' are the last ones
+    const int ctx = (n + 31) / 32, tiles = ctx + (min(cnt, c.max_len - n) + 31) / 32, per = (tiles + (int)gridDim.x - 1) / (int)gridDim.x;
+    const int t0 = blockIdx.x * per, t1 = min(tiles, t0 + per);
+    if (t0 >= t1) return;
+    const size_t base = ((size_t)s * c.n_kv + h) * c.max_len;
+    const uint16_t *kp = c.k + (size_t)h * c.head_stride;
+    const uint32_t ko = (uint32_t)ln * (uint32_t)c.slot_stride + 8 * g;
+
+    int rb = 0;
+    do {   // once without rows: scores decay
+        const int rt = min(RB / 16, (rows - rb + 15) / 16);
+        if (rb) __syncthreads();
+        for (int r = threadIdx.x; r < 16 * rt; r += 64 * kScoreWaves) {
+            const int row = rb + r, i = row / d.G;
+            see[r] = 0;
+            ((float *)sl)[r] = 0.0f;
+            if (row < rows) {
+                const int ti = nth_bit(acc, i);
+                see[r] = token_mask(d, first + ti, ti);
+                ((float *)sl)[r] = J.lse[(size_t)(first + ti) * c.n_kv * d.G + h * d.G + row - i * d.G];
             }
         }
-    const size_t o = ((size_t)s * c.n_kv + h) * c.max_len + j;
-    score_out[o] = tj < 0 ? decay * score[o] + sum : sum;
+        for (int r = wave; r < rt; r += kScoreWaves) {
+            const int row = rb + 16 * r + ln, i = row / d.G;
+            const bool on = row < rows;
+            const size_t at = on ? (size_t)(first + nth_bit(acc, i)) * d.ld_q + (size_t)(h * d.G + row - i * d.G) * d.hs_q + 8 * g : 0;
+            float f = d.scale;
+            if constexpr (QF) {
+                float x[C][8];
+                f = load_split<C, BF>((const float *)d.q + at, on, f, x);
+#pragma unroll
+                for (int k = 0; k < C; ++k) {
+                    uint4v p[QP];
+                    split8<BF, QP>(x[k], p);
+#pragma unroll
+                    for (int u = 0; u < QP; ++u) sq[r][u][k][lane] = p[u];
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < C; ++k) sq[r][0][k][lane] = on ? *(const uint4v *)((const uint16_t *)d.q + at + 32 * k) : uint4v{0, 0, 0, 0};
+            }
+            if (g == 0) ((float *)sc)[16 * r + ln] = f;
+        }
+        __syncthreads();
+
+        uint4v kf[2][C];
+        // the tile's weights, summed over the rows: lane l < 32 has slot l's. hide: bit i of byte t set where row 4 g + i of
+        // the row tile does not see the lane's slot of half t
+        auto sum_rows = [&](bool draft, int tj0, int tj1) {
+            float w0 = 0.0f, w1 = 0.0f;
+            for (int r = 0; r < rt; ++r) {
+                const float4v l = sl[4 * r + g], f = sc[4 * r + g];
+                float4v s0 = {0, 0, 0, 0}, s1 = {0, 0, 0, 0};
+#pragma unroll
+                for (int u = QP - 1; u >= 0; --u)
+#pragma unroll
+                    for (int k = 0; k < C; ++k) {
+                        const uint4v q = sq[r][u][k][lane];
+                        s0 = mfma<BF>(q, kf[0][k], s0);
+                        s1 = mfma<BF>(q, kf[1][k], s1);
+                    }
+                const int left = rows - rb - 16 * r - 4 * g;   // rows of the lane's four that are there
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float e0 = __builtin_amdgcn_exp2f(fmaf(s0[i], f[i], -l[i]) * kLog2e), e1 = __builtin_amdgcn_exp2f(fmaf(s1[i], f[i], -l[i]) * kLog2e);
+                    if (draft) {
+                        const uint64_t m = see[16 * r + 4 * g + i];
+                        if (!(m >> tj0 & 1)) e0 = 0.0f;
+                        if (!(m >> tj1 & 1)) e1 = 0.0f;
+                    }
+                    w0 += i < left ? e0 : 0.0f;
+                    w1 += i < left ? e1 : 0.0f;
+                }
+            }
+            w0 += __shfl_xor(w0, 16);
+            w0 += __shfl_xor(w0, 32);
+            w1 += __shfl_xor(w1, 16);
+            w1 += __shfl_xor(w1, 32);
+            return lane < 16 ? w0 : w1;
+        };
+        auto put = [&](int slot, int end, bool old, float w, float before) {
+            if (lane < 32 && slot + lane < end) {
+                float *o = J.score_out + base + slot + lane;
+                *o = rb ? *o + w : old ? J.decay * before + w : w;
+            }
+        };
+
+        for (int tb = t0 + wave; tb < min(t1, ctx); tb += 32 * kScoreWaves) {
+            // offsets of the wave's next 64 halves, a lane each
+            int64_t off = -1;
+            {
+                const int t = tb + kScoreWaves * (lane >> 1), slot = 32 * t + 16 * (lane & 1);
+                if (t < min(t1, ctx) && slot < n) off = slot_offset(c, s, slot);
+            }
+            const int lo = (int)off, hi = (int)(off >> 32), many = min(32, (min(t1, ctx) - tb + kScoreWaves - 1) / kScoreWaves);
+            auto half = [&](int i) { return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, i) << 32 | (uint32_t)__builtin_amdgcn_readlane(lo, i)); };
+            for (int i = 0; i < many; ++i) {
+                const int slot = 32 * (tb + kScoreWaves * i);
+                const int64_t h0 = half(2 * i), h1 = half(2 * i + 1);
+                const bool on0 = h0 >= 0 && slot + ln < n, on1 = h1 >= 0 && slot + 16 + ln < n;
+                const float before = lane < 32 && slot + lane < n && !rb ? J.score[base + slot + lane] : 0.0f;
+#pragma unroll
+                for (int k = 0; k < C; ++k) {
+                    kf[0][k] = on0 ? *(const uint4v *)(kp + h0 + ko + 32 * k) : uint4v{0, 0, 0, 0};
+                    kf[1][k] = on1 ? *(const uint4v *)(kp + h1 + ko + 32 * k) : uint4v{0, 0, 0, 0};
+                }
+                float w = rt > 0 ? sum_rows(false, 0, 0) : 0.0f;
+                if ((lane < 16 ? h0 : h1) < 0) w = 0.0f;
+                put(slot, n, true, w, before);
+            }
+        }
+        for (int t = max(t0, ctx) + wave; t < t1; t += kScoreWaves) {   // accepted tokens
+            const int r0 = 32 * (t - ctx), j0 = r0 + ln < cnt ? nth_bit(acc, r0 + ln) : 0, j1 = r0 + 16 + ln < cnt ? nth_bit(acc, r0 + 16 + ln) : 0;
+#pragma unroll
+            for (int k = 0; k < C; ++k) {
+                kf[0][k] = draft8(d.k, (size_t)(first + j0) * d.ld_kv + (size_t)h * d.hs_kv + 32 * k + 8 * g, d.kv_f32, BF);
+                kf[1][k] = draft8(d.k, (size_t)(first + j1) * d.ld_kv + (size_t)h * d.hs_kv + 32 * k + 8 * g, d.kv_f32, BF);
+            }
+            put(n + r0, min(n + cnt, c.max_len), false, sum_rows(true, j0, j1), 0.0f);
+        }
+        rb += RB;
+    } while (rb < rows);
+}
+
+template <int D>
+static void score_types(const ScoreJob &J, dim3 grid, hipStream_t st) {
+    if (J.d.q_f32 && J.d.n_tokens) {
+        if (J.c.bf16) k_score<D, true, true><<<grid, 64 * kScoreWaves, 0, st>>>(J);
+        else k_score<D, false, true><<<grid, 64 * kScoreWaves, 0, st>>>(J);
+    } else {
+        if (J.c.bf16) k_score<D, true, false><<<grid, 64 * kScoreWaves, 0, st>>>(J);
+        else k_score<D, false, false><<<grid, 64 * kScoreWaves, 0, st>>>(J);
+    }
 }
 
 int launch_kv_score(const KvDev &c, const DraftDev &d, int D, const uint64_t *accept, const float *lse, float decay, const float *score,
                     float *score_out, hipStream_t st) {
-    const dim3 grid((c.max_len + 255) / 256, c.n_kv, c.n_seq);
-    if (D == 64) k_score<64><<<grid, 256, 0, st>>>(c, d, accept, lse, decay, score, score_out);
-    else if (D == 128) k_score<128><<<grid, 256, 0, st>>>(c, d, accept, lse, decay, score, score_out);
-    else k_score<256><<<grid, 256, 0, st>>>(c, d, accept, lse, decay, score, score_out);
+    if (c.slot_stride >= (1u << 26)) return set_error(P8X_ERR_UNSUPPORTED, "p8x_kv_score: slot_stride %zu (below 2^26)", c.slot_stride);
+    const ScoreJob J{c, d, accept, lse, score, score_out, decay};
+    const int64_t heads = (int64_t)c.n_seq * c.n_kv, tiles = (c.max_len + 31) / 32 + 2;
+    const int nb = (int)std::max<int64_t>(1, std::min<int64_t>((tiles + kScoreWaves - 1) / kScoreWaves, (4 * num_cus() + heads - 1) / heads));
+    const dim3 grid(nb, c.n_kv, c.n_seq);
+    if (D == 64) score_types<64>(J, grid, st);
+    else if (D == 128) score_types<128>(J, grid, st);
+    else score_types<256>(J, grid, st);
     return hip_check(hipGetLastError(), "p8x_kv_score launch");
 }
 
