@@ -1,102 +1,37 @@
-// p8x_attn.hip -- attention of drafted tokens over the cache and each other (p8x_attn_tree), and the attention weight
-// that accepted tokens gave (p8x_kv_score).
-#include <hip/hip_runtime.h>
-
-#include <algorithm>
-
-#include "p8x_kv.h"
-
-namespace p8x {
-
-__device__ __forceinline__ uint64_t token_mask(const DraftDev &d, int tok, int i) {
-    return d.mask ? d.mask[tok] : i == 63 ? ~0ull : (2ull << i) - 1;
-}
-
-// ---- attention ----------------------------------------------------------------------------------------------
+// p8x_attn.hip -- attention of drafted tokens over the cache and each other (p8x_attn_tree).
+//
 // Rows: the (token, head of the group) pairs of a sequence and key/value head, token-major; they share K and V. A wave
 // multiplies tiles of 32 slots with its 16 NT rows on v_mfma_f32_16x16x32, transposed throughout so that nothing passes
 // through LDS between the two products:
 //   S^T [slot][row] = K Q^T: A = K (lane m = slot, 8 elements of the row at 8 (lane / 16)), B = Q, kept in registers;
 //   its result has, in lane (row, g), slots 4 g + i of each 16: the weights p in that place are, as they are, the B operand
 //   of O^T [element][row] = V^T P^T when the operand's k index 8 g + j stands for slot 4 g + j (j < 4) or 16 + 4 g + j - 4.
-//   A = V^T: lane (m, g) loads D / 16 elements of its group's 8 slots and transposes them in registers (one v_perm a
-//   dword); output tile t's row m then is element (D / 16) m + t.
+//   A = V^T: from memory, lane (m, g) takes D / 16 elements of its group's 8 slots and transposes them in registers (one
+//   v_perm a dword), output tile t's row m then is element (D / 16) m + t; from LDS, ds_read_b64_tr_b16 transposes blocks
+//   of 4 slots by 16 elements, and row m is element 16 t + m.
 // Softmax: the running maximum m of a row only moves when a score exceeds it by 2^8 in the weight, seen by each lane for
 // itself, so that the usual tile needs no exchange between lanes and no rescaling; sums l stay in their lanes until the
-// end. Weights stand relative to m, times 2^kBias for fp16 (subnormals).
-typedef _Float16 half8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bhalf8 __attribute__((ext_vector_type(8)));
-typedef float float4v __attribute__((ext_vector_type(4)));
-typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
-typedef uint32_t uint2v __attribute__((ext_vector_type(2)));
+// end. Weights stand relative to m, times 2^7 for fp16 (subnormals), and enter the product as two 16-bit parts (three for
+// f32 queries on a bf16 cache), so that their rounding does not show in out.
+//
+// Work: the 32-slot tiles of all (sequence, head, row tile) segments in a row, an equal share for each of one workgroup a
+// compute unit. Where the shares can be cut at the segments' ends without more workgroups or longer shares they are (each
+// segment that a workgroup visits costs it about 8 us of latency: queries, sums through LDS, records); else a share may
+// span segments. A segment of several workgroups leaves records (sums, maximum, sum of weights) that the last of them
+// joins in order, or, where they are many, a second launch.
+#include <hip/hip_runtime.h>
 
-template <bool BF>
-__device__ __forceinline__ float4v mfma(uint4v a, uint4v b, float4v c) {
-    if constexpr (BF) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bhalf8, a), __builtin_bit_cast(bhalf8, b), c, 0, 0, 0);
-    else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
-}
-template <bool BF>
-__device__ __forceinline__ uint32_t pack2(float x, float y) {
-    if constexpr (BF) return (uint32_t)to_bf16(x) | (uint32_t)to_bf16(y) << 16;
-    else return (uint32_t)to_f16(x) | (uint32_t)to_f16(y) << 16;
-}
-template <bool BF>
-__device__ __forceinline__ float part_lo(uint32_t w) { return BF ? __builtin_bit_cast(float, w << 16) : from_f16((uint16_t)w); }
-template <bool BF>
-__device__ __forceinline__ float part_hi(uint32_t w) { return BF ? __builtin_bit_cast(float, w & 0xFFFF0000u) : from_f16((uint16_t)(w >> 16)); }
+#include <algorithm>
 
-// 8 f32 as N operands of 16 bits that sum to them: N x 11 (fp16) or N x 8 (bf16) bits
-template <bool BF, int N>
-__device__ __forceinline__ void split8(const float *f, uint4v *o) {
-    float r[8];
-    for (int e = 0; e < 8; ++e) r[e] = f[e];
-#pragma unroll
-    for (int n = 0; n < N; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const uint32_t w = pack2<BF>(r[2 * e], r[2 * e + 1]);
-            o[n][e] = w;
-            if (n + 1 < N) {
-                r[2 * e] -= part_lo<BF>(w);
-                r[2 * e + 1] -= part_hi<BF>(w);
-            }
-        }
-}
+#include "p8x_attn.h"
+
+namespace p8x {
 
 // waves of a workgroup, one of which a compute unit holds: 256 registers a lane, or 512 for rows of 256 elements
 __host__ __device__ constexpr int attn_waves(int D) { return D == 256 ? 4 : 8; }
-// A lane's pieces of an f32 query row, 8 elements at 32 k, for splitting: fp16 parts need the row scaled to 2^13 (the lanes
-// 16 apart hold the rest of the row). Returns the factor of a product, f with that power taken back out.
-template <int C, bool BF>
-__device__ __forceinline__ float load_split(const float *q, bool on, float f, float (&x)[C][8]) {
-    float mx = 0.0f;
-#pragma unroll
-    for (int k = 0; k < C; ++k) {
-        const float4v lo = on ? *(const float4v *)(q + 32 * k) : float4v{0, 0, 0, 0}, hi = on ? *(const float4v *)(q + 32 * k + 4) : float4v{0, 0, 0, 0};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            x[k][e] = lo[e];
-            x[k][e + 4] = hi[e];
-            mx = fmaxf(mx, fmaxf(fabsf(lo[e]), fabsf(hi[e])));
-        }
-    }
-    if constexpr (!BF) {
-        mx = fmaxf(mx, __shfl_xor(mx, 16));
-        mx = fmaxf(mx, __shfl_xor(mx, 32));
-        const int ex = mx > 0.0f && mx < INFINITY ? 13 - (int)((__builtin_bit_cast(uint32_t, mx) >> 23) - 127) : 0;
-        const int e1 = min(ex, 100);   // in two steps: 2^ex may be beyond f32
-        const float s1 = ldexpf(1.0f, e1), s2 = ldexpf(1.0f, ex - e1);
-#pragma unroll
-        for (int k = 0; k < C; ++k)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[k][e] = x[k][e] * s1 * s2;
-        f = ldexpf(f, -ex);
-    }
-    return f;
-}
-
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kLazy = 8.0f;   // log2 of how far a weight may exceed 1 before its row's maximum moves
+// tiles that a workgroup's waves share through LDS at a time
+__host__ __device__ constexpr int stage_tiles(int D) { return D == 256 ? 1 : 2; }
 
 struct AttnJob {
     KvDev c;
@@ -104,28 +39,75 @@ struct AttnJob {
     void *out; size_t ldo, hso;
     float *lse;
     unsigned *count;   // arrivals of a segment's workgroups, 0 between calls
-    float *part;       // two records a workgroup: rows x D sums, then rows m, rows l
+    float *part;       // two records a workgroup: rows x D sums, then rows x (m, l)
     int rw, rt, least; // row waves of a workgroup; row tiles of a sequence at most; units a workgroup takes at least
     int split;         // unit: a tile; 0: a whole segment (no records)
     int join;          // records are joined by a launch of their own
     int nwg;
 };
 
-// the units (32-slot tiles) of sequence s: tokens, slots, row tiles, tiles
-struct SeqUnits { int nt, n, first, rts, tiles, per_seg; };
-__device__ __forceinline__ SeqUnits seq_units(const AttnJob &J, int s, int rows_wg) {
-    SeqUnits u;
-    u.nt = seq_tokens(J.d, s, u.first);
-    u.n = seq_len(J.c, s);
-    u.rts = (u.nt * J.d.G + rows_wg - 1) / rows_wg;
-    u.tiles = u.nt ? (u.n + 31) / 32 + (u.nt + 31) / 32 : 0;
-    u.per_seg = J.split ? u.tiles : u.nt ? 1 : 0;
-    return u;
+struct Seq { int nt, n, first, rts, tiles; };   // tokens, slots, first token's row, row tiles, tiles of slots and drafts
+__device__ __forceinline__ Seq seq_of(const AttnJob &J, int s, int rows_wg) {
+    Seq q;
+    q.nt = seq_tokens(J.d, s, q.first);
+    q.n = seq_len(J.c, s);
+    q.rts = (q.nt * J.d.G + rows_wg - 1) / rows_wg;
+    q.tiles = q.nt ? (q.n + 31) / 32 + (q.nt + 31) / 32 : 0;
+    return q;
 }
 
-template <int D, bool BF, bool QF, int NT>
+__device__ __forceinline__ int wave_sum(int v) {
+    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+    return __builtin_amdgcn_readfirstlane(v);
+}
+
+// How the tiles are shared out: `per` units a workgroup, units of a segment of `tiles` tiles. The same in every wave.
+struct Shares {
+    int per, aligned, split, total;
+    __device__ __forceinline__ int units(int tiles) const { return !split ? tiles > 0 : aligned ? (tiles + per - 1) / per * per : tiles; }
+};
+__device__ __forceinline__ Shares share_out(const AttnJob &J, int rows_wg) {
+    const int lane = threadIdx.x & 63, n_seq = J.c.n_seq;
+    // f(tiles) summed over all segments
+    auto over = [&](auto f) {
+        int t = 0;
+        for (int s0 = 0; s0 < n_seq; s0 += 64) {
+            int v = 0;
+            if (s0 + lane < n_seq) {
+                const Seq q = seq_of(J, s0 + lane, rows_wg);
+                v = J.c.n_kv * q.rts * f(q.tiles);
+            }
+            t += n_seq > 1 ? wave_sum(v) : __builtin_amdgcn_readfirstlane(v);
+        }
+        return t;
+    };
+    Shares h;
+    h.split = J.split;
+    h.aligned = 0;
+    if (!J.split) {
+        h.total = over([](int t) { return t > 0 ? 1 : 0; });
+        h.per = max(1, (h.total + J.nwg - 1) / J.nwg);
+        return h;
+    }
+    h.total = over([](int t) { return t; });
+    h.per = max(J.least, (h.total + J.nwg - 1) / J.nwg);
+    for (int k = 0; k < 2; ++k) {   // shares cut at segments' ends, of this length or a sixteenth more
+        const int per = k ? h.per + (h.per + 15) / 16 : h.per;
+        const int parts = over([&](int t) { return (t + per - 1) / per; });
+        if (parts <= J.nwg) {
+            h.per = per;
+            h.aligned = 1;
+            h.total = parts * per;
+            break;
+        }
+    }
+    return h;
+}
+
+template <int D, bool BF, bool QF, int NT, bool SHARE>
 struct Wave {
     static constexpr int C = D / 32, DV = D / 16, VW = DV / 2;       // K operands a row; elements and dwords of V a lane and slot
+    static constexpr int PC = D / 8, KP = PC + 1, VP = PC + 2;      // 16-byte pieces of a row; of one of K and V in LDS: the rows of a read in other banks
     static constexpr int QP = QF ? (BF ? 3 : 2) : 1, PP = QF && BF ? 3 : 2;   // 16-bit parts of a query and of a weight
     static constexpr float kBias = BF ? 0.0f : 7.0f;
     uint4v q[NT][QP][C];
@@ -134,7 +116,7 @@ struct Wave {
     uint4v kf[2][C];
     uint32_t vf[8][VW];
 
-    // the lane's rows' queries; f32 ones scaled to 2^13 (fp16 parts), the power put into c2
+    // the lane's rows' queries; a negative scale's sign goes into them
     __device__ __forceinline__ void load_q(const DraftDev &d, int first, int h, int row0, int rows, int lane) {
         const float sc = fabsf(d.scale) * kLog2e;
 #pragma unroll
@@ -150,17 +132,13 @@ struct Wave {
             for (int t = 0; t < DV; ++t) o[a][t] = float4v{0, 0, 0, 0};
             if constexpr (QF) {
                 float f[C][8];
-                c2[a] = load_split<C, BF>((const float *)d.q + at, on, d.scale < 0 ? -sc : sc, f);
-                if (d.scale < 0) {
-                    c2[a] = -c2[a];
-#pragma unroll
-                    for (int k = 0; k < C; ++k)
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) f[k][e] = -f[k][e];
-                }
+                c2[a] = load_split<C, BF>((const float *)d.q + at, on, sc, f);
 #pragma unroll
                 for (int k = 0; k < C; ++k) {
                     uint4v p[QP];
+                    if (d.scale < 0)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) f[k][e] = -f[k][e];
                     split8<BF, QP>(f[k], p);
 #pragma unroll
                     for (int n = 0; n < QP; ++n) q[a][n][k] = p[n];
@@ -198,12 +176,15 @@ struct Wave {
             load_v1(v + h1 + vo + j * ss, vf[j + 4]);
         }
     }
-
-    __device__ __forceinline__ void qk(float (&x)[NT][8]) {
+    // k: the lane's piece of a tile in LDS (SHARE), else K is in its registers
+    __device__ __forceinline__ void qk(float (&x)[NT][8], const uint4v *k) {
 #pragma unroll
-        for (int a = 0; a < NT; ++a)
+        for (int t = 0; t < 2; ++t) {
+            if constexpr (SHARE)
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
+                for (int c = 0; c < C; ++c) kf[t][c] = k[16 * t * KP + 4 * c];
+#pragma unroll
+            for (int a = 0; a < NT; ++a) {
                 float4v s = {0, 0, 0, 0};
 #pragma unroll
                 for (int n = QP - 1; n >= 0; --n)   // small parts first
@@ -212,15 +193,18 @@ struct Wave {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) x[a][4 * t + i] = s[i];
             }
+        }
     }
 
+    // (NaN propagates; fmaxf would quiet each operand first, an instruction apiece)
+    static __device__ __forceinline__ float top(float a, float b) { return __builtin_elementwise_maximum(a, b); }
     // scores to weights: x[a][j] of slot j of the lane's eight (-inf: hidden)
     __device__ __forceinline__ void softmax(float (&x)[NT][8]) {
         float mx[NT];
         bool move = false;
 #pragma unroll
         for (int a = 0; a < NT; ++a) {
-            mx[a] = fmaxf(fmaxf(fmaxf(x[a][0], x[a][1]), fmaxf(x[a][2], x[a][3])), fmaxf(fmaxf(x[a][4], x[a][5]), fmaxf(x[a][6], x[a][7]))) * c2[a];
+            mx[a] = top(top(top(top(x[a][0], x[a][1]), x[a][2]), top(x[a][3], x[a][4])), top(top(x[a][5], x[a][6]), x[a][7])) * c2[a];
             move |= mx[a] > m[a] + kLazy;
         }
         if (__any(move)) {
@@ -249,18 +233,47 @@ struct Wave {
         }
     }
 
-    __device__ __forceinline__ void pv(const float (&x)[NT][8]) {
-        uint4v p[NT][PP];
+    // the weights' parts; of two fp16 parts the first may be rounded toward zero, the second holds what is left
+    __device__ __forceinline__ void parts(const float *x, uint4v *p) {
+        if constexpr (!BF && PP == 2 && !QF) {
+            float minus1 = -1.0f;
+            __asm__("" : "+s"(minus1));   // not known to be -1: x - hi is one v_fma_mix, not a conversion and a subtraction
 #pragma unroll
-        for (int a = 0; a < NT; ++a) split8<BF, PP>(x[a], p[a]);
-#pragma unroll
-        for (int w = 0; w < VW; ++w) {
-            uint4v e0, e1;
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x[2 * e], x[2 * e + 1]));
+                p[0][e] = w;
+                p[1][e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(fmaf(part_lo<BF>(w), minus1, x[2 * e]), fmaf(part_hi<BF>(w), minus1, x[2 * e + 1])));
+            }
+        } else {
+            split8<BF, PP>(x, p);
+        }
+    }
+
+    // V^T operands of output tiles 2 w and 2 w + 1; v: the lane's piece of a tile in LDS (SHARE)
+    __device__ __forceinline__ void operands(int w, const uint16_t *v, uint4v &e0, uint4v &e1) {
+        if constexpr (SHARE) {
+            typedef short s4 __attribute__((ext_vector_type(4)));
+            auto tr = [&](int at) { return __builtin_bit_cast(uint2v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)(v + at))); };
+            const uint2v a = tr(32 * w), b = tr(32 * w + 16 * 8 * VP), c = tr(32 * w + 16), d = tr(32 * w + 16 + 16 * 8 * VP);
+            e0 = uint4v{a[0], a[1], b[0], b[1]};
+            e1 = uint4v{c[0], c[1], d[0], d[1]};
+        } else {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 e0[j] = __builtin_amdgcn_perm(vf[2 * j + 1][w], vf[2 * j][w], 0x05040100u);
                 e1[j] = __builtin_amdgcn_perm(vf[2 * j + 1][w], vf[2 * j][w], 0x07060302u);
             }
+        }
+    }
+
+    __device__ __forceinline__ void pv(const float (&x)[NT][8], const uint16_t *v) {
+        uint4v p[NT][PP];
+#pragma unroll
+        for (int a = 0; a < NT; ++a) parts(x[a], p[a]);
+#pragma unroll
+        for (int w = 0; w < VW; ++w) {
+            uint4v e0, e1;
+            operands(w, v, e0, e1);
 #pragma unroll
             for (int a = 0; a < NT; ++a)
 #pragma unroll
@@ -270,18 +283,66 @@ struct Wave {
                 }
         }
     }
+    __device__ __forceinline__ void tile(float (&x)[NT][8], const uint4v *k, const uint16_t *v) {
+        qk(x, k);
+        softmax(x);
+        pv(x, v);
+    }
+    // A masked tile (rows that are not there: zeros): see[a] bit j = slot j of the 32 is seen by the lane's row.
+    __device__ __forceinline__ void masked(float (&x)[NT][8], const uint4v *k, const uint16_t *v, const uint32_t (&see)[NT], int lane) {
+        qk(x, k);
+#pragma unroll
+        for (int a = 0; a < NT; ++a) {
+            const uint32_t lo = see[a] >> (4 * (lane >> 4)), hi = lo >> 16;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (!((j < 4 ? lo >> j : hi >> (j - 4)) & 1)) x[a][j] = -INFINITY;
+        }
+        softmax(x);
+        pv(x, v);
+    }
+    // A drafted token's infinities and NaN, which must not meet the zero weight of a row that does not see the token, are
+    // zeros in the product; here they are added to the rows that do. odd: the tokens of the tile (from row tok0 on) that have any.
+    __device__ __forceinline__ void add_odd(uint32_t odd, const uint32_t (&see)[NT], const DraftDev &d, int tok0, int h, int lane) {
+        const int g = lane >> 4;
+        for (; odd; odd &= odd - 1) {
+            const int j = __ffs(odd) - 1;
+            const size_t at = (size_t)(tok0 + j) * d.ld_kv + (size_t)h * d.hs_kv;
+#pragma unroll 1
+            for (int t = 0; t < DV; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const size_t e = at + (SHARE ? 16 * t + 4 * g + i : DV * (4 * g + i) + t);
+                    const float v = d.kv_f32 ? from16(to16(((const float *)d.v)[e], BF), BF) : from16(((const uint16_t *)d.v)[e], BF);
+#pragma unroll
+                    for (int a = 0; a < NT; ++a) {
+                        const float put = !(v - v == 0.0f) && (see[a] >> j & 1) ? v : 0.0f;
+#pragma unroll
+                        for (int k = 0; k < DV; ++k) o[a][k][i] += k == t ? put : 0.0f;   // (constant indices keep o in registers)
+                    }
+                }
+        }
+    }
 };
 
-// 8 elements of a draft row as the cache holds them
-__device__ __forceinline__ uint4v draft8(const void *p, size_t at, int f32, int bf16) {
-    if (!f32) return *(const uint4v *)((const uint16_t *)p + at);
-    const float4v lo = *(const float4v *)((const float *)p + at), hi = *(const float4v *)((const float *)p + at + 4);
-    uint4v o;
-    for (int e = 0; e < 2; ++e) {
-        o[e] = to16(lo[2 * e], bf16) | (uint32_t)to16(lo[2 * e + 1], bf16) << 16;
-        o[e + 2] = to16(hi[2 * e], bf16) | (uint32_t)to16(hi[2 * e + 1], bf16) << 16;
+// Whether a dword holds a 16-bit infinity or NaN, and the dword without them.
+template <bool BF>
+__device__ __forceinline__ bool take_odd(uint32_t &w) {
+    constexpr uint32_t inf = BF ? 0x7F80u : 0x7C00u;
+    const bool lo = (w & inf) == inf, hi = (w >> 16 & inf) == inf;
+    w &= (lo ? 0 : 0xFFFFu) | (hi ? 0 : 0xFFFF0000u);
+    return lo || hi;
+}
+
+// which of the drafted tokens j0 .. j0 + 31 the lane's rows see
+template <int NT>
+__device__ __forceinline__ void draft_mask(const DraftDev &d, const Seq &q, int j0, int row0, int rows, int ln, uint32_t (&see)[NT]) {
+    const int left = q.nt - j0;
+#pragma unroll
+    for (int a = 0; a < NT; ++a) {
+        const int r = row0 + 16 * a + ln, i = r / d.G;
+        see[a] = r < rows ? (uint32_t)(token_mask(d, q.first + i, i) >> j0) & (left >= 32 ? 0xFFFFFFFFu : (1u << left) - 1) : 0;
     }
-    return o;
 }
 
 __device__ __forceinline__ float2 load2_agent(const float *p) {
@@ -292,93 +353,99 @@ __device__ __forceinline__ void store2_agent(float *p, float a, float b) {
     __hip_atomic_store((uint64_t *)p, (uint64_t)__builtin_bit_cast(uint32_t, b) << 32 | __builtin_bit_cast(uint32_t, a), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// A record: [row][D] sums, then [row] (m, l). Elements e .. e + 3 of row r over the np records of a segment, in order, eight
-// loads in flight at a time; AGENT: written in this launch by other workgroups.
+struct Part { float4v v; float m, l; };   // four elements of a row
+__device__ __forceinline__ void add_part(Part &a, const Part &b) {
+    const float mn = fmaxf(a.m, b.m), mb = mn == -INFINITY ? 0.0f : mn;
+    const float f0 = exp2f(a.m - mb), f1 = exp2f(b.m - mb);
+    a.m = mn;
+    a.l = a.l * f0 + b.l * f1;
+    a.v = a.v * f0 + b.v * f1;
+}
+
+// Elements e .. e + 3 of row r over records b0 .. b1 - 1 of a segment (of workgroups p0 ..), in order, eight loads in flight
+// at a time; AGENT: written in this launch by other workgroups.
 template <int D, bool AGENT>
-__device__ __forceinline__ void join_records(const float *part, size_t rec, int rows_wg, int p0, int np, int r, int e, float4v &v, float &m, float &l) {
-    m = -INFINITY, l = 0.0f, v = float4v{0, 0, 0, 0};
-    for (int b = 0; b < np; b += 8) {
-        float2 ml[8];
-        float4v x[8];
+__device__ __forceinline__ Part join_records(const float *part, size_t rec, int rows_wg, int p0, int b0, int b1, int r, int e) {
+    Part s{float4v{0, 0, 0, 0}, -INFINITY, 0.0f};
+    for (int b = b0; b < b1; b += 8) {
+        Part x[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            const int p = min(b + k, np - 1);
+            const int p = min(b + k, b1 - 1);
             const float *q = part + (2 * (size_t)(p0 + p) + (p == 0 ? 1 : 0)) * rec;
+            float2 ml;
             if constexpr (AGENT) {
-                ml[k] = load2_agent(q + (size_t)rows_wg * D + 2 * r);
-                const float2 a = load2_agent(q + (size_t)r * D + e), c = load2_agent(q + (size_t)r * D + e + 2);
-                x[k] = float4v{a.x, a.y, c.x, c.y};
+                ml = load2_agent(q + (size_t)rows_wg * D + 2 * r);
+                const float2 lo = load2_agent(q + (size_t)r * D + e), hi = load2_agent(q + (size_t)r * D + e + 2);
+                x[k].v = float4v{lo.x, lo.y, hi.x, hi.y};
             } else {
-                ml[k] = *(const float2 *)(q + (size_t)rows_wg * D + 2 * r);
-                x[k] = *(const float4v *)(q + (size_t)r * D + e);
+                ml = *(const float2 *)(q + (size_t)rows_wg * D + 2 * r);
+                x[k].v = *(const float4v *)(q + (size_t)r * D + e);
             }
+            x[k].m = ml.x, x[k].l = ml.y;
         }
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            if (b + k >= np) break;
-            const float mn = fmaxf(m, ml[k].x), mb = mn == -INFINITY ? 0.0f : mn;
-            const float f0 = exp2f(m - mb), f1 = exp2f(ml[k].x - mb);
-            m = mn;
-            l = l * f0 + ml[k].y * f1;
-            v = v * f0 + x[k] * f1;
-        }
+        for (int k = 0; k < 8; ++k)
+            if (b + k < b1) add_part(s, x[k]);
     }
+    return s;
 }
 
 template <int D, bool BF, bool QF>
-__device__ __forceinline__ void store_row(const AttnJob &J, int first, int h, int row, int e, float4v v, float m, float l) {
+__device__ __forceinline__ void store_row(const AttnJob &J, int first, int h, int row, int e, Part p) {
     constexpr float bias = BF ? 0.0f : 7.0f;
-    v *= l == 0.0f ? 0.0f : 1.0f / l;
+    p.v *= p.l == 0.0f ? 0.0f : 1.0f / p.l;
     const int G = J.d.G, i = row / G, head = h * G + row - i * G;
     const size_t at = (size_t)(first + i) * J.ldo + (size_t)head * J.hso + e;
-    if constexpr (QF) *(float4v *)((float *)J.out + at) = v;
-    else {
-        const uint2v p = {pack2<BF>(v[0], v[1]), pack2<BF>(v[2], v[3])};
-        *(uint2v *)((uint16_t *)J.out + at) = p;
-    }
-    if (e == 0 && J.lse) J.lse[(size_t)(first + i) * J.c.n_kv * G + head] = l == 0.0f ? -INFINITY : (m - bias + __log2f(l)) * kLn2;
+    if constexpr (QF) *(float4v *)((float *)J.out + at) = p.v;
+    else *(uint2v *)((uint16_t *)J.out + at) = uint2v{pack2<BF>(p.v[0], p.v[1]), pack2<BF>(p.v[2], p.v[3])};
+    if (e == 0 && J.lse) J.lse[(size_t)(first + i) * J.c.n_kv * G + head] = p.l == 0.0f ? -INFINITY : (p.m - bias + __log2f(p.l)) * kLn2;
 }
 
-// The records of split segments in a launch of their own: a thread four elements of a row.
+// The records of split segments in a launch of their own: 32 threads a 128-element piece of rows, eight ranges of records
+// side by side.
 template <int D, bool BF, bool QF>
 __global__ __launch_bounds__(256) void k_attn_join(AttnJob J, int rows_wg) {
+    __shared__ Part sh[8][32];
     const int lane = threadIdx.x & 63, s = blockIdx.z / J.c.n_kv, h = blockIdx.z % J.c.n_kv, rt = blockIdx.y;
-    const int x4 = blockIdx.x * 256 + threadIdx.x, r = x4 / (D / 4), e = x4 % (D / 4) * 4;
-    int total = 0, base = 0;
-    for (int s0 = 0; s0 < J.c.n_seq; s0 += 64) {
+    const int sub = threadIdx.x >> 5, x4 = blockIdx.x * 32 + (threadIdx.x & 31), r = x4 / (D / 4), e = x4 % (D / 4) * 4;
+    const Shares w = share_out(J, rows_wg);
+    int base = 0;
+    for (int s0 = 0; s0 < s; s0 += 64) {
         int v = 0;
-        if (s0 + lane < J.c.n_seq) {
-            const SeqUnits u = seq_units(J, s0 + lane, rows_wg);
-            v = J.c.n_kv * u.rts * u.per_seg;
+        if (s0 + lane < s) {
+            const Seq q = seq_of(J, s0 + lane, rows_wg);
+            v = J.c.n_kv * q.rts * w.units(q.tiles);
         }
-        int b = s0 + lane < s ? v : 0;
-        if (J.c.n_seq > 1)
-            for (int o = 32; o; o >>= 1) {
-                v += __shfl_xor(v, o);
-                b += __shfl_xor(b, o);
-            }
-        else v = __builtin_amdgcn_readfirstlane(v);
-        total += v;
-        base += J.c.n_seq > 1 ? b : 0;
+        base += wave_sum(v);
     }
-    const int per = max(J.least, (total + J.nwg - 1) / J.nwg);
-    const SeqUnits q = seq_units(J, s, rows_wg);
-    if (rt >= q.rts || rt * rows_wg + r >= q.nt * J.d.G || r >= rows_wg) return;
-    const int sa = base + (h * q.rts + rt) * q.tiles, sb = sa + q.tiles, p0 = sa / per, np = (sb - 1) / per - p0 + 1;
+    const Seq q = seq_of(J, s, rows_wg);
+    if (rt >= q.rts) return;
+    const int ps = w.units(q.tiles), sa = base + (h * q.rts + rt) * ps, p0 = sa / w.per, np = (sa + ps - 1) / w.per - p0 + 1;
     if (np < 2) return;
-    float4v v;
-    float m, l;
-    join_records<D, false>(J.part, (size_t)rows_wg * (D + 2), rows_wg, p0, np, r, e, v, m, l);
-    store_row<D, BF, QF>(J, q.first, h, rt * rows_wg + r, e, v, m, l);
+    const bool on = r < min(rows_wg, q.nt * J.d.G - rt * rows_wg);
+    const int each = (np + 7) / 8;
+    Part p{float4v{0, 0, 0, 0}, -INFINITY, 0.0f};
+    if (on) p = join_records<D, false>(J.part, (size_t)rows_wg * (D + 2), rows_wg, p0, min(np, sub * each), min(np, (sub + 1) * each), r, e);
+    sh[sub][threadIdx.x & 31] = p;
+    __syncthreads();
+    if (sub || !on) return;
+    for (int k = 1; k < 8; ++k) add_part(p, sh[k][threadIdx.x & 31]);
+    store_row<D, BF, QF>(J, q.first, h, rt * rows_wg + r, e, p);
 }
 
-template <int D, bool BF, bool QF, int NT>
+// SHARE: the waves' rows are many; each tile of K and V is brought to LDS once for all of them, a stage of tiles ahead in
+// registers. Else each wave loads its tiles straight into operands.
+template <int D, bool BF, bool QF, int NT, bool SHARE>
 __global__ __launch_bounds__(64 * attn_waves(D)) void k_attn(AttnJob J) {
     constexpr int kWaves = attn_waves(D);
-    typedef Wave<D, BF, QF, NT> W;
-    constexpr int R16 = 16 * NT, DV = W::DV;
-    extern __shared__ float sh[];   // [wave][row][D + 4] sums, then [wave][row] m, l
+    typedef Wave<D, BF, QF, NT, SHARE> W;
+    constexpr int R16 = 16 * NT, DV = W::DV, PC = W::PC;
+    extern __shared__ float4v sh4[];   // SHARE: two stages of K, V; then [wave][row][D + 4] sums, [wave][row] m, l
     __shared__ unsigned last;
+    __shared__ int paged[4][2 * stage_tiles(D)];   // SHARE: whether a stage's halves have a page
+    __shared__ int odd_row[4][32 * stage_tiles(D)];   // SHARE: drafted tokens with infinities or NaN among their values
+    float *sh = (float *)sh4;
     const KvDev &c = J.c;
     const DraftDev &d = J.d;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, ln = lane & 15;
@@ -386,20 +453,8 @@ __global__ __launch_bounds__(64 * attn_waves(D)) void k_attn(AttnJob J) {
     // consecutive units on one XCD: workgroups go round robin over the eight
     const int nwg = gridDim.x, wg = nwg % 8 ? (int)blockIdx.x : (int)(blockIdx.x % 8) * (nwg / 8) + (int)(blockIdx.x / 8);
 
-    // all units, and the workgroup's share [u0, u1)
-    int total = 0;
-    for (int s0 = 0; s0 < c.n_seq; s0 += 64) {
-        int v = 0;
-        if (s0 + lane < c.n_seq) {
-            const SeqUnits u = seq_units(J, s0 + lane, rows_wg);
-            v = c.n_kv * u.rts * u.per_seg;
-        }
-        if (c.n_seq > 1)
-            for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-        total += __builtin_amdgcn_readfirstlane(v);
-    }
-    const int per = max(J.least, (total + nwg - 1) / nwg);
-    const int u0 = wg * per, u1 = min(total, u0 + per);
+    const Shares share = share_out(J, rows_wg);
+    const int per = share.per, u0 = wg * per, u1 = min(share.total, u0 + per);
     if (u0 >= u1) return;
     // the sequence of unit u0
     int s = 0, base = 0;
@@ -407,8 +462,8 @@ __global__ __launch_bounds__(64 * attn_waves(D)) void k_attn(AttnJob J) {
         for (int s0 = 0; s0 < c.n_seq; s0 += 64) {
             int v = 0;
             if (s0 + lane < c.n_seq) {
-                const SeqUnits u = seq_units(J, s0 + lane, rows_wg);
-                v = c.n_kv * u.rts * u.per_seg;
+                const Seq q = seq_of(J, s0 + lane, rows_wg);
+                v = c.n_kv * q.rts * share.units(q.tiles);
             }
             int x = v;
             for (int o = 1; o < 64; o <<= 1) {
@@ -426,227 +481,273 @@ __global__ __launch_bounds__(64 * attn_waves(D)) void k_attn(AttnJob J) {
         }
 
     W w;
-    const uint32_t ko = (uint32_t)ln * (uint32_t)c.slot_stride + 8 * g, vo = 4 * g * (uint32_t)c.slot_stride + DV * ln;
+    const uint32_t ss = (uint32_t)c.slot_stride, ko = (uint32_t)ln * ss + 8 * g, vo = 4 * g * ss + DV * ln;
     for (int u = u0; u < u1;) {
-        SeqUnits q = seq_units(J, s, rows_wg);
+        Seq q = seq_of(J, s, rows_wg);
         q.nt = __builtin_amdgcn_readfirstlane(q.nt), q.n = __builtin_amdgcn_readfirstlane(q.n), q.first = __builtin_amdgcn_readfirstlane(q.first);
         q.rts = __builtin_amdgcn_readfirstlane(q.rts), q.tiles = __builtin_amdgcn_readfirstlane(q.tiles);
-        const int ps = J.split ? q.tiles : q.nt ? 1 : 0, units = c.n_kv * q.rts * ps;
+        const int ps = share.units(q.tiles), units = c.n_kv * q.rts * ps;
         if (u >= base + units) {   // past this sequence (or none of its units)
             base += units;
             ++s;
             continue;
         }
         const int seg = (u - base) / ps, t0 = (u - base) - seg * ps, h = seg / q.rts, rt = seg - h * q.rts;
-        const int t1 = J.split ? min(q.tiles, t0 + (u1 - u)) : q.tiles, ctx = (q.n + 31) / 32;
+        const int t1 = share.split ? min(q.tiles, t0 + (u1 - u)) : q.tiles, ctx = (q.n + 31) / 32;
         const int sa = u - t0, sb = sa + ps;   // the segment's units
         u = min(u1, sb);
         const int rows = q.nt * d.G, row0 = rt * rows_wg + rwi * R16;
-        w.load_q(d, q.first, h, row0, rows, lane);
-
         const uint16_t *kp = c.k + (size_t)h * c.head_stride, *vp = c.v + (size_t)h * c.head_stride;
-        const int full = min(t1, q.n / 32);   // tiles of 32 slots in use
         float x[NT][8];
-        for (int tb = t0 + swi; tb < full; tb += 32 * SW) {
-            // offsets of the wave's next 64 halves, a lane each: tile tb + SW (lane / 2), half lane & 1
-            int64_t off = -1;
-            {
-                const int t = tb + SW * (lane >> 1);
-                if (t < full) off = slot_offset(c, s, 32 * t + 16 * (lane & 1));
-            }
-            const int lo = (int)off, hi = (int)(off >> 32), nt = min(32, (full - tb + SW - 1) / SW);
-            auto half = [&](int i) { return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, i) << 32 | (uint32_t)__builtin_amdgcn_readlane(lo, i)); };
-            int64_t h0 = half(0), h1 = half(1);
-            w.load_k(kp, max(h0, (int64_t)0), max(h1, (int64_t)0), ko);
-            w.load_v(vp, max(h0, (int64_t)0), max(h1, (int64_t)0), vo, (uint32_t)c.slot_stride);
-            for (int i = 0; i < nt; ++i) {
-                const int64_t n0 = half(2 * min(i + 1, nt - 1)), n1 = half(2 * min(i + 1, nt - 1) + 1);
-                w.qk(x);
-                if (i + 1 < nt) w.load_k(kp, max(n0, (int64_t)0), max(n1, (int64_t)0), ko);
-                if ((h0 | h1) < 0) {   // a half without a page: hidden, its values zeros
+
+        if constexpr (SHARE) {
+            constexpr int ST = stage_tiles(D), RWV = 64 / PC, RP = kWaves * RWV, PASS = 32 * ST / RP;   // rows of a wave and of the workgroup in a pass
+            uint4v *kb = (uint4v *)sh4, *vb = kb + 2 * 32 * ST * W::KP;
+            const int rl = lane / PC, pl = lane % PC;
+            uint4v sk[PASS], sv[PASS];
+            int lo = 0, hi = 0;
+            const int stages = (t1 - t0 + ST - 1) / ST;
+            auto load = [&](int st) {
+                constexpr int CH = 64 / PASS;   // stages whose row offsets the lanes hold
+                if (st % CH == 0) {
+                    const int r0 = (lane % PASS) * RP + wave * RWV, t = t0 + (st + lane / PASS) * ST + r0 / 32, slot = 32 * t + r0 % 32;
+                    int64_t off = -1;
+                    if (t < min(t1, ctx) && slot < q.n) off = slot_offset(c, s, slot & ~15);
+                    lo = (int)off, hi = (int)(off >> 32);
+                }
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        if ((j < 4 ? h0 : h1) >= 0) continue;
+                for (int p = 0; p < PASS; ++p) {
+                    const int r0 = p * RP + wave * RWV, t = t0 + st * ST + r0 / 32, from = st % CH * PASS + p;
+                    const int64_t off = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, from) << 32 | (uint32_t)__builtin_amdgcn_readlane(lo, from));
+                    sk[p] = sv[p] = uint4v{0, 0, 0, 0};
+                    if (t < min(t1, ctx)) {
+                        if (off >= 0 && 32 * t + r0 % 32 + rl < q.n) {
+                            const size_t at = (size_t)off + (r0 % 16 + rl) * ss + 8 * pl;
+                            sk[p] = *(const uint4v *)(kp + at);
+                            sv[p] = *(const uint4v *)(vp + at);
+                        }
+                    } else if (t < t1) {
+                        const int j = 32 * (t - ctx) + r0 % 32 + rl;
+                        bool has = false;
+                        if (j < q.nt) {
+                            const size_t at = (size_t)(q.first + j) * d.ld_kv + (size_t)h * d.hs_kv + 8 * pl;
+                            sk[p] = draft8(d.k, at, d.kv_f32, BF);
+                            sv[p] = draft8(d.v, at, d.kv_f32, BF);
 #pragma unroll
-                        for (int a = 0; a < NT; ++a) x[a][j] = -INFINITY;
-                        for (int e = 0; e < W::VW; ++e) w.vf[j][e] = 0;
+                            for (int e = 0; e < 4; ++e) {
+                                uint32_t v = sv[p][e];
+                                has |= take_odd<BF>(v);
+                                sv[p][e] = v;
+                            }
+                        }
+                        const uint64_t by = __ballot(has);
+                        if (pl == 0) odd_row[st & 3][r0 + rl] = (by >> (rl * PC) & (PC == 64 ? ~0ull : (1ull << PC) - 1)) != 0;
+                    }
+                    if (lane == 0 && r0 % 16 == 0) paged[st & 3][r0 / 16] = off >= 0;
+                }
+            };
+            auto put = [&](int st) {
+#pragma unroll
+                for (int p = 0; p < PASS; ++p) {
+                    const int r = (st & 1) * 32 * ST + p * RP + wave * RWV + rl;
+                    kb[r * W::KP + pl] = sk[p];
+                    vb[r * W::VP + pl] = sv[p];
+                }
+            };
+            load(0);
+            w.load_q(d, q.first, h, row0, rows, lane);
+            put(0);
+            if (stages > 1) load(1);
+            __syncthreads();
+            for (int st = 0; st < stages; ++st) {
+                if (st + 1 < stages) put(st + 1);
+                if (st + 2 < stages) load(st + 2);
+#pragma unroll 1
+                for (int i = SW == 1 ? 0 : swi; i < ST; i += SW) {
+                    const int t = t0 + st * ST + i, left = q.n - 32 * t;
+                    if (t >= t1) break;
+                    const uint4v *kt = kb + ((st & 1) * ST + i) * 32 * W::KP + ln * W::KP + g;
+                    const uint16_t *vt = (const uint16_t *)(vb + ((st & 1) * ST + i) * 32 * W::VP) + (4 * g + ln / 4) * 8 * W::VP + 4 * (ln % 4);
+                    const int pg = __builtin_amdgcn_readfirstlane(paged[st & 3][2 * i] + 2 * paged[st & 3][2 * i + 1]);
+                    if (left >= 32 && pg == 3) {
+                        w.tile(x, kt, vt);
+                    } else {
+                        uint32_t see[NT];
+                        if (t >= ctx) draft_mask<NT>(d, q, 32 * (t - ctx), row0, rows, ln, see);
+                        else
+                            for (int a = 0; a < NT; ++a) see[a] = (left >= 32 ? 0xFFFFFFFFu : (1u << left) - 1) & ((pg & 1 ? 0xFFFFu : 0) | (pg & 2 ? 0xFFFF0000u : 0));
+                        w.masked(x, kt, vt, see, lane);
+                        if (t >= ctx) {
+                            const uint32_t odd = (uint32_t)__ballot(lane < 32 && odd_row[st & 3][32 * i + lane]);
+                            if (odd) w.add_odd(odd, see, d, q.first + 32 * (t - ctx), h, lane);
+                        }
                     }
                 }
-                w.softmax(x);
-                w.pv(x);
-                if (i + 1 < nt) w.load_v(vp, max(n0, (int64_t)0), max(n1, (int64_t)0), vo, (uint32_t)c.slot_stride);
-                h0 = n0, h1 = n1;
-            }
-        }
-        // the cache's last, partial tile and the drafted tokens: rows that are not there are zeros, scores are masked
-        const int t_rest = max(t0, q.n / 32);
-        for (int t = t_rest + (swi - (t_rest - t0) % SW + SW) % SW; t < t1; t += SW) {
-            const bool draft = t >= ctx;
-            uint64_t see[NT];
-            if (draft) {
-                const int j0 = 32 * (t - ctx), left = q.nt - j0;
+                __syncthreads();            }
+        } else {
+            const int full = min(t1, q.n / 32);   // tiles of 32 slots in use
+            bool have_q = false;
+            for (int tb = t0 + swi; tb < full; tb += 32 * SW) {
+                // offsets of the wave's next 64 halves, a lane each: tile tb + SW (lane / 2), half lane & 1
+                int64_t off = -1;
+                {
+                    const int t = tb + SW * (lane >> 1);
+                    if (t < full) off = slot_offset(c, s, 32 * t + 16 * (lane & 1));
+                }
+                const int lo = (int)off, hi = (int)(off >> 32), many = min(32, (full - tb + SW - 1) / SW);
+                auto half = [&](int i) { return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, i) << 32 | (uint32_t)__builtin_amdgcn_readlane(lo, i)); };
+                int64_t h0 = half(0), h1 = half(1);
+                w.load_k(kp, max(h0, (int64_t)0), max(h1, (int64_t)0), ko);
+                w.load_v(vp, max(h0, (int64_t)0), max(h1, (int64_t)0), vo, ss);
+                if (!have_q) w.load_q(d, q.first, h, row0, rows, lane);   // behind the loads of the first tile
+                have_q = true;
+                for (int i = 0; i < many; ++i) {
+                    const int64_t n0 = half(2 * min(i + 1, many - 1)), n1 = half(2 * min(i + 1, many - 1) + 1);
+                    w.qk(x, nullptr);
+                    if (i + 1 < many) w.load_k(kp, max(n0, (int64_t)0), max(n1, (int64_t)0), ko);
+                    if ((h0 | h1) < 0) {   // a half without a page: hidden, its values zeros
 #pragma unroll
-                for (int a = 0; a < NT; ++a) {
-                    const int r = row0 + 16 * a + ln, i = r / d.G;
-                    see[a] = r < rows ? token_mask(d, q.first + i, i) >> j0 & (left >= 32 ? 0xFFFFFFFFu : (1u << left) - 1) : 0;
+                        for (int j = 0; j < 8; ++j) {
+                            if ((j < 4 ? h0 : h1) >= 0) continue;
+#pragma unroll
+                            for (int a = 0; a < NT; ++a) x[a][j] = -INFINITY;
+                            for (int e = 0; e < W::VW; ++e) w.vf[j][e] = 0;
+                        }
+                    }
+                    w.softmax(x);
+                    w.pv(x, nullptr);
+                    if (i + 1 < many) w.load_v(vp, max(n0, (int64_t)0), max(n1, (int64_t)0), vo, ss);
+                    h0 = n0, h1 = n1;
+                }
+            }
+            if (!have_q) w.load_q(d, q.first, h, row0, rows, lane);
+            // the cache's last, partial tile and the drafted tokens
+            const int t_rest = max(t0, q.n / 32);
+            for (int t = t_rest + (swi - (t_rest - t0) % SW + SW) % SW; t < t1; t += SW) {
+                const bool draft = t >= ctx;
+                uint32_t see[NT];
+                const int j0 = 32 * (t - ctx), left = draft ? q.nt - j0 : q.n - 32 * t;
+                int64_t h0 = 0, h1 = 0;
+                if (draft) {
+                    draft_mask<NT>(d, q, j0, row0, rows, ln, see);
+                } else {
+                    h0 = slot_offset(c, s, 32 * t);
+                    h1 = left > 16 ? slot_offset(c, s, 32 * t + 16) : -1;
+                    for (int a = 0; a < NT; ++a) see[a] = ((1u << left) - 1) & ((h0 >= 0 ? 0xFFFFu : 0) | (h1 >= 0 ? 0xFFFF0000u : 0));
                 }
 #pragma unroll
                 for (int b = 0; b < 2; ++b)
 #pragma unroll
-                    for (int k = 0; k < W::C; ++k)
-                        w.kf[b][k] = 16 * b + ln < left ? draft8(d.k, (size_t)(q.first + j0 + 16 * b + ln) * d.ld_kv + (size_t)h * d.hs_kv + 32 * k + 8 * g, d.kv_f32, BF)
-                                                        : uint4v{0, 0, 0, 0};
+                    for (int k = 0; k < W::C; ++k) {
+                        uint4v v = {0, 0, 0, 0};
+                        if (16 * b + ln < left) {
+                            if (draft) v = draft8(d.k, (size_t)(q.first + j0 + 16 * b + ln) * d.ld_kv + (size_t)h * d.hs_kv + 32 * k + 8 * g, d.kv_f32, BF);
+                            else if ((b ? h1 : h0) >= 0) v = *(const uint4v *)(kp + (b ? h1 : h0) + ko + 32 * k);
+                        }
+                        w.kf[b][k] = v;
+                    }
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const int jj = (j < 4 ? 0 : 12) + 4 * g + j;
                     const size_t at = (size_t)(q.first + j0 + jj) * d.ld_kv + (size_t)h * d.hs_kv + DV * ln;
+                    const int64_t hb = j < 4 ? h0 : h1;
 #pragma unroll
                     for (int e = 0; e < W::VW; ++e) {
                         uint32_t v = 0;
-                        if (jj < left) {
-                            if (d.kv_f32) {
-                                const float *p = (const float *)d.v + at + 2 * e;
-                                v = to16(p[0], BF) | (uint32_t)to16(p[1], BF) << 16;
-                            } else {
-                                v = *(const uint32_t *)((const uint16_t *)d.v + at + 2 * e);
-                            }
+                        if (jj < left && hb >= 0) {
+                            if (!draft) v = *(const uint32_t *)(vp + hb + vo + (j & 3) * ss + 2 * e);
+                            else if (d.kv_f32) v = pack2<BF>(((const float *)d.v)[at + 2 * e], ((const float *)d.v)[at + 2 * e + 1]);
+                            else v = *(const uint32_t *)((const uint16_t *)d.v + at + 2 * e);
                         }
                         w.vf[j][e] = v;
                     }
-                    }
-            } else {
-                const int j0 = 32 * t, left = q.n - j0;
-                const int64_t h0 = slot_offset(c, s, j0), h1 = left > 16 ? slot_offset(c, s, j0 + 16) : -1;
-#pragma unroll
-                for (int b = 0; b < 2; ++b)
-#pragma unroll
-                    for (int k = 0; k < W::C; ++k)
-                        w.kf[b][k] = 16 * b + ln < left && (b ? h1 : h0) >= 0 ? *(const uint4v *)(kp + (b ? h1 : h0) + ko + 32 * k) : uint4v{0, 0, 0, 0};
-                uint32_t in = 0;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int jj = (j < 4 ? 0 : 12) + 4 * g + j;
-                    const int64_t hb = j < 4 ? h0 : h1;
-                    const bool on = jj < left && hb >= 0;
-#pragma unroll
-                    for (int e = 0; e < W::VW; ++e)
-                        w.vf[j][e] = on ? *(const uint32_t *)(vp + hb + vo + (j & 3) * (uint32_t)c.slot_stride + 2 * e) : 0;
-                    in |= (uint32_t)on << jj;
                 }
-#pragma unroll
-                for (int a = 0; a < NT; ++a) see[a] = in;
-            }
-            w.qk(x);
-#pragma unroll
-            for (int a = 0; a < NT; ++a)
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (!(see[a] >> ((j < 4 ? 0 : 12) + 4 * g + j) & 1)) x[a][j] = -INFINITY;
-            w.softmax(x);
-            if (draft) {
-                // A hidden token's infinite or NaN value must not meet its zero weight in the product: rows with such values
-                // are taken out of the operand and added element by element to the rows of o that see them.
                 uint32_t odd = 0;
+                if (draft)
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-#pragma unroll
-                    for (int e = 0; e < W::VW; ++e) {
-                        constexpr uint32_t ex = BF ? 0x7F80u : 0x7C00u;
-                        if ((w.vf[j][e] & ex) == ex || (w.vf[j][e] >> 16 & ex) == ex) odd |= 1u << j;
-                    }
-                if (__any(odd != 0)) {
-                    const int j0 = 32 * (t - ctx);
                     for (int j = 0; j < 8; ++j) {
-                        uint32_t gs = 0;   // groups (of 16 lanes) with such a row at j
+                        bool has = false;
+#pragma unroll
+                        for (int e = 0; e < W::VW; ++e) has |= take_odd<BF>(w.vf[j][e]);
+                        const uint64_t by = __ballot(has);
                         for (int k = 0; k < 4; ++k)
-                            if (__ballot(odd >> j & 1) >> (16 * k) & 0xFFFF) gs |= 1u << k;
-                        if (gs >> g & 1)
-                            for (int e = 0; e < W::VW; ++e) {
-                                // (select over constant indices keeps vf in registers)
-#pragma unroll
-                                for (int jj = 0; jj < 8; ++jj)
-                                    if (jj == j) w.vf[jj][e] = 0;
-                            }
-                        for (int k = 0; k < 4; ++k) {
-                            if (!(gs >> k & 1)) continue;
-                            const int tok = (j < 4 ? 0 : 12) + 4 * k + j;
-#pragma unroll
-                            for (int a = 0; a < NT; ++a) {
-                                float p = 0;
-#pragma unroll
-                                for (int jj = 0; jj < 8; ++jj)
-                                    if (jj == j) p = x[a][jj];
-                                p = __shfl(p, 16 * k + ln);   // the row's weight of that token
-                                const bool on = see[a] >> tok & 1;
-#pragma unroll
-                                for (int e = 0; e < DV; ++e)
-#pragma unroll
-                                    for (int i = 0; i < 4; ++i) {
-                                        const size_t at = (size_t)(q.first + j0 + tok) * d.ld_kv + (size_t)h * d.hs_kv + DV * (4 * g + i) + e;
-                                        const float v = d.kv_f32 ? from16(to16(((const float *)d.v)[at], BF), BF) : from16(((const uint16_t *)d.v)[at], BF);
-                                        if (on) w.o[a][e][i] = fmaf(p, v, w.o[a][e][i]);
-                                    }
-                            }
-                        }
+                            if (by >> (16 * k) & 0xFFFF) odd |= 1u << ((j < 4 ? 0 : 12) + 4 * k + j);
                     }
-                }
+                w.masked(x, nullptr, nullptr, see, lane);
+                if (odd) w.add_odd(odd, see, d, q.first + j0, h, lane);
             }
-            w.pv(x);
         }
 
-        // the workgroup's waves of the same rows, then the segment's workgroups
-        constexpr int LD = D + 4;
-        float *po = sh + (size_t)wave * R16 * LD, *pm = sh + (size_t)kWaves * R16 * LD, *pl = pm + kWaves * R16;
-#pragma unroll
-        for (int a = 0; a < NT; ++a) {
-            float l = w.l[a];
-            l += __shfl_xor(l, 16);
-            l += __shfl_xor(l, 32);
-            const int r = 16 * a + ln;
-            if (row0 + r < rows) {
-                if (g == 0) {
-                    pm[wave * R16 + r] = w.m[a];
-                    pl[wave * R16 + r] = l;
-                }
-                // element DV (4 g + i) + t of the row
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int t = 0; t < DV; t += 4)
-                        *(float4v *)(po + r * LD + DV * (4 * g + i) + t) = float4v{w.o[a][t][i], w.o[a][t + 1][i], w.o[a][t + 2][i], w.o[a][t + 3][i]};
-            }
-        }
-        __syncthreads();
         const bool whole = t0 == 0 && t1 == q.tiles;
         const int here = min(rows_wg, rows - rt * rows_wg);
         const int p0 = sa / per, np = (sb - 1) / per - p0 + 1;   // the segment's workgroups p0 .. p0 + np - 1
         const size_t rec = (size_t)rows_wg * (D + 2);
         float *mine = whole ? nullptr : J.part + (2 * (size_t)wg + (sa < wg * per ? 0 : 1)) * rec;
-        for (int x4 = threadIdx.x; x4 < here * (D / 4); x4 += 64 * kWaves) {
-            const int r = x4 / (D / 4), e = x4 % (D / 4) * 4, rg = r / R16, rr = r % R16;
-            float m = -INFINITY;
-            for (int k = 0; k < SW; ++k) m = fmaxf(m, pm[(k * RW + rg) * R16 + rr]);
-            const float mb = m == -INFINITY ? 0.0f : m;
-            float l = 0;
-            float4v v = {0, 0, 0, 0};
-            for (int k = 0; k < SW; ++k) {
-                const int wv = k * RW + rg;
-                const float f = exp2f(pm[wv * R16 + rr] - mb);
-                l += f * pl[wv * R16 + rr];
-                v += f * *(const float4v *)(sh + ((size_t)wv * R16 + rr) * LD + e);
-            }
+        auto leave = [&](int r, int e, const Part &p) {   // row r of the row tile
             if (whole) {
-                store_row<D, BF, QF>(J, q.first, h, rt * rows_wg + r, e, v, m, l);
-            } else if (J.join) {
-                *(float4v *)(mine + (size_t)r * D + e) = v;
-                if (e == 0) *(float2 *)(mine + (size_t)rows_wg * D + 2 * r) = make_float2(m, l);
+                store_row<D, BF, QF>(J, q.first, h, rt * rows_wg + r, e, p);
+            } else if (SHARE || J.join) {
+                *(float4v *)(mine + (size_t)r * D + e) = p.v;
+                if (e == 0) *(float2 *)(mine + (size_t)rows_wg * D + 2 * r) = make_float2(p.m, p.l);
             } else {
-                store2_agent(mine + (size_t)r * D + e, v[0], v[1]);
-                store2_agent(mine + (size_t)r * D + e + 2, v[2], v[3]);
-                if (e == 0) store2_agent(mine + (size_t)rows_wg * D + 2 * r, m, l);
+                store2_agent(mine + (size_t)r * D + e, p.v[0], p.v[1]);
+                store2_agent(mine + (size_t)r * D + e + 2, p.v[2], p.v[3]);
+                if (e == 0) store2_agent(mine + (size_t)rows_wg * D + 2 * r, p.m, p.l);
+            }
+        };
+#pragma unroll
+        for (int a = 0; a < NT; ++a) {
+            w.l[a] += __shfl_xor(w.l[a], 16);
+            w.l[a] += __shfl_xor(w.l[a], 32);
+        }
+        // f(element, four of the row's sums) over what the lane has of row tile a
+        auto pieces = [&](int a, auto f) {
+            if constexpr (SHARE) {
+#pragma unroll
+                for (int t = 0; t < DV; ++t) f(16 * t + 4 * g, w.o[a][t]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int t = 0; t < DV; t += 4) f(DV * (4 * g + i) + t, float4v{w.o[a][t][i], w.o[a][t + 1][i], w.o[a][t + 2][i], w.o[a][t + 3][i]});
+            }
+        };
+        if (SW == 1) {   // the wave's sums are the workgroup's
+#pragma unroll
+            for (int a = 0; a < NT; ++a) {
+                const int r = rwi * R16 + 16 * a + ln;
+                if (r < here) pieces(a, [&](int e, float4v v) { leave(r, e, Part{v, w.m[a], w.l[a]}); });
+            }
+        } else {   // the workgroup's waves of the same rows meet in LDS
+            constexpr int LD = D + 4;
+            float *po = sh + (size_t)wave * R16 * LD, *pm = sh + (size_t)kWaves * R16 * LD, *pl = pm + kWaves * R16;
+#pragma unroll
+            for (int a = 0; a < NT; ++a) {
+                const int r = 16 * a + ln;
+                if (row0 + r >= rows) continue;
+                if (g == 0) {
+                    pm[wave * R16 + r] = w.m[a];
+                    pl[wave * R16 + r] = w.l[a];
+                }
+                pieces(a, [&](int e, float4v v) { *(float4v *)(po + r * LD + e) = v; });
+            }
+            __syncthreads();
+            for (int x4 = threadIdx.x; x4 < here * (D / 4); x4 += 64 * kWaves) {
+                const int r = x4 / (D / 4), e = x4 % (D / 4) * 4, rg = r / R16, rr = r % R16;
+                float m = -INFINITY;
+                for (int k = 0; k < SW; ++k) m = fmaxf(m, pm[(k * RW + rg) * R16 + rr]);
+                const float mb = m == -INFINITY ? 0.0f : m;
+                Part p{float4v{0, 0, 0, 0}, m, 0.0f};
+                for (int k = 0; k < SW; ++k) {
+                    const int wv = k * RW + rg;
+                    const float f = exp2f(pm[wv * R16 + rr] - mb);
+                    p.l += f * pl[wv * R16 + rr];
+                    p.v += f * *(const float4v *)(sh + ((size_t)wv * R16 + rr) * LD + e);
+                }
+                leave(r, e, p);
             }
         }
-        if (!whole && !J.join) {
+        if (!SHARE && !whole && !J.join) {
             // the segment's last workgroup adds the records in the workgroups' order
             unsigned *ctr = J.count + ((size_t)s * c.n_kv + h) * J.rt + rt;
             __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the wave's record stores complete before the arrival
@@ -657,14 +758,24 @@ __global__ __launch_bounds__(64 * attn_waves(D)) void k_attn(AttnJob J) {
                 if (last) __hip_atomic_store(ctr, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
             __syncthreads();
-            if (last)
-                for (int x4 = threadIdx.x; x4 < here * (D / 4); x4 += 64 * kWaves) {
-                    const int r = x4 / (D / 4), e = x4 % (D / 4) * 4;
-                    float4v v;
-                    float m, l;
-                    join_records<D, true>(J.part, rec, rows_wg, p0, np, r, e, v, m, l);
-                    store_row<D, BF, QF>(J, q.first, h, rt * rows_wg + r, e, v, m, l);
+            if (last) {
+                // ranges of records side by side where the threads are more than the row pieces
+                Part *ps4 = (Part *)sh4;
+                const int items = here * (D / 4), subs = max(1, min(8, 64 * kWaves / items)), each = (np + subs - 1) / subs;
+                for (int x0 = 0; x0 < items; x0 += 64 * kWaves) {
+                    const int xi = x0 + (int)threadIdx.x, sub = subs > 1 ? xi / items : 0, x4 = xi - sub * items, r = x4 / (D / 4), e = x4 % (D / 4) * 4;
+                    const bool on = sub < subs && x4 < items;
+                    Part p{float4v{0, 0, 0, 0}, -INFINITY, 0.0f};
+                    if (on) p = join_records<D, true>(J.part, rec, rows_wg, p0, min(np, sub * each), min(np, (sub + 1) * each), r, e);
+                    if (subs > 1) {
+                        if (on && sub) ps4[xi] = p;
+                        __syncthreads();
+                        if (on && !sub)
+                            for (int k = 1; k < subs; ++k) add_part(p, ps4[k * items + x4]);
+                    }
+                    if (on && !sub) store_row<D, BF, QF>(J, q.first, h, rt * rows_wg + r, e, p);
                 }
+            }
         }
         __syncthreads();   // sh and last are free again
     }
@@ -672,15 +783,16 @@ __global__ __launch_bounds__(64 * attn_waves(D)) void k_attn(AttnJob J) {
 
 // Rows a wave and row waves a workgroup: 16 rows while they hold all, else 32 (16 with queries of several parts or
 // wide rows, whose operands fill the registers).
-constexpr size_t kJoinBytes = 64 << 10;   // records of more bytes than this are joined by a launch of their own
-struct AttnPlan { int nt, rw, rows_wg, rt; size_t segs, rec_bytes, head_bytes; };
+constexpr size_t kJoinBytes = 96 << 10;   // records of a segment of more bytes than this are joined by a launch of their own
+struct AttnPlan { int nt, rw, rows_wg, rt, share; size_t segs, rec_bytes, head_bytes; };
 static AttnPlan attn_plan(const KvDev &c, const DraftDev &d, int D) {
-    const int kWaves = attn_waves(D);
+    const int waves = attn_waves(D);
     AttnPlan p;
     const int rows = d.max_tokens * d.G;
     p.nt = rows <= 16 || d.q_f32 || D == 256 ? 1 : 2;
     p.rw = 1;
-    while (p.rw < kWaves && p.rw * 16 * p.nt < rows) p.rw *= 2;
+    while (p.rw < waves && p.rw * 16 * p.nt < rows) p.rw *= 2;
+    p.share = waves / p.rw <= stage_tiles(D);
     p.rows_wg = 16 * p.nt * p.rw;
     p.rt = (rows + p.rows_wg - 1) / p.rows_wg;
     p.segs = (size_t)c.n_seq * c.n_kv * p.rt;
@@ -694,229 +806,51 @@ size_t attn_workspace(const KvDev &c, const DraftDev &d, int D) {
     return p.head_bytes + 2 * (size_t)num_cus() * p.rec_bytes;
 }
 
-template <int D, bool BF, bool QF, int NT>
+template <int D, bool BF, bool QF, int NT, bool SHARE>
 static int attn_run(const AttnJob &J, int rows_wg, hipStream_t st) {
-    constexpr int kWaves = attn_waves(D), lds = kWaves * 16 * NT * (D + 4 + 2) * 4;
-    static const hipError_t e = hipFuncSetAttribute((const void *)k_attn<D, BF, QF, NT>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    constexpr int waves = attn_waves(D);
+    constexpr int sums = waves * 16 * NT * (D + 4 + 2) * 4, stages = SHARE ? 2 * 32 * stage_tiles(D) * (2 * 2 * D + 16 + 32) : 0;
+    const int lds = SHARE && J.rw == waves ? std::max(stages, waves * 64 * (int)sizeof(Part)) : std::max(sums, stages);
+    static const hipError_t e = hipFuncSetAttribute((const void *)k_attn<D, BF, QF, NT, SHARE>, hipFuncAttributeMaxDynamicSharedMemorySize, std::max(sums, stages));
     if (e != hipSuccess) return hip_check(e, "p8x_attn_tree LDS");
-    k_attn<D, BF, QF, NT><<<J.nwg, 64 * kWaves, lds, st>>>(J);
-    if (J.join) k_attn_join<D, BF, QF><<<dim3((rows_wg * (D / 4) + 255) / 256, J.rt, J.c.n_seq * J.c.n_kv), 256, 0, st>>>(J, rows_wg);
+    k_attn<D, BF, QF, NT, SHARE><<<J.nwg, 64 * waves, lds, st>>>(J);
+    if (J.join) k_attn_join<D, BF, QF><<<dim3((rows_wg * (D / 4) + 31) / 32, J.rt, J.c.n_seq * J.c.n_kv), 256, 0, st>>>(J, rows_wg);
     return hip_check(hipGetLastError(), "p8x_attn_tree launch");
+}
+
+template <int D, bool BF, bool QF, int NT>
+static int attn_form(const AttnJob &J, const AttnPlan &p, hipStream_t st) {
+    return p.share ? attn_run<D, BF, QF, NT, true>(J, p.rows_wg, st) : attn_run<D, BF, QF, NT, false>(J, p.rows_wg, st);
 }
 
 template <int D>
 static int attn_types(const AttnJob &J, const AttnPlan &p, hipStream_t st) {
     const bool bf = J.c.bf16;
-    if (J.d.q_f32) return bf ? attn_run<D, true, true, 1>(J, p.rows_wg, st) : attn_run<D, false, true, 1>(J, p.rows_wg, st);
+    if (J.d.q_f32) return bf ? attn_form<D, true, true, 1>(J, p, st) : attn_form<D, false, true, 1>(J, p, st);
     if constexpr (D < 256)
-        if (p.nt == 2) return bf ? attn_run<D, true, false, 2>(J, p.rows_wg, st) : attn_run<D, false, false, 2>(J, p.rows_wg, st);
-    return bf ? attn_run<D, true, false, 1>(J, p.rows_wg, st) : attn_run<D, false, false, 1>(J, p.rows_wg, st);
+        if (p.nt == 2) return bf ? attn_form<D, true, false, 2>(J, p, st) : attn_form<D, false, false, 2>(J, p, st);
+    return bf ? attn_form<D, true, false, 1>(J, p, st) : attn_form<D, false, false, 1>(J, p, st);
 }
 
 int launch_attn_tree(const KvDev &c, const DraftDev &d, int D, void *out, size_t ldo, size_t hso, float *lse, void *ws, size_t ws_bytes,
                      hipStream_t st) {
     const AttnPlan p = attn_plan(c, d, D);
-    const size_t most = p.segs * ((size_t)(c.max_len + 31) / 32 + 2);   // units
-    if (most >= (1u << 30)) return set_error(P8X_ERR_UNSUPPORTED, "p8x_attn_tree: %zu tiles of 32 slots (fewer than 2^30)", most);
+    const size_t most = p.segs * ((size_t)(c.max_len + 31) / 32 + 2);   // tiles
+    if (most >= (1u << 29)) return set_error(P8X_ERR_UNSUPPORTED, "p8x_attn_tree: %zu tiles of 32 slots (fewer than 2^29)", most);
     if (c.slot_stride >= (1u << 26)) return set_error(P8X_ERR_UNSUPPORTED, "p8x_attn_tree: slot_stride %zu (below 2^26)", c.slot_stride);
     AttnJob J{c, d, out, ldo, hso, lse, (unsigned *)ws, (float *)((char *)ws + p.head_bytes), p.rw, p.rt, attn_waves(D) / p.rw, 1, 0, 0};
     const size_t room = ws_bytes > p.head_bytes ? (ws_bytes - p.head_bytes) / (2 * p.rec_bytes) : 0;   // workgroups with records
     int nwg = (int)std::min<size_t>(num_cus(), room);
-    if (nwg < 16) {   // whole segments then
+    if (nwg < 16 || p.segs / p.rt > 65535 || p.rt > 65535) {   // whole segments then
         nwg = (int)std::min<size_t>(num_cus(), p.segs);
         J.split = 0, J.least = 1;
     }
     if (nwg >= 8) nwg = nwg / 8 * 8;
     J.nwg = nwg;
     // records of a segment, about, that one workgroup would join
-    const size_t each = J.split ? nwg / p.segs * p.rec_bytes : 0;
-    J.join = each > kJoinBytes && p.segs / p.rt <= 65535;
+    const size_t rows = std::min((size_t)d.max_tokens * d.G, (size_t)p.rows_wg), each = J.split ? nwg / p.segs * rows * (D + 2) * 4 : 0;
+    J.join = J.split && (p.share || each > kJoinBytes);
     return D == 64 ? attn_types<64>(J, p, st) : D == 128 ? attn_types<128>(J, p, st) : attn_types<256>(J, p, st);
-}
-
-// ---- scores -----------------------------------------------------------------------------------------------
-// sum over the accepted tokens' rows of exp(scale q k - lse) per slot. S [row][slot] = Q K^T with K as the B operand (lane
-// n = slot) straight from memory, each slot's keys read by one wave once, and Q as A from LDS, where the workgroup
-// leaves its rows in operand order; a lane's four rows of every tile are added in place, the four lane groups at the end.
-constexpr int kScoreWaves = 4;
-// rows that LDS holds at a time; more of them take the slots again
-__host__ __device__ constexpr int score_rows(int D) { return D == 256 ? 32 : 64; }
-
-struct ScoreJob {
-    KvDev c;
-    DraftDev d;
-    const uint64_t *accept;
-    const float *lse, *score;
-    float *score_out;
-    float decay;
-};
-
-// token of accepted rank r
-__device__ __forceinline__ int nth_bit(uint64_t b, int r) {
-    for (; r; --r) b &= b - 1;
-    return __ffsll((unsigned long long)b) - 1;
-}
-
-template <int D, bool BF, bool QF>
-__global__ __launch_bounds__(64 * kScoreWaves) void k_score(ScoreJob J) {
-    constexpr int C = D / 32, QP = QF ? (BF ? 3 : 2) : 1, RB = score_rows(D);
-    __shared__ uint4v sq[RB / 16][QP][C][64];
-    __shared__ float4v sl[RB / 4], sc[RB / 4];   // lse and factor of a product, by row (rows that are not there: 0)
-    __shared__ uint64_t see[RB];
-    const KvDev &c = J.c;
-    const DraftDev &d = J.d;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, ln = lane & 15;
-    const int s = blockIdx.z, h = blockIdx.y;
-    int first = 0;
-    const int nt = __builtin_amdgcn_readfirstlane(d.n_tokens ? seq_tokens(d, s, first) : 0), n = __builtin_amdgcn_readfirstlane(seq_len(c, s));
-    const uint64_t all = nt >= 64 ? ~0ull : (1ull << nt) - 1, acc = J.accept ? J.accept[s] & all : all;
-    const int cnt = __popcll(acc), rows = cnt * d.G;
-    // the workgroup's tiles of 32 slots; the drafts' are the last ones
-    const int ctx = (n + 31) / 32, tiles = ctx + (min(cnt, c.max_len - n) + 31) / 32, per = (tiles + (int)gridDim.x - 1) / (int)gridDim.x;
-    const int t0 = blockIdx.x * per, t1 = min(tiles, t0 + per);
-    if (t0 >= t1) return;
-    const size_t base = ((size_t)s * c.n_kv + h) * c.max_len;
-    const uint16_t *kp = c.k + (size_t)h * c.head_stride;
-    const uint32_t ko = (uint32_t)ln * (uint32_t)c.slot_stride + 8 * g;
-
-    int rb = 0;
-    do {   // once without rows: scores decay
-        const int rt = min(RB / 16, (rows - rb + 15) / 16);
-        if (rb) __syncthreads();
-        for (int r = threadIdx.x; r < 16 * rt; r += 64 * kScoreWaves) {
-            const int row = rb + r, i = row / d.G;
-            see[r] = 0;
-            ((float *)sl)[r] = 0.0f;
-            if (row < rows) {
-                const int ti = nth_bit(acc, i);
-                see[r] = token_mask(d, first + ti, ti);
-                ((float *)sl)[r] = J.lse[(size_t)(first + ti) * c.n_kv * d.G + h * d.G + row - i * d.G];
-            }
-        }
-        for (int r = wave; r < rt; r += kScoreWaves) {
-            const int row = rb + 16 * r + ln, i = row / d.G;
-            const bool on = row < rows;
-            const size_t at = on ? (size_t)(first + nth_bit(acc, i)) * d.ld_q + (size_t)(h * d.G + row - i * d.G) * d.hs_q + 8 * g : 0;
-            float f = d.scale;
-            if constexpr (QF) {
-                float x[C][8];
-                f = load_split<C, BF>((const float *)d.q + at, on, f, x);
-#pragma unroll
-                for (int k = 0; k < C; ++k) {
-                    uint4v p[QP];
-                    split8<BF, QP>(x[k], p);
-#pragma unroll
-                    for (int u = 0; u < QP; ++u) sq[r][u][k][lane] = p[u];
-                }
-            } else {
-#pragma unroll
-                for (int k = 0; k < C; ++k) sq[r][0][k][lane] = on ? *(const uint4v *)((const uint16_t *)d.q + at + 32 * k) : uint4v{0, 0, 0, 0};
-            }
-            if (g == 0) ((float *)sc)[16 * r + ln] = f;
-        }
-        __syncthreads();
-
-        uint4v kf[2][C];
-        // the tile's weights, summed over the rows: lane l < 32 has slot l's. hide: bit i of byte t set where row 4 g + i of
-        // the row tile does not see the lane's slot of half t
-        auto sum_rows = [&](bool draft, int tj0, int tj1) {
-            float w0 = 0.0f, w1 = 0.0f;
-            for (int r = 0; r < rt; ++r) {
-                const float4v l = sl[4 * r + g], f = sc[4 * r + g];
-                float4v s0 = {0, 0, 0, 0}, s1 = {0, 0, 0, 0};
-#pragma unroll
-                for (int u = QP - 1; u >= 0; --u)
-#pragma unroll
-                    for (int k = 0; k < C; ++k) {
-                        const uint4v q = sq[r][u][k][lane];
-                        s0 = mfma<BF>(q, kf[0][k], s0);
-                        s1 = mfma<BF>(q, kf[1][k], s1);
-                    }
-                const int left = rows - rb - 16 * r - 4 * g;   // rows of the lane's four that are there
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float e0 = __builtin_amdgcn_exp2f(fmaf(s0[i], f[i], -l[i]) * kLog2e), e1 = __builtin_amdgcn_exp2f(fmaf(s1[i], f[i], -l[i]) * kLog2e);
-                    if (draft) {
-                        const uint64_t m = see[16 * r + 4 * g + i];
-                        if (!(m >> tj0 & 1)) e0 = 0.0f;
-                        if (!(m >> tj1 & 1)) e1 = 0.0f;
-                    }
-                    w0 += i < left ? e0 : 0.0f;
-                    w1 += i < left ? e1 : 0.0f;
-                }
-            }
-            w0 += __shfl_xor(w0, 16);
-            w0 += __shfl_xor(w0, 32);
-            w1 += __shfl_xor(w1, 16);
-            w1 += __shfl_xor(w1, 32);
-            return lane < 16 ? w0 : w1;
-        };
-        auto put = [&](int slot, int end, bool old, float w, float before) {
-            if (lane < 32 && slot + lane < end) {
-                float *o = J.score_out + base + slot + lane;
-                *o = rb ? *o + w : old ? J.decay * before + w : w;
-            }
-        };
-
-        for (int tb = t0 + wave; tb < min(t1, ctx); tb += 32 * kScoreWaves) {
-            // offsets of the wave's next 64 halves, a lane each
-            int64_t off = -1;
-            {
-                const int t = tb + kScoreWaves * (lane >> 1), slot = 32 * t + 16 * (lane & 1);
-                if (t < min(t1, ctx) && slot < n) off = slot_offset(c, s, slot);
-            }
-            const int lo = (int)off, hi = (int)(off >> 32), many = min(32, (min(t1, ctx) - tb + kScoreWaves - 1) / kScoreWaves);
-            auto half = [&](int i) { return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, i) << 32 | (uint32_t)__builtin_amdgcn_readlane(lo, i)); };
-            for (int i = 0; i < many; ++i) {
-                const int slot = 32 * (tb + kScoreWaves * i);
-                const int64_t h0 = half(2 * i), h1 = half(2 * i + 1);
-                const bool on0 = h0 >= 0 && slot + ln < n, on1 = h1 >= 0 && slot + 16 + ln < n;
-                const float before = lane < 32 && slot + lane < n && !rb ? J.score[base + slot + lane] : 0.0f;
-#pragma unroll
-                for (int k = 0; k < C; ++k) {
-                    kf[0][k] = on0 ? *(const uint4v *)(kp + h0 + ko + 32 * k) : uint4v{0, 0, 0, 0};
-                    kf[1][k] = on1 ? *(const uint4v *)(kp + h1 + ko + 32 * k) : uint4v{0, 0, 0, 0};
-                }
-                float w = rt > 0 ? sum_rows(false, 0, 0) : 0.0f;
-                if ((lane < 16 ? h0 : h1) < 0) w = 0.0f;
-                put(slot, n, true, w, before);
-            }
-        }
-        for (int t = max(t0, ctx) + wave; t < t1; t += kScoreWaves) {   // accepted tokens
-            const int r0 = 32 * (t - ctx), j0 = r0 + ln < cnt ? nth_bit(acc, r0 + ln) : 0, j1 = r0 + 16 + ln < cnt ? nth_bit(acc, r0 + 16 + ln) : 0;
-#pragma unroll
-            for (int k = 0; k < C; ++k) {
-                kf[0][k] = draft8(d.k, (size_t)(first + j0) * d.ld_kv + (size_t)h * d.hs_kv + 32 * k + 8 * g, d.kv_f32, BF);
-                kf[1][k] = draft8(d.k, (size_t)(first + j1) * d.ld_kv + (size_t)h * d.hs_kv + 32 * k + 8 * g, d.kv_f32, BF);
-            }
-            put(n + r0, min(n + cnt, c.max_len), false, sum_rows(true, j0, j1), 0.0f);
-        }
-        rb += RB;
-    } while (rb < rows);
-}
-
-template <int D>
-static void score_types(const ScoreJob &J, dim3 grid, hipStream_t st) {
-    if (J.d.q_f32 && J.d.n_tokens) {
-        if (J.c.bf16) k_score<D, true, true><<<grid, 64 * kScoreWaves, 0, st>>>(J);
-        else k_score<D, false, true><<<grid, 64 * kScoreWaves, 0, st>>>(J);
-    } else {
-        if (J.c.bf16) k_score<D, true, false><<<grid, 64 * kScoreWaves, 0, st>>>(J);
-        else k_score<D, false, false><<<grid, 64 * kScoreWaves, 0, st>>>(J);
-    }
-}
-
-int launch_kv_score(const KvDev &c, const DraftDev &d, int D, const uint64_t *accept, const float *lse, float decay, const float *score,
-                    float *score_out, hipStream_t st) {
-    if (c.slot_stride >= (1u << 26)) return set_error(P8X_ERR_UNSUPPORTED, "p8x_kv_score: slot_stride %zu (below 2^26)", c.slot_stride);
-    const ScoreJob J{c, d, accept, lse, score, score_out, decay};
-    const int64_t heads = (int64_t)c.n_seq * c.n_kv, tiles = (c.max_len + 31) / 32 + 2;
-    const int nb = (int)std::max<int64_t>(1, std::min<int64_t>((tiles + kScoreWaves - 1) / kScoreWaves, (4 * num_cus() + heads - 1) / heads));
-    const dim3 grid(nb, c.n_kv, c.n_seq);
-    if (D == 64) score_types<64>(J, grid, st);
-    else if (D == 128) score_types<128>(J, grid, st);
-    else score_types<256>(J, grid, st);
-    return hip_check(hipGetLastError(), "p8x_kv_score launch");
 }
 
 }  // namespace p8x
