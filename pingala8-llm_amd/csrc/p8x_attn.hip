@@ -32,6 +32,7 @@ __host__ __device__ constexpr int attn_waves(int D) { return D == 256 ? 4 : 8; }
 constexpr float kLazy = 8.0f;   // log2 of how far a weight may exceed 1 before its row's maximum moves
 // tiles that a workgroup's waves share through LDS at a time
 __host__ __device__ constexpr int stage_tiles(int D) { return D == 256 ? 1 : 2; }
+constexpr int kStages = 4;   // stages in LDS: one in use, the others on their way
 
 struct AttnJob {
     KvDev c;
@@ -40,6 +41,7 @@ struct AttnJob {
     float *lse;
     unsigned *count;   // arrivals of a segment's workgroups, 0 between calls
     float *part;       // two records a workgroup: rows x D sums, then rows x (m, l)
+    int2 *where;       // of a segment: first workgroup, workgroups (for a join launch)
     int rw, rt, least; // row waves of a workgroup; row tiles of a sequence at most; units a workgroup takes at least
     int split;         // unit: a tile; 0: a whole segment (no records)
     int join;          // records are joined by a launch of their own
@@ -107,7 +109,11 @@ __device__ __forceinline__ Shares share_out(const AttnJob &J, int rows_wg) {
 template <int D, bool BF, bool QF, int NT, bool SHARE>
 struct Wave {
     static constexpr int C = D / 32, DV = D / 16, VW = DV / 2;       // K operands a row; elements and dwords of V a lane and slot
-    static constexpr int PC = D / 8, KP = PC + 1, VP = PC + 2;      // 16-byte pieces of a row; of one of K and V in LDS: the rows of a read in other banks
+    // 16-byte pieces of a row. In LDS a row's pieces lie at p ^ fk(row) (K) or p ^ fv(row) (V), so that the rows of a read are in
+    // other banks: 16 rows by 16 bytes of K (ds_read_b128), 8 rows by 32 bytes of V (ds_read_b64_tr_b16).
+    static constexpr int PC = D / 8, ROW = 2 * D;
+    static __device__ __forceinline__ int fk(int row) { return row & (PC < 16 ? PC - 1 : 15); }
+    static __device__ __forceinline__ int fv(int row) { return PC < 16 ? (row >> 1 & 3) << 1 : (row & 7) << 1; }
     static constexpr int QP = QF ? (BF ? 3 : 2) : 1, PP = QF && BF ? 3 : 2;   // 16-bit parts of a query and of a weight
     static constexpr float kBias = BF ? 0.0f : 7.0f;
     uint4v q[NT][QP][C];
@@ -176,24 +182,34 @@ struct Wave {
             load_v1(v + h1 + vo + j * ss, vf[j + 4]);
         }
     }
-    // k: the lane's piece of a tile in LDS (SHARE), else K is in its registers
-    __device__ __forceinline__ void qk(float (&x)[NT][8], const uint4v *k) {
+    // scores x[a][j] of slot j of the lane's eight; k: a tile in LDS (SHARE), else K is in its registers
+    __device__ __forceinline__ void qk(float (&x)[NT][8], const char *k) {
+        float4v s[2][NT];
+        if constexpr (SHARE) {
+            const int lane = threadIdx.x & 63, ln = lane & 15, at = ln * ROW + ((lane >> 4) ^ fk(ln)) * 16;   // pieces 4 c + g: c only flips higher bits
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            if constexpr (SHARE)
+            for (int c = 0; c < C; ++c)
 #pragma unroll
-                for (int c = 0; c < C; ++c) kf[t][c] = k[16 * t * KP + 4 * c];
-#pragma unroll
-            for (int a = 0; a < NT; ++a) {
-                float4v s = {0, 0, 0, 0};
-#pragma unroll
-                for (int n = QP - 1; n >= 0; --n)   // small parts first
-#pragma unroll
-                    for (int c = 0; c < C; ++c) s = mfma<BF>(kf[t][c], q[a][n][c], s);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) x[a][4 * t + i] = s[i];
-            }
+                for (int t = 0; t < 2; ++t) kf[t][c] = *(const uint4v *)(k + (at ^ 64 * c) + 16 * t * ROW);
         }
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int a = 0; a < NT; ++a) s[t][a] = float4v{0, 0, 0, 0};
+#pragma unroll
+        for (int n = QP - 1; n >= 0; --n)   // small parts first
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int a = 0; a < NT; ++a) s[t][a] = mfma<BF>(kf[t][c], q[a][n][c], s[t][a]);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int a = 0; a < NT; ++a)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[a][4 * t + i] = s[t][a][i];
     }
 
     // (NaN propagates; fmaxf would quiet each operand first, an instruction apiece)
@@ -249,12 +265,15 @@ struct Wave {
         }
     }
 
-    // V^T operands of output tiles 2 w and 2 w + 1; v: the lane's piece of a tile in LDS (SHARE)
-    __device__ __forceinline__ void operands(int w, const uint16_t *v, uint4v &e0, uint4v &e1) {
+    // V^T operands of output tiles 2 w and 2 w + 1; v: a tile in LDS (SHARE)
+    __device__ __forceinline__ void operands(int w, const char *v, uint4v &e0, uint4v &e1) {
         if constexpr (SHARE) {
             typedef short s4 __attribute__((ext_vector_type(4)));
-            auto tr = [&](int at) { return __builtin_bit_cast(uint2v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)(v + at))); };
-            const uint2v a = tr(32 * w), b = tr(32 * w + 16 * 8 * VP), c = tr(32 * w + 16), d = tr(32 * w + 16 + 16 * 8 * VP);
+            const int lane = threadIdx.x & 63, ln = lane & 15, row = 4 * (lane >> 4) + ln / 4, at = row * ROW + fv(row) * 16 + 8 * (ln & 3);
+            auto tr = [&](int t, int half) {
+                return __builtin_bit_cast(uint2v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)(v + (at ^ 32 * t) + 16 * half * ROW)));
+            };
+            const uint2v a = tr(2 * w, 0), b = tr(2 * w, 1), c = tr(2 * w + 1, 0), d = tr(2 * w + 1, 1);
             e0 = uint4v{a[0], a[1], b[0], b[1]};
             e1 = uint4v{c[0], c[1], d[0], d[1]};
         } else {
@@ -266,7 +285,7 @@ struct Wave {
         }
     }
 
-    __device__ __forceinline__ void pv(const float (&x)[NT][8], const uint16_t *v) {
+    __device__ __forceinline__ void pv(const float (&x)[NT][8], const char *v) {
         uint4v p[NT][PP];
 #pragma unroll
         for (int a = 0; a < NT; ++a) parts(x[a], p[a]);
@@ -275,21 +294,21 @@ struct Wave {
             uint4v e0, e1;
             operands(w, v, e0, e1);
 #pragma unroll
-            for (int a = 0; a < NT; ++a)
+            for (int n = PP - 1; n >= 0; --n)
 #pragma unroll
-                for (int n = PP - 1; n >= 0; --n) {
+                for (int a = 0; a < NT; ++a) {
                     o[a][2 * w] = mfma<BF>(e0, p[a][n], o[a][2 * w]);
                     o[a][2 * w + 1] = mfma<BF>(e1, p[a][n], o[a][2 * w + 1]);
                 }
         }
     }
-    __device__ __forceinline__ void tile(float (&x)[NT][8], const uint4v *k, const uint16_t *v) {
+    __device__ __forceinline__ void tile(float (&x)[NT][8], const char *k, const char *v) {
         qk(x, k);
         softmax(x);
         pv(x, v);
     }
     // A masked tile (rows that are not there: zeros): see[a] bit j = slot j of the 32 is seen by the lane's row.
-    __device__ __forceinline__ void masked(float (&x)[NT][8], const uint4v *k, const uint16_t *v, const uint32_t (&see)[NT], int lane) {
+    __device__ __forceinline__ void masked(float (&x)[NT][8], const char *k, const char *v, const uint32_t (&see)[NT], int lane) {
         qk(x, k);
 #pragma unroll
         for (int a = 0; a < NT; ++a) {
@@ -407,21 +426,12 @@ __device__ __forceinline__ void store_row(const AttnJob &J, int first, int h, in
 template <int D, bool BF, bool QF>
 __global__ __launch_bounds__(256) void k_attn_join(AttnJob J, int rows_wg) {
     __shared__ Part sh[8][32];
-    const int lane = threadIdx.x & 63, s = blockIdx.z / J.c.n_kv, h = blockIdx.z % J.c.n_kv, rt = blockIdx.y;
+    const int s = blockIdx.z / J.c.n_kv, h = blockIdx.z % J.c.n_kv, rt = blockIdx.y;
     const int sub = threadIdx.x >> 5, x4 = blockIdx.x * 32 + (threadIdx.x & 31), r = x4 / (D / 4), e = x4 % (D / 4) * 4;
-    const Shares w = share_out(J, rows_wg);
-    int base = 0;
-    for (int s0 = 0; s0 < s; s0 += 64) {
-        int v = 0;
-        if (s0 + lane < s) {
-            const Seq q = seq_of(J, s0 + lane, rows_wg);
-            v = J.c.n_kv * q.rts * w.units(q.tiles);
-        }
-        base += wave_sum(v);
-    }
+    const int2 at = J.where[(size_t)blockIdx.z * J.rt + rt];
     const Seq q = seq_of(J, s, rows_wg);
-    if (rt >= q.rts) return;
-    const int ps = w.units(q.tiles), sa = base + (h * q.rts + rt) * ps, p0 = sa / w.per, np = (sa + ps - 1) / w.per - p0 + 1;
+    if (rt >= q.rts || q.tiles == 0) return;
+    const int p0 = at.x, np = at.y;
     if (np < 2) return;
     const bool on = r < min(rows_wg, q.nt * J.d.G - rt * rows_wg);
     const int each = (np + 7) / 8;
@@ -434,17 +444,25 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnJob J, int rows_wg) {
     store_row<D, BF, QF>(J, q.first, h, rt * rows_wg + r, e, p);
 }
 
-// SHARE: the waves' rows are many; each tile of K and V is brought to LDS once for all of them, a stage of tiles ahead in
-// registers. Else each wave loads its tiles straight into operands.
+// 16 bytes a lane from base + off to LDS at `to` + 16 lane, without a wait. Written by hand: the compiler, which knows no other
+// wait than for all of these, would put one before every read of LDS. M0 holds `to` while the load is issued; five wait
+// states lie between it, or a VALU write of the base, and the load. Nothing is loaded into registers.
+__device__ __forceinline__ void load_lds(const uint16_t *base, uint32_t off, uint32_t to) {
+    uint32_t m0;
+    __asm__ volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0" : "=&s"(m0) : "v"(off), "s"(base), "s"(to) : "memory");
+}
+
+// SHARE: the waves' rows are many; each tile of K and V is brought to LDS once for all of them, three stages of tiles
+// ahead. Else each wave loads its tiles straight into operands.
 template <int D, bool BF, bool QF, int NT, bool SHARE>
 __global__ __launch_bounds__(64 * attn_waves(D)) void k_attn(AttnJob J) {
     constexpr int kWaves = attn_waves(D);
     typedef Wave<D, BF, QF, NT, SHARE> W;
     constexpr int R16 = 16 * NT, DV = W::DV, PC = W::PC;
-    extern __shared__ float4v sh4[];   // SHARE: two stages of K, V; then [wave][row][D + 4] sums, [wave][row] m, l
+    extern __shared__ float4v sh4[];   // SHARE: stages of K, V; then [wave][row][D + 4] sums, [wave][row] m, l
     __shared__ unsigned last;
-    __shared__ int paged[4][2 * stage_tiles(D)];   // SHARE: whether a stage's halves have a page
-    __shared__ int odd_row[4][32 * stage_tiles(D)];   // SHARE: drafted tokens with infinities or NaN among their values
+    __shared__ int paged[8][2 * stage_tiles(D)];   // SHARE: whether a stage's halves have a page
+    __shared__ int odd_row[8][32 * stage_tiles(D)];   // SHARE: drafted tokens with infinities or NaN among their values
     float *sh = (float *)sh4;
     const KvDev &c = J.c;
     const DraftDev &d = J.d;
@@ -498,15 +516,17 @@ __global__ __launch_bounds__(64 * attn_waves(D)) void k_attn(AttnJob J) {
         u = min(u1, sb);
         const int rows = q.nt * d.G, row0 = rt * rows_wg + rwi * R16;
         const uint16_t *kp = c.k + (size_t)h * c.head_stride, *vp = c.v + (size_t)h * c.head_stride;
-        float x[NT][8];
 
         if constexpr (SHARE) {
             constexpr int ST = stage_tiles(D), RWV = 64 / PC, RP = kWaves * RWV, PASS = 32 * ST / RP;   // rows of a wave and of the workgroup in a pass
-            uint4v *kb = (uint4v *)sh4, *vb = kb + 2 * 32 * ST * W::KP;
+            constexpr int STAGE = 32 * ST * W::ROW;   // bytes of a stage's K; its V follows
             const int rl = lane / PC, pl = lane % PC;
-            uint4v sk[PASS], sv[PASS];
+            char *const lds = (char *)sh4;
+            const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
             int lo = 0, hi = 0;
             const int stages = (t1 - t0 + ST - 1) / ST;
+            // Brings the wave's rows of stage st to LDS: straight there, asynchronously, where all of them are in use and have a
+            // page, else through registers, rows that are not there as zeros.
             auto load = [&](int st) {
                 constexpr int CH = 64 / PASS;   // stages whose row offsets the lanes hold
                 if (st % CH == 0) {
@@ -515,60 +535,80 @@ __global__ __launch_bounds__(64 * attn_waves(D)) void k_attn(AttnJob J) {
                     if (t < min(t1, ctx) && slot < q.n) off = slot_offset(c, s, slot & ~15);
                     lo = (int)off, hi = (int)(off >> 32);
                 }
+                const int buf = (st % kStages) * 2 * STAGE;
+                bool direct = true;
+                int64_t off[PASS];
 #pragma unroll
                 for (int p = 0; p < PASS; ++p) {
                     const int r0 = p * RP + wave * RWV, t = t0 + st * ST + r0 / 32, from = st % CH * PASS + p;
-                    const int64_t off = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, from) << 32 | (uint32_t)__builtin_amdgcn_readlane(lo, from));
-                    sk[p] = sv[p] = uint4v{0, 0, 0, 0};
+                    off[p] = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, from) << 32 | (uint32_t)__builtin_amdgcn_readlane(lo, from));
+                    direct = direct && t < min(t1, ctx) && off[p] >= 0 && 32 * t + r0 % 32 + RWV <= q.n;
+                    if (lane == 0 && r0 % 16 == 0) paged[st % 8][r0 / 16] = off[p] >= 0;
+                }
+                if (direct) {
+#pragma unroll
+                    for (int p = 0; p < PASS; ++p) {
+                        const uint32_t to = lds0 + buf + (p * RP + wave * RWV) * W::ROW;
+                        const uint16_t *kf = kp + off[p], *vf = vp + off[p];
+                        const int r15 = (p * RP + wave * RWV + rl) & 15;   // the lane's row; its bytes from the half's first slot:
+                        const uint32_t kl = 2 * (r15 * ss + 8 * (pl ^ W::fk(r15))), vl = 2 * (r15 * ss + 8 * (pl ^ W::fv(r15)));
+                        load_lds(kf, kl, to);
+                        load_lds(vf, vl, to + STAGE);
+                    }
+                    return;
+                }
+                __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the stages before have arrived (see the stage loop)
+#pragma unroll 1
+                for (int p = 0; p < PASS; ++p) {
+                    const int r0 = p * RP + wave * RWV, t = t0 + st * ST + r0 / 32, from = st % CH * PASS + p, r = r0 + rl;
+                    const int64_t offs = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, from) << 32 | (uint32_t)__builtin_amdgcn_readlane(lo, from));
+                    uint4v k = {0, 0, 0, 0}, v = {0, 0, 0, 0};
                     if (t < min(t1, ctx)) {
-                        if (off >= 0 && 32 * t + r0 % 32 + rl < q.n) {
-                            const size_t at = (size_t)off + (r0 % 16 + rl) * ss + 8 * pl;
-                            sk[p] = *(const uint4v *)(kp + at);
-                            sv[p] = *(const uint4v *)(vp + at);
+                        if (offs >= 0 && 32 * t + r % 32 < q.n) {
+                            const size_t at = (size_t)offs + (r % 16) * ss + 8 * pl;
+                            k = *(const uint4v *)(kp + at);
+                            v = *(const uint4v *)(vp + at);
                         }
                     } else if (t < t1) {
-                        const int j = 32 * (t - ctx) + r0 % 32 + rl;
+                        const int j = 32 * (t - ctx) + r % 32;
                         bool has = false;
                         if (j < q.nt) {
                             const size_t at = (size_t)(q.first + j) * d.ld_kv + (size_t)h * d.hs_kv + 8 * pl;
-                            sk[p] = draft8(d.k, at, d.kv_f32, BF);
-                            sv[p] = draft8(d.v, at, d.kv_f32, BF);
+                            k = draft8(d.k, at, d.kv_f32, BF);
+                            v = draft8(d.v, at, d.kv_f32, BF);
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
-                                uint32_t v = sv[p][e];
-                                has |= take_odd<BF>(v);
-                                sv[p][e] = v;
+                                uint32_t w4 = v[e];
+                                has |= take_odd<BF>(w4);
+                                v[e] = w4;
                             }
                         }
                         const uint64_t by = __ballot(has);
-                        if (pl == 0) odd_row[st & 3][r0 + rl] = (by >> (rl * PC) & (PC == 64 ? ~0ull : (1ull << PC) - 1)) != 0;
+                        if (pl == 0) odd_row[st % 8][r] = (by >> (rl * PC) & (PC == 64 ? ~0ull : (1ull << PC) - 1)) != 0;
                     }
-                    if (lane == 0 && r0 % 16 == 0) paged[st & 3][r0 / 16] = off >= 0;
+                    *(uint4v *)(lds + buf + r * W::ROW + (pl ^ W::fk(r)) * 16) = k;
+                    *(uint4v *)(lds + buf + STAGE + r * W::ROW + (pl ^ W::fv(r)) * 16) = v;
                 }
             };
-            auto put = [&](int st) {
-#pragma unroll
-                for (int p = 0; p < PASS; ++p) {
-                    const int r = (st & 1) * 32 * ST + p * RP + wave * RWV + rl;
-                    kb[r * W::KP + pl] = sk[p];
-                    vb[r * W::VP + pl] = sv[p];
-                }
-            };
-            load(0);
+            for (int st = 0; st < min(stages, kStages - 1); ++st) load(st);
             w.load_q(d, q.first, h, row0, rows, lane);
-            put(0);
-            if (stages > 1) load(1);
-            __syncthreads();
             for (int st = 0; st < stages; ++st) {
-                if (st + 1 < stages) put(st + 1);
-                if (st + 2 < stages) load(st + 2);
+                // Stage st has arrived, and the stage before is no longer read: its place takes stage st + kStages - 1. Loads come
+                // back in order, 2 PASS of each stage: the younger ones may be on their way (a stage that went through
+                // registers has waited for all before it; other loads make the wait longer, never shorter).
+                const int young = min(kStages - 2, stages - 1 - st);
+                if (young == 2) __asm__ volatile("s_waitcnt vmcnt(%0)" ::"n"(4 * PASS) : "memory");
+                else if (young == 1) __asm__ volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * PASS) : "memory");
+                else __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                __syncthreads();
+                if (st + kStages - 1 < stages) load(st + kStages - 1);
 #pragma unroll 1
                 for (int i = SW == 1 ? 0 : swi; i < ST; i += SW) {
                     const int t = t0 + st * ST + i, left = q.n - 32 * t;
                     if (t >= t1) break;
-                    const uint4v *kt = kb + ((st & 1) * ST + i) * 32 * W::KP + ln * W::KP + g;
-                    const uint16_t *vt = (const uint16_t *)(vb + ((st & 1) * ST + i) * 32 * W::VP) + (4 * g + ln / 4) * 8 * W::VP + 4 * (ln % 4);
-                    const int pg = __builtin_amdgcn_readfirstlane(paged[st & 3][2 * i] + 2 * paged[st & 3][2 * i + 1]);
+                    const char *kt = lds + (st % kStages) * 2 * STAGE + 32 * i * W::ROW, *vt = kt + STAGE;
+                    const int pg = __builtin_amdgcn_readfirstlane(paged[st % 8][2 * i] + 2 * paged[st % 8][2 * i + 1]);
+                    float x[NT][8];
                     if (left >= 32 && pg == 3) {
                         w.tile(x, kt, vt);
                     } else {
@@ -578,12 +618,13 @@ __global__ __launch_bounds__(64 * attn_waves(D)) void k_attn(AttnJob J) {
                             for (int a = 0; a < NT; ++a) see[a] = (left >= 32 ? 0xFFFFFFFFu : (1u << left) - 1) & ((pg & 1 ? 0xFFFFu : 0) | (pg & 2 ? 0xFFFF0000u : 0));
                         w.masked(x, kt, vt, see, lane);
                         if (t >= ctx) {
-                            const uint32_t odd = (uint32_t)__ballot(lane < 32 && odd_row[st & 3][32 * i + lane]);
+                            const uint32_t odd = (uint32_t)__ballot(lane < 32 && odd_row[st % 8][32 * i + lane]);
                             if (odd) w.add_odd(odd, see, d, q.first + 32 * (t - ctx), h, lane);
                         }
                     }
                 }
-                __syncthreads();            }
+            }
+            __syncthreads();   // the stages' place is free
         } else {
             const int full = min(t1, q.n / 32);   // tiles of 32 slots in use
             bool have_q = false;
@@ -603,6 +644,7 @@ __global__ __launch_bounds__(64 * attn_waves(D)) void k_attn(AttnJob J) {
                 have_q = true;
                 for (int i = 0; i < many; ++i) {
                     const int64_t n0 = half(2 * min(i + 1, many - 1)), n1 = half(2 * min(i + 1, many - 1) + 1);
+                    float x[NT][8];
                     w.qk(x, nullptr);
                     if (i + 1 < many) w.load_k(kp, max(n0, (int64_t)0), max(n1, (int64_t)0), ko);
                     if ((h0 | h1) < 0) {   // a half without a page: hidden, its values zeros
@@ -673,6 +715,7 @@ __global__ __launch_bounds__(64 * attn_waves(D)) void k_attn(AttnJob J) {
                         for (int k = 0; k < 4; ++k)
                             if (by >> (16 * k) & 0xFFFF) odd |= 1u << ((j < 4 ? 0 : 12) + 4 * k + j);
                     }
+                float x[NT][8];
                 w.masked(x, nullptr, nullptr, see, lane);
                 if (odd) w.add_odd(odd, see, d, q.first + j0, h, lane);
             }
@@ -682,6 +725,7 @@ __global__ __launch_bounds__(64 * attn_waves(D)) void k_attn(AttnJob J) {
         const int here = min(rows_wg, rows - rt * rows_wg);
         const int p0 = sa / per, np = (sb - 1) / per - p0 + 1;   // the segment's workgroups p0 .. p0 + np - 1
         const size_t rec = (size_t)rows_wg * (D + 2);
+        if (J.join && t0 == 0 && threadIdx.x == 0) J.where[((size_t)s * c.n_kv + h) * J.rt + rt] = make_int2(p0, np);
         float *mine = whole ? nullptr : J.part + (2 * (size_t)wg + (sa < wg * per ? 0 : 1)) * rec;
         auto leave = [&](int r, int e, const Part &p) {   // row r of the row tile
             if (whole) {
@@ -796,7 +840,7 @@ static AttnPlan attn_plan(const KvDev &c, const DraftDev &d, int D) {
     p.rows_wg = 16 * p.nt * p.rw;
     p.rt = (rows + p.rows_wg - 1) / p.rows_wg;
     p.segs = (size_t)c.n_seq * c.n_kv * p.rt;
-    p.head_bytes = (4 * p.segs + 255) / 256 * 256;
+    p.head_bytes = (12 * p.segs + 8 + 255) / 256 * 256;   // counters, then places
     p.rec_bytes = 4 * (size_t)p.rows_wg * (D + 2);
     return p;
 }
@@ -809,7 +853,7 @@ size_t attn_workspace(const KvDev &c, const DraftDev &d, int D) {
 template <int D, bool BF, bool QF, int NT, bool SHARE>
 static int attn_run(const AttnJob &J, int rows_wg, hipStream_t st) {
     constexpr int waves = attn_waves(D);
-    constexpr int sums = waves * 16 * NT * (D + 4 + 2) * 4, stages = SHARE ? 2 * 32 * stage_tiles(D) * (2 * 2 * D + 16 + 32) : 0;
+    constexpr int sums = waves * 16 * NT * (D + 4 + 2) * 4, stages = SHARE ? kStages * 2 * 32 * stage_tiles(D) * 2 * D : 0;
     const int lds = SHARE && J.rw == waves ? std::max(stages, waves * 64 * (int)sizeof(Part)) : std::max(sums, stages);
     static const hipError_t e = hipFuncSetAttribute((const void *)k_attn<D, BF, QF, NT, SHARE>, hipFuncAttributeMaxDynamicSharedMemorySize, std::max(sums, stages));
     if (e != hipSuccess) return hip_check(e, "p8x_attn_tree LDS");
@@ -838,7 +882,7 @@ int launch_attn_tree(const KvDev &c, const DraftDev &d, int D, void *out, size_t
     const size_t most = p.segs * ((size_t)(c.max_len + 31) / 32 + 2);   // tiles
     if (most >= (1u << 29)) return set_error(P8X_ERR_UNSUPPORTED, "p8x_attn_tree: %zu tiles of 32 slots (fewer than 2^29)", most);
     if (c.slot_stride >= (1u << 26)) return set_error(P8X_ERR_UNSUPPORTED, "p8x_attn_tree: slot_stride %zu (below 2^26)", c.slot_stride);
-    AttnJob J{c, d, out, ldo, hso, lse, (unsigned *)ws, (float *)((char *)ws + p.head_bytes), p.rw, p.rt, attn_waves(D) / p.rw, 1, 0, 0};
+    AttnJob J{c, d, out, ldo, hso, lse, (unsigned *)ws, (float *)((char *)ws + p.head_bytes), (int2 *)((char *)ws + (4 * p.segs + 7) / 8 * 8), p.rw, p.rt, attn_waves(D) / p.rw, 1, 0, 0};
     const size_t room = ws_bytes > p.head_bytes ? (ws_bytes - p.head_bytes) / (2 * p.rec_bytes) : 0;   // workgroups with records
     int nwg = (int)std::min<size_t>(num_cus(), room);
     if (nwg < 16 || p.segs / p.rt > 65535 || p.rt > 65535) {   // whole segments then
