@@ -27,8 +27,9 @@
 
 namespace p8x {
 
-// waves of a workgroup, one of which a compute unit holds: 256 registers a lane, or 512 for rows of 256 elements
-__host__ __device__ constexpr int attn_waves(int D) { return D == 256 ? 4 : 8; }
+// Waves of a workgroup, one of which a compute unit holds: 8 of 256 registers a lane, or 4 of 512 for rows of 256 elements.
+// SHARE: the waves that share K and V through LDS, 0 for none.
+__host__ __device__ constexpr int attn_waves(int D, int share) { return share ? share : D == 256 ? 4 : 8; }
 constexpr float kLazy = 8.0f;   // log2 of how far a weight may exceed 1 before its row's maximum moves
 // tiles that a workgroup's waves share through LDS at a time
 __host__ __device__ constexpr int stage_tiles(int D) { return D == 256 ? 1 : 2; }
@@ -63,27 +64,38 @@ __device__ __forceinline__ int wave_sum(int v) {
     return __builtin_amdgcn_readfirstlane(v);
 }
 
-// How the tiles are shared out: `per` units a workgroup, units of a segment of `tiles` tiles. The same in every wave.
+// How the tiles are shared out: `per` units a workgroup, units of a segment of `tiles` tiles. The same in every wave. A lane
+// holds the numbers of one of the first 64 sequences; those of others are read again.
 struct Shares {
     int per, aligned, split, total;
+    int tiles, segs;   // of the lane's sequence: tiles of a segment, segments
     __device__ __forceinline__ int units(int tiles) const { return !split ? tiles > 0 : aligned ? (tiles + per - 1) / per * per : tiles; }
 };
+// f(tiles, segments) for the lane's sequence of s0 .. s0 + 63
+template <typename F>
+__device__ __forceinline__ int lane_seq(const AttnJob &J, int rows_wg, const Shares &h, int s0, F f) {
+    const int s = s0 + (threadIdx.x & 63);
+    if (s0 == 0) return f(h.tiles, h.segs);
+    if (s >= J.c.n_seq) return 0;
+    const Seq q = seq_of(J, s, rows_wg);
+    return f(q.tiles, J.c.n_kv * q.rts);
+}
 __device__ __forceinline__ Shares share_out(const AttnJob &J, int rows_wg) {
     const int lane = threadIdx.x & 63, n_seq = J.c.n_seq;
-    // f(tiles) summed over all segments
-    auto over = [&](auto f) {
+    Shares h;
+    h.tiles = h.segs = 0;
+    if (lane < n_seq) {
+        const Seq q = seq_of(J, lane, rows_wg);
+        h.tiles = q.tiles, h.segs = J.c.n_kv * q.rts;
+    }
+    auto over = [&](auto f) {   // f(tiles) summed over all segments
         int t = 0;
         for (int s0 = 0; s0 < n_seq; s0 += 64) {
-            int v = 0;
-            if (s0 + lane < n_seq) {
-                const Seq q = seq_of(J, s0 + lane, rows_wg);
-                v = J.c.n_kv * q.rts * f(q.tiles);
-            }
+            const int v = lane_seq(J, rows_wg, h, s0, [&](int tiles, int segs) { return segs * f(tiles); });
             t += n_seq > 1 ? wave_sum(v) : __builtin_amdgcn_readfirstlane(v);
         }
         return t;
     };
-    Shares h;
     h.split = J.split;
     h.aligned = 0;
     if (!J.split) {
@@ -106,7 +118,7 @@ __device__ __forceinline__ Shares share_out(const AttnJob &J, int rows_wg) {
     return h;
 }
 
-template <int D, bool BF, bool QF, int NT, bool SHARE>
+template <int D, bool BF, bool QF, int NT, int SHARE>
 struct Wave {
     static constexpr int C = D / 32, DV = D / 16, VW = DV / 2;       // K operands a row; elements and dwords of V a lane and slot
     // 16-byte pieces of a row. In LDS a row's pieces lie at p ^ fk(row) (K) or p ^ fv(row) (V), so that the rows of a read are in
@@ -120,7 +132,8 @@ struct Wave {
     float4v o[NT][DV];
     float m[NT], l[NT], c2[NT];
     uint4v kf[2][C];
-    uint32_t vf[8][VW];
+    uint32_t vf[SHARE ? 1 : 8][VW];
+    uint4v ve[SHARE ? DV : 1];
 
     // the lane's rows' queries; a negative scale's sign goes into them
     __device__ __forceinline__ void load_q(const DraftDev &d, int first, int h, int row0, int rows, int lane) {
@@ -182,16 +195,30 @@ struct Wave {
             load_v1(v + h1 + vo + j * ss, vf[j + 4]);
         }
     }
-    // scores x[a][j] of slot j of the lane's eight; k: a tile in LDS (SHARE), else K is in its registers
-    __device__ __forceinline__ void qk(float (&x)[NT][8], const char *k) {
-        float4v s[2][NT];
-        if constexpr (SHARE) {
-            const int lane = threadIdx.x & 63, ln = lane & 15, at = ln * ROW + ((lane >> 4) ^ fk(ln)) * 16;   // pieces 4 c + g: c only flips higher bits
+    // the same operands from a tile in LDS; ve: V^T operands of the output tiles
+    __device__ __forceinline__ void lds_k(const char *k) {
+        const int lane = threadIdx.x & 63, ln = lane & 15, at = ln * ROW + ((lane >> 4) ^ fk(ln)) * 16;   // pieces 4 c + g: c only flips higher bits
 #pragma unroll
-            for (int c = 0; c < C; ++c)
+        for (int c = 0; c < C; ++c)
 #pragma unroll
-                for (int t = 0; t < 2; ++t) kf[t][c] = *(const uint4v *)(k + (at ^ 64 * c) + 16 * t * ROW);
+            for (int t = 0; t < 2; ++t) kf[t][c] = *(const uint4v *)(k + (at ^ 64 * c) + 16 * t * ROW);
+    }
+    __device__ __forceinline__ void lds_v(const char *v) {
+        typedef short s4 __attribute__((ext_vector_type(4)));
+        const int lane = threadIdx.x & 63, ln = lane & 15, row = 4 * (lane >> 4) + ln / 4, at = row * ROW + fv(row) * 16 + 8 * (ln & 3);
+#pragma unroll
+        for (int t = 0; t < DV; ++t) {
+            uint2v e[2];
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+                e[half] = __builtin_bit_cast(uint2v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)(v + (at ^ 32 * t) + 16 * half * ROW)));
+            ve[t] = uint4v{e[0][0], e[0][1], e[1][0], e[1][1]};
         }
+    }
+
+    // scores x[a][j] of slot j of the lane's eight
+    __device__ __forceinline__ void qk(float (&x)[NT][8]) {
+        float4v s[2][NT];
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -265,34 +292,22 @@ struct Wave {
         }
     }
 
-    // V^T operands of output tiles 2 w and 2 w + 1; v: a tile in LDS (SHARE)
-    __device__ __forceinline__ void operands(int w, const char *v, uint4v &e0, uint4v &e1) {
-        if constexpr (SHARE) {
-            typedef short s4 __attribute__((ext_vector_type(4)));
-            const int lane = threadIdx.x & 63, ln = lane & 15, row = 4 * (lane >> 4) + ln / 4, at = row * ROW + fv(row) * 16 + 8 * (ln & 3);
-            auto tr = [&](int t, int half) {
-                return __builtin_bit_cast(uint2v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)(v + (at ^ 32 * t) + 16 * half * ROW)));
-            };
-            const uint2v a = tr(2 * w, 0), b = tr(2 * w, 1), c = tr(2 * w + 1, 0), d = tr(2 * w + 1, 1);
-            e0 = uint4v{a[0], a[1], b[0], b[1]};
-            e1 = uint4v{c[0], c[1], d[0], d[1]};
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                e0[j] = __builtin_amdgcn_perm(vf[2 * j + 1][w], vf[2 * j][w], 0x05040100u);
-                e1[j] = __builtin_amdgcn_perm(vf[2 * j + 1][w], vf[2 * j][w], 0x07060302u);
-            }
-        }
-    }
-
-    __device__ __forceinline__ void pv(const float (&x)[NT][8], const char *v) {
+    __device__ __forceinline__ void pv(const float (&x)[NT][8]) {
         uint4v p[NT][PP];
 #pragma unroll
         for (int a = 0; a < NT; ++a) parts(x[a], p[a]);
 #pragma unroll
-        for (int w = 0; w < VW; ++w) {
+        for (int w = 0; w < VW; ++w) {   // output tiles 2 w and 2 w + 1
             uint4v e0, e1;
-            operands(w, v, e0, e1);
+            if constexpr (SHARE) {
+                e0 = ve[2 * w], e1 = ve[2 * w + 1];
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    e0[j] = __builtin_amdgcn_perm(vf[2 * j + 1][w], vf[2 * j][w], 0x05040100u);
+                    e1[j] = __builtin_amdgcn_perm(vf[2 * j + 1][w], vf[2 * j][w], 0x07060302u);
+                }
+            }
 #pragma unroll
             for (int n = PP - 1; n >= 0; --n)
 #pragma unroll
@@ -302,23 +317,15 @@ struct Wave {
                 }
         }
     }
-    __device__ __forceinline__ void tile(float (&x)[NT][8], const char *k, const char *v) {
-        qk(x, k);
-        softmax(x);
-        pv(x, v);
-    }
-    // A masked tile (rows that are not there: zeros): see[a] bit j = slot j of the 32 is seen by the lane's row.
-    __device__ __forceinline__ void masked(float (&x)[NT][8], const char *k, const char *v, const uint32_t (&see)[NT], int lane) {
-        qk(x, k);
+    // hides from the lane's rows the slots whose bit of see[a] (j: slot j of the 32) is not set
+    __device__ __forceinline__ void hide(float (&x)[NT][8], const uint32_t (&see)[NT]) {
 #pragma unroll
         for (int a = 0; a < NT; ++a) {
-            const uint32_t lo = see[a] >> (4 * (lane >> 4)), hi = lo >> 16;
+            const uint32_t lo = see[a] >> (4 * ((threadIdx.x & 63) >> 4)), hi = lo >> 16;
 #pragma unroll
             for (int j = 0; j < 8; ++j)
                 if (!((j < 4 ? lo >> j : hi >> (j - 4)) & 1)) x[a][j] = -INFINITY;
         }
-        softmax(x);
-        pv(x, v);
     }
     // A drafted token's infinities and NaN, which must not meet the zero weight of a row that does not see the token, are
     // zeros in the product; here they are added to the rows that do. odd: the tokens of the tile (from row tok0 on) that have any.
@@ -454,9 +461,9 @@ __device__ __forceinline__ void load_lds(const uint16_t *base, uint32_t off, uin
 
 // SHARE: the waves' rows are many; each tile of K and V is brought to LDS once for all of them, three stages of tiles
 // ahead. Else each wave loads its tiles straight into operands.
-template <int D, bool BF, bool QF, int NT, bool SHARE>
-__global__ __launch_bounds__(64 * attn_waves(D)) void k_attn(AttnJob J) {
-    constexpr int kWaves = attn_waves(D);
+template <int D, bool BF, bool QF, int NT, int SHARE>
+__global__ __launch_bounds__(64 * attn_waves(D, SHARE)) void k_attn(AttnJob J) {
+    constexpr int kWaves = attn_waves(D, SHARE);
     typedef Wave<D, BF, QF, NT, SHARE> W;
     constexpr int R16 = 16 * NT, DV = W::DV, PC = W::PC;
     extern __shared__ float4v sh4[];   // SHARE: stages of K, V; then [wave][row][D + 4] sums, [wave][row] m, l
@@ -478,11 +485,7 @@ __global__ __launch_bounds__(64 * attn_waves(D)) void k_attn(AttnJob J) {
     int s = 0, base = 0;
     if (c.n_seq > 1)
         for (int s0 = 0; s0 < c.n_seq; s0 += 64) {
-            int v = 0;
-            if (s0 + lane < c.n_seq) {
-                const Seq q = seq_of(J, s0 + lane, rows_wg);
-                v = c.n_kv * q.rts * share.units(q.tiles);
-            }
+            const int v = lane_seq(J, rows_wg, share, s0, [&](int tiles, int segs) { return segs * share.units(tiles); });
             int x = v;
             for (int o = 1; o < 64; o <<= 1) {
                 const int y = __shfl_up(x, o);
@@ -590,40 +593,61 @@ __global__ __launch_bounds__(64 * attn_waves(D)) void k_attn(AttnJob J) {
                     *(uint4v *)(lds + buf + STAGE + r * W::ROW + (pl ^ W::fv(r)) * 16) = v;
                 }
             };
-            for (int st = 0; st < min(stages, kStages - 1); ++st) load(st);
             w.load_q(d, q.first, h, row0, rows, lane);
-            for (int st = 0; st < stages; ++st) {
-                // Stage st has arrived, and the stage before is no longer read: its place takes stage st + kStages - 1. Loads come
-                // back in order, 2 PASS of each stage: the younger ones may be on their way (a stage that went through
-                // registers has waited for all before it; other loads make the wait longer, never shorter).
+            for (int st = 0; st < min(stages, kStages - 1); ++st) load(st);
+            // Waits until stage st has arrived; the stage before it is no longer read then, and its place takes stage st +
+            // kStages - 1. Loads come back in order, 2 PASS of each stage: the younger ones may be on their way (a stage that went
+            // through registers has waited for all before it; other loads make the wait longer, never shorter).
+            auto arrive = [&](int st) {
                 const int young = min(kStages - 2, stages - 1 - st);
                 if (young == 2) __asm__ volatile("s_waitcnt vmcnt(%0)" ::"n"(4 * PASS) : "memory");
                 else if (young == 1) __asm__ volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * PASS) : "memory");
                 else __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
                 __syncthreads();
                 if (st + kStages - 1 < stages) load(st + kStages - 1);
+            };
+            auto place = [&](int t) { return lds + ((t - t0) / ST % kStages) * 2 * STAGE + 32 * ((t - t0) % ST) * W::ROW; };
+            arrive(0);
+            w.lds_k(place(t0));
+            uint32_t odd[2] = {0, 0};
+            // One body for all tiles, so that the sums stay in their registers. V of a tile and K of the next come from LDS while the
+            // scores become weights (the barriers to the scheduler keep it from moving the reads to their uses).
 #pragma unroll 1
-                for (int i = SW == 1 ? 0 : swi; i < ST; i += SW) {
-                    const int t = t0 + st * ST + i, left = q.n - 32 * t;
-                    if (t >= t1) break;
-                    const char *kt = lds + (st % kStages) * 2 * STAGE + 32 * i * W::ROW, *vt = kt + STAGE;
-                    const int pg = __builtin_amdgcn_readfirstlane(paged[st % 8][2 * i] + 2 * paged[st % 8][2 * i + 1]);
-                    float x[NT][8];
-                    if (left >= 32 && pg == 3) {
-                        w.tile(x, kt, vt);
-                    } else {
-                        uint32_t see[NT];
-                        if (t >= ctx) draft_mask<NT>(d, q, 32 * (t - ctx), row0, rows, ln, see);
-                        else
-                            for (int a = 0; a < NT; ++a) see[a] = (left >= 32 ? 0xFFFFFFFFu : (1u << left) - 1) & ((pg & 1 ? 0xFFFFu : 0) | (pg & 2 ? 0xFFFF0000u : 0));
-                        w.masked(x, kt, vt, see, lane);
-                        if (t >= ctx) {
-                            const uint32_t odd = (uint32_t)__ballot(lane < 32 && odd_row[st % 8][32 * i + lane]);
-                            if (odd) w.add_odd(odd, see, d, q.first + 32 * (t - ctx), h, lane);
-                        }
-                    }
+            for (int t = t0; t < t1; ++t) {
+                const int st = (t - t0) / ST, i = (t - t0) % ST, left = q.n - 32 * t;
+                float x[NT][8];
+                w.qk(x);
+                __builtin_amdgcn_sched_barrier(0);
+                w.lds_v(place(t) + STAGE);
+                uint32_t in = (paged[st % 8][2 * i] ? 0xFFFFu : 0) | (paged[st % 8][2 * i + 1] ? 0xFFFF0000u : 0);
+                in = t < ctx ? __builtin_amdgcn_readfirstlane(in) & (left >= 32 ? 0xFFFFFFFFu : (1u << left) - 1) : 0;
+                if (t >= ctx) {
+                    const uint32_t o = (uint32_t)__ballot(lane < 32 && odd_row[st % 8][32 * i + lane]);
+                    if (t == ctx) odd[0] = o;
+                    else odd[1] = o;
                 }
+                if (t + 1 < t1) {
+                    if (i == ST - 1) arrive(st + 1);
+                    w.lds_k(place(t + 1));
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                if (in != 0xFFFFFFFFu) {
+                    uint32_t see[NT];
+                    if (t >= ctx) draft_mask<NT>(d, q, 32 * (t - ctx), row0, rows, ln, see);
+                    else
+                        for (int a = 0; a < NT; ++a) see[a] = in;
+                    w.hide(x, see);
+                }
+                w.softmax(x);
+                w.pv(x);
             }
+#pragma unroll 1
+            for (int j = 0; j < 2; ++j)
+                if (const uint32_t o = j ? odd[1] : odd[0]) {
+                    uint32_t see[NT];
+                    draft_mask<NT>(d, q, 32 * j, row0, rows, ln, see);
+                    w.add_odd(o, see, d, q.first + 32 * j, h, lane);
+                }
             __syncthreads();   // the stages' place is free
         } else {
             const int full = min(t1, q.n / 32);   // tiles of 32 slots in use
@@ -645,7 +669,7 @@ __global__ __launch_bounds__(64 * attn_waves(D)) void k_attn(AttnJob J) {
                 for (int i = 0; i < many; ++i) {
                     const int64_t n0 = half(2 * min(i + 1, many - 1)), n1 = half(2 * min(i + 1, many - 1) + 1);
                     float x[NT][8];
-                    w.qk(x, nullptr);
+                    w.qk(x);
                     if (i + 1 < many) w.load_k(kp, max(n0, (int64_t)0), max(n1, (int64_t)0), ko);
                     if ((h0 | h1) < 0) {   // a half without a page: hidden, its values zeros
 #pragma unroll
@@ -657,7 +681,7 @@ __global__ __launch_bounds__(64 * attn_waves(D)) void k_attn(AttnJob J) {
                         }
                     }
                     w.softmax(x);
-                    w.pv(x, nullptr);
+                    w.pv(x);
                     if (i + 1 < many) w.load_v(vp, max(n0, (int64_t)0), max(n1, (int64_t)0), vo, ss);
                     h0 = n0, h1 = n1;
                 }
@@ -716,7 +740,10 @@ __global__ __launch_bounds__(64 * attn_waves(D)) void k_attn(AttnJob J) {
                             if (by >> (16 * k) & 0xFFFF) odd |= 1u << ((j < 4 ? 0 : 12) + 4 * k + j);
                     }
                 float x[NT][8];
-                w.masked(x, nullptr, nullptr, see, lane);
+                w.qk(x);
+                w.hide(x, see);
+                w.softmax(x);
+                w.pv(x);
                 if (odd) w.add_odd(odd, see, d, q.first + j0, h, lane);
             }
         }
@@ -825,18 +852,23 @@ __global__ __launch_bounds__(64 * attn_waves(D)) void k_attn(AttnJob J) {
     }
 }
 
-// Rows a wave and row waves a workgroup: 16 rows while they hold all, else 32 (16 with queries of several parts or
-// wide rows, whose operands fill the registers).
+// Rows of a wave and row waves of a workgroup. Up to 32 rows: 16 or 32 in every wave (16 with queries of several parts or rows
+// of 256 elements, whose operands fill the registers), the waves take slots in turn. More: 4 or 8 waves share K and V through
+// LDS, each with 16 or 32 of the rows.
 constexpr size_t kJoinBytes = 96 << 10;   // records of a segment of more bytes than this are joined by a launch of their own
 struct AttnPlan { int nt, rw, rows_wg, rt, share; size_t segs, rec_bytes, head_bytes; };
 static AttnPlan attn_plan(const KvDev &c, const DraftDev &d, int D) {
-    const int waves = attn_waves(D);
     AttnPlan p;
     const int rows = d.max_tokens * d.G;
-    p.nt = rows <= 16 || d.q_f32 || D == 256 ? 1 : 2;
-    p.rw = 1;
-    while (p.rw < waves && p.rw * 16 * p.nt < rows) p.rw *= 2;
-    p.share = waves / p.rw <= stage_tiles(D);
+    if (rows > 32) {
+        p.share = rows <= 64 || D == 256 ? 4 : 8;
+        p.nt = rows > 16 * p.share && !d.q_f32 && D < 256 ? 2 : 1;
+        p.rw = p.share;
+    } else {
+        p.share = 0;
+        p.nt = rows <= 16 || d.q_f32 || D == 256 ? 1 : 2;
+        p.rw = rows > 16 * p.nt ? 2 : 1;
+    }
     p.rows_wg = 16 * p.nt * p.rw;
     p.rt = (rows + p.rows_wg - 1) / p.rows_wg;
     p.segs = (size_t)c.n_seq * c.n_kv * p.rt;
@@ -850,30 +882,33 @@ size_t attn_workspace(const KvDev &c, const DraftDev &d, int D) {
     return p.head_bytes + 2 * (size_t)num_cus() * p.rec_bytes;
 }
 
-template <int D, bool BF, bool QF, int NT, bool SHARE>
+template <int D, bool BF, bool QF, int NT, int SHARE>
 static int attn_run(const AttnJob &J, int rows_wg, hipStream_t st) {
-    constexpr int waves = attn_waves(D);
-    constexpr int sums = waves * 16 * NT * (D + 4 + 2) * 4, stages = SHARE ? kStages * 2 * 32 * stage_tiles(D) * 2 * D : 0;
-    const int lds = SHARE && J.rw == waves ? std::max(stages, waves * 64 * (int)sizeof(Part)) : std::max(sums, stages);
-    static const hipError_t e = hipFuncSetAttribute((const void *)k_attn<D, BF, QF, NT, SHARE>, hipFuncAttributeMaxDynamicSharedMemorySize, std::max(sums, stages));
+    constexpr int waves = attn_waves(D, SHARE);
+    constexpr int lds = SHARE ? kStages * 2 * 32 * stage_tiles(D) * 2 * D : waves * 16 * NT * (D + 4 + 2) * 4;
+    static const hipError_t e = hipFuncSetAttribute((const void *)k_attn<D, BF, QF, NT, SHARE>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e != hipSuccess) return hip_check(e, "p8x_attn_tree LDS");
     k_attn<D, BF, QF, NT, SHARE><<<J.nwg, 64 * waves, lds, st>>>(J);
     if (J.join) k_attn_join<D, BF, QF><<<dim3((rows_wg * (D / 4) + 31) / 32, J.rt, J.c.n_seq * J.c.n_kv), 256, 0, st>>>(J, rows_wg);
     return hip_check(hipGetLastError(), "p8x_attn_tree launch");
 }
 
-template <int D, bool BF, bool QF, int NT>
+template <int D, bool BF, bool QF>
 static int attn_form(const AttnJob &J, const AttnPlan &p, hipStream_t st) {
-    return p.share ? attn_run<D, BF, QF, NT, true>(J, p.rows_wg, st) : attn_run<D, BF, QF, NT, false>(J, p.rows_wg, st);
+    if constexpr (D < 256) {
+        if constexpr (!QF) {
+            if (p.share == 8 && p.nt == 2) return attn_run<D, BF, QF, 2, 8>(J, p.rows_wg, st);
+            if (!p.share && p.nt == 2) return attn_run<D, BF, QF, 2, 0>(J, p.rows_wg, st);
+        }
+        if (p.share == 8) return attn_run<D, BF, QF, 1, 8>(J, p.rows_wg, st);
+    }
+    return p.share ? attn_run<D, BF, QF, 1, 4>(J, p.rows_wg, st) : attn_run<D, BF, QF, 1, 0>(J, p.rows_wg, st);
 }
 
 template <int D>
 static int attn_types(const AttnJob &J, const AttnPlan &p, hipStream_t st) {
-    const bool bf = J.c.bf16;
-    if (J.d.q_f32) return bf ? attn_form<D, true, true, 1>(J, p, st) : attn_form<D, false, true, 1>(J, p, st);
-    if constexpr (D < 256)
-        if (p.nt == 2) return bf ? attn_form<D, true, false, 2>(J, p, st) : attn_form<D, false, false, 2>(J, p, st);
-    return bf ? attn_form<D, true, false, 1>(J, p, st) : attn_form<D, false, false, 1>(J, p, st);
+    if (J.d.q_f32) return J.c.bf16 ? attn_form<D, true, true>(J, p, st) : attn_form<D, false, true>(J, p, st);
+    return J.c.bf16 ? attn_form<D, true, false>(J, p, st) : attn_form<D, false, false>(J, p, st);
 }
 
 int launch_attn_tree(const KvDev &c, const DraftDev &d, int D, void *out, size_t ldo, size_t hso, float *lse, void *ws, size_t ws_bytes,
@@ -882,7 +917,7 @@ int launch_attn_tree(const KvDev &c, const DraftDev &d, int D, void *out, size_t
     const size_t most = p.segs * ((size_t)(c.max_len + 31) / 32 + 2);   // tiles
     if (most >= (1u << 29)) return set_error(P8X_ERR_UNSUPPORTED, "p8x_attn_tree: %zu tiles of 32 slots (fewer than 2^29)", most);
     if (c.slot_stride >= (1u << 26)) return set_error(P8X_ERR_UNSUPPORTED, "p8x_attn_tree: slot_stride %zu (below 2^26)", c.slot_stride);
-    AttnJob J{c, d, out, ldo, hso, lse, (unsigned *)ws, (float *)((char *)ws + p.head_bytes), (int2 *)((char *)ws + (4 * p.segs + 7) / 8 * 8), p.rw, p.rt, attn_waves(D) / p.rw, 1, 0, 0};
+    AttnJob J{c, d, out, ldo, hso, lse, (unsigned *)ws, (float *)((char *)ws + p.head_bytes), (int2 *)((char *)ws + (4 * p.segs + 7) / 8 * 8), p.rw, p.rt, attn_waves(D, p.share) / p.rw, 1, 0, 0};
     const size_t room = ws_bytes > p.head_bytes ? (ws_bytes - p.head_bytes) / (2 * p.rec_bytes) : 0;   // workgroups with records
     int nwg = (int)std::min<size_t>(num_cus(), room);
     if (nwg < 16 || p.segs / p.rt > 65535 || p.rt > 65535) {   // whole segments then
