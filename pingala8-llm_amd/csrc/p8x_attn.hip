@@ -69,6 +69,7 @@ __device__ __forceinline__ int wave_sum(int v) {
 struct Shares {
     int per, aligned, split, total;
     int tiles, segs;   // of the lane's sequence: tiles of a segment, segments
+    Seq q;             // and its numbers
     __device__ __forceinline__ int units(int tiles) const { return !split ? tiles > 0 : aligned ? (tiles + per - 1) / per * per : tiles; }
 };
 // f(tiles, segments) for the lane's sequence of s0 .. s0 + 63
@@ -85,8 +86,8 @@ __device__ __forceinline__ Shares share_out(const AttnJob &J, int rows_wg) {
     Shares h;
     h.tiles = h.segs = 0;
     if (lane < n_seq) {
-        const Seq q = seq_of(J, lane, rows_wg);
-        h.tiles = q.tiles, h.segs = J.c.n_kv * q.rts;
+        h.q = seq_of(J, lane, rows_wg);
+        h.tiles = h.q.tiles, h.segs = J.c.n_kv * h.q.rts;
     }
     auto over = [&](auto f) {   // f(tiles) summed over all segments
         int t = 0;
@@ -428,27 +429,29 @@ __device__ __forceinline__ void store_row(const AttnJob &J, int first, int h, in
     if (e == 0 && J.lse) J.lse[(size_t)(first + i) * J.c.n_kv * G + head] = p.l == 0.0f ? -INFINITY : (p.m - bias + __log2f(p.l)) * kLn2;
 }
 
-// The records of split segments in a launch of their own: 32 threads a 128-element piece of rows, eight ranges of records
-// side by side.
-template <int D, bool BF, bool QF>
+// The records of split segments in a launch of their own: a thread four elements of a row, over all records of its segment
+// (SUB 1), or, where they are many and the rows few, over one of eight ranges of them.
+template <int D, bool BF, bool QF, int SUB>
 __global__ __launch_bounds__(256) void k_attn_join(AttnJob J, int rows_wg) {
-    __shared__ Part sh[8][32];
+    constexpr int PIECES = 256 / SUB;
+    __shared__ Part sh[SUB > 1 ? SUB : 1][SUB > 1 ? PIECES : 1];
     const int s = blockIdx.z / J.c.n_kv, h = blockIdx.z % J.c.n_kv, rt = blockIdx.y;
-    const int sub = threadIdx.x >> 5, x4 = blockIdx.x * 32 + (threadIdx.x & 31), r = x4 / (D / 4), e = x4 % (D / 4) * 4;
+    const int sub = threadIdx.x / PIECES, x4 = blockIdx.x * PIECES + threadIdx.x % PIECES, r = x4 / (D / 4), e = x4 % (D / 4) * 4;
     const int2 at = J.where[(size_t)blockIdx.z * J.rt + rt];
     const Seq q = seq_of(J, s, rows_wg);
-    if (rt >= q.rts || q.tiles == 0) return;
     const int p0 = at.x, np = at.y;
-    if (np < 2) return;
+    if (rt >= q.rts || q.tiles == 0 || np < 2) return;
     const bool on = r < min(rows_wg, q.nt * J.d.G - rt * rows_wg);
-    const int each = (np + 7) / 8;
+    const int each = (np + SUB - 1) / SUB;
     Part p{float4v{0, 0, 0, 0}, -INFINITY, 0.0f};
     if (on) p = join_records<D, false>(J.part, (size_t)rows_wg * (D + 2), rows_wg, p0, min(np, sub * each), min(np, (sub + 1) * each), r, e);
-    sh[sub][threadIdx.x & 31] = p;
-    __syncthreads();
-    if (sub || !on) return;
-    for (int k = 1; k < 8; ++k) add_part(p, sh[k][threadIdx.x & 31]);
-    store_row<D, BF, QF>(J, q.first, h, rt * rows_wg + r, e, p);
+    if constexpr (SUB > 1) {
+        sh[sub][threadIdx.x % PIECES] = p;
+        __syncthreads();
+        if (sub) return;
+        for (int k = 1; k < SUB; ++k) add_part(p, sh[k][threadIdx.x % PIECES]);
+    }
+    if (on) store_row<D, BF, QF>(J, q.first, h, rt * rows_wg + r, e, p);
 }
 
 // 16 bytes a lane from base + off to LDS at `to` + 16 lane, without a wait. Written by hand: the compiler, which knows no other
@@ -504,9 +507,11 @@ __global__ __launch_bounds__(64 * attn_waves(D, SHARE)) void k_attn(AttnJob J) {
     W w;
     const uint32_t ss = (uint32_t)c.slot_stride, ko = (uint32_t)ln * ss + 8 * g, vo = 4 * g * ss + DV * ln;
     for (int u = u0; u < u1;) {
-        Seq q = seq_of(J, s, rows_wg);
-        q.nt = __builtin_amdgcn_readfirstlane(q.nt), q.n = __builtin_amdgcn_readfirstlane(q.n), q.first = __builtin_amdgcn_readfirstlane(q.first);
-        q.rts = __builtin_amdgcn_readfirstlane(q.rts), q.tiles = __builtin_amdgcn_readfirstlane(q.tiles);
+        Seq q = share.q;
+        if (s >= 64) q = seq_of(J, s, rows_wg);
+        const int from = s < 64 ? s : 0;
+        q.nt = __builtin_amdgcn_readlane(q.nt, from), q.n = __builtin_amdgcn_readlane(q.n, from), q.first = __builtin_amdgcn_readlane(q.first, from);
+        q.rts = __builtin_amdgcn_readlane(q.rts, from), q.tiles = __builtin_amdgcn_readlane(q.tiles, from);
         const int ps = share.units(q.tiles), units = c.n_kv * q.rts * ps;
         if (u >= base + units) {   // past this sequence (or none of its units)
             base += units;
@@ -594,20 +599,22 @@ __global__ __launch_bounds__(64 * attn_waves(D, SHARE)) void k_attn(AttnJob J) {
                 }
             };
             w.load_q(d, q.first, h, row0, rows, lane);
-            for (int st = 0; st < min(stages, kStages - 1); ++st) load(st);
             // Waits until stage st has arrived; the stage before it is no longer read then, and its place takes stage st +
             // kStages - 1. Loads come back in order, 2 PASS of each stage: the younger ones may be on their way (a stage that went
             // through registers has waited for all before it; other loads make the wait longer, never shorter).
+            int loaded = 0;
             auto arrive = [&](int st) {
                 const int young = min(kStages - 2, stages - 1 - st);
                 if (young == 2) __asm__ volatile("s_waitcnt vmcnt(%0)" ::"n"(4 * PASS) : "memory");
                 else if (young == 1) __asm__ volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * PASS) : "memory");
                 else __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
                 __syncthreads();
-                if (st + kStages - 1 < stages) load(st + kStages - 1);
+#pragma unroll 1
+                for (; loaded < min(stages, st + kStages); ++loaded) load(loaded);
             };
             auto place = [&](int t) { return lds + ((t - t0) / ST % kStages) * 2 * STAGE + 32 * ((t - t0) % ST) * W::ROW; };
-            arrive(0);
+#pragma unroll 1
+            for (int st = -1; st < 1; ++st) arrive(st);   // (-1: the first loads)
             w.lds_k(place(t0));
             uint32_t odd[2] = {0, 0};
             // One body for all tiles, so that the sums stay in their registers. V of a tile and K of the next come from LDS while the
@@ -889,7 +896,9 @@ static int attn_run(const AttnJob &J, int rows_wg, hipStream_t st) {
     static const hipError_t e = hipFuncSetAttribute((const void *)k_attn<D, BF, QF, NT, SHARE>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e != hipSuccess) return hip_check(e, "p8x_attn_tree LDS");
     k_attn<D, BF, QF, NT, SHARE><<<J.nwg, 64 * waves, lds, st>>>(J);
-    if (J.join) k_attn_join<D, BF, QF><<<dim3((rows_wg * (D / 4) + 31) / 32, J.rt, J.c.n_seq * J.c.n_kv), 256, 0, st>>>(J, rows_wg);
+    const dim3 heads(0, J.rt, J.c.n_seq * J.c.n_kv);
+    if (J.join && J.nwg > 12 * (int)(heads.y * heads.z)) k_attn_join<D, BF, QF, 8><<<dim3((rows_wg * (D / 4) + 31) / 32, heads.y, heads.z), 256, 0, st>>>(J, rows_wg);
+    else if (J.join) k_attn_join<D, BF, QF, 1><<<dim3((rows_wg * (D / 4) + 255) / 256, heads.y, heads.z), 256, 0, st>>>(J, rows_wg);
     return hip_check(hipGetLastError(), "p8x_attn_tree launch");
 }
 
