@@ -97,154 +97,259 @@ struct EvictDev {
 };
 
 // A slot's key: kept slots are those of the largest keys. Protected ones are above every score, NaN below.
-__device__ __forceinline__ uint32_t evict_key(const EvictDev &a, size_t base, int j, int64_t recent) {
-    if (a.pos) {
-        const int p = a.pos[base + j];
-        if (p < a.n_sink || p >= recent) return 0xFFFFFFFFu;
-    }
-    const float f = a.score[base + j];
+__device__ __forceinline__ uint32_t score_key(float f) {
     if (f != f) return 0;
     const uint32_t b = __builtin_bit_cast(uint32_t, f + 0.0f);   // -0 becomes +0
     return b >> 31 ? ~b : b | 0x80000000u;
 }
 
-// sum of v over the workgroup's threads before this one, and over all (1024 threads)
-__device__ __forceinline__ int block_scan(int v, int *red, int &total) {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    int x = v;
-    for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(x, o);
-        if (lane >= o) x += y;
-    }
+// sums of v over the waves before this one, and over all; v is the wave's
+template <int WAVES>
+__device__ __forceinline__ int wave_scan(int v, int *red, int &total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     __syncthreads();
-    if (lane == 63) red[w] = x;
+    if (lane == 0) red[wave] = v;
     __syncthreads();
-    int before = 0;
-    total = 0;
-    for (int i = 0; i < 16; ++i) {
-        if (i < w) before += red[i];
-        total += red[i];
-    }
-    return before + x - v;
+    int r = lane < WAVES ? red[lane] : 0, before = lane < wave ? r : 0;
+    for (int o = WAVES / 2; o; o >>= 1) before += __shfl_xor(before, o), r += __shfl_xor(r, o);
+    total = __builtin_amdgcn_readfirstlane(r);
+    return __builtin_amdgcn_readfirstlane(before);
 }
 
-// One workgroup a key/value head: the budget-th largest key by four passes of 8 bits, then every slot's fate in slot
-// order, a contiguous range of slots a thread.
-__global__ __launch_bounds__(1024) void k_evict_select(KvDev c, EvictDev a) {
-    __shared__ int hist[256], red[16], pick[2];
-    const int h = blockIdx.x, s = blockIdx.y, t = threadIdx.x;
+// One workgroup of WAVES waves a key/value head. Each wave has a contiguous range of the slots, in groups of 64, a slot a lane:
+// the budget-th largest key by three passes of 11, 11 and 10 bits over counts in LDS (protected slots are counted apart), then
+// every slot's fate in slot order, by ballots, which wait in LDS for the numbers of holes and movers before them. REGS: up to
+// 64 WAVES GMAX slots, whose keys stay in registers; else each pass reads scores and positions again, GMAX groups at a time, and
+// the ballots are taken again. Bound by one compute unit's issue rate (some 100 instructions a group of 64) and, for few slots, by
+// the latency of the passes.
+template <int WAVES, int GMAX, bool REGS>
+__global__ __launch_bounds__(64 * WAVES) void k_evict_select(KvDev c, EvictDev a) {
+    constexpr int BINS = 2048 / (64 * WAVES);   // of a thread
+    __shared__ int hist[2048], red[WAVES], pick[2];
+    __shared__ uint64_t fate[REGS ? WAVES * GMAX : 1][2];
+    const int h = blockIdx.x, s = blockIdx.y, t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const size_t hd = (size_t)s * c.n_kv + h, base = hd * c.max_len;
-    const int n = seq_len(c, s), keep = min(n, a.budget);
+    const int n = __builtin_amdgcn_readfirstlane(seq_len(c, s)), keep = min(n, a.budget);
     int *ws = a.ws + hd * evict_words(c.max_len, a.budget);
-    if (a.score_out != a.score)
-        for (int j = t; j < keep; j += 1024) a.score_out[base + j] = a.score[base + j];
-    if (a.pos && a.pos_out != a.pos)
-        for (int j = t; j < keep; j += 1024) a.pos_out[base + j] = a.pos[base + j];
     if (t == 0) ws[1] = n;
+    if (n == 0) {
+        if (t == 0) ws[0] = 0;
+        return;
+    }
+    const int groups = (n + 64 * WAVES - 1) / (64 * WAVES);   // of a wave
+    const uint32_t first = wave * groups * 64 + lane, end = n - 1;   // the lane's first slot; the last slot
+    const float *score = a.score + base;
+    const int *pos = a.pos ? a.pos + base : nullptr;
+    const bool copy_s = a.score_out != a.score, copy_p = pos && a.pos_out != a.pos;
+    uint32_t keys[GMAX];
+    // positions of groups g0 .. into keys, every load before the first use
+    auto load_pos = [&](int g0) {
+#pragma unroll
+        for (int g = 0; g < GMAX; ++g)
+            if (g0 + g < groups) keys[g] = (uint32_t)pos[min(first + 64 * (g0 + g), end)];
+    };
+    int m = INT32_MIN;   // the largest position; positions of slots that stay in place to pos_out
+    if (pos)
+        for (int g0 = 0; g0 < groups; g0 += GMAX) {
+            load_pos(g0);
+#pragma unroll
+            for (int g = 0; g < GMAX; ++g)
+                if (g0 + g < groups) {
+                    m = max(m, (int)keys[g]);
+                    const uint32_t j = first + 64 * (g0 + g);
+                    if (copy_p && j < (uint32_t)keep) a.pos_out[base + j] = (int)keys[g];
+                }
+        }
+    int64_t recent = INT64_MAX;   // positions from here on are protected
+    if (pos && a.n_recent && n > a.budget) {
+        for (int o = 32; o; o >>= 1) m = max(m, __shfl_xor(m, o));
+        if (lane == 0) red[wave] = m;
+        __syncthreads();
+        m = red[lane & (WAVES - 1)];
+        for (int o = WAVES / 2; o; o >>= 1) m = max(m, __shfl_xor(m, o));
+        recent = (int64_t)m + 1 - a.n_recent;
+    }
+    // keys of groups g0 .. over the positions in them; FIRST: the scores of slots that stay in place to score_out
+    int guarded = 0;
+    auto make = [&](int g0, bool first_time) {
+#pragma unroll
+        for (int b = 0; b < GMAX; b += 8) {
+            float sc[8];
+#pragma unroll
+            for (int g = b; g < b + 8 && g < GMAX; ++g)
+                if (g0 + g < groups) sc[g - b] = score[min(first + 64 * (g0 + g), end)];
+#pragma unroll
+            for (int g = b; g < b + 8 && g < GMAX; ++g)
+                if (g0 + g < groups) {
+                    const uint32_t j = first + 64 * (g0 + g);
+                    const bool safe = pos && ((int)keys[g] < a.n_sink || (int)keys[g] >= recent);
+                    if (first_time && copy_s && j < (uint32_t)keep) a.score_out[base + j] = sc[g - b];
+                    keys[g] = safe ? 0xFFFFFFFFu : score_key(sc[g - b]);
+                    if (first_time) guarded += __popcll(__ballot(safe && j <= end));
+                }
+        }
+    };
+    for (int g0 = 0; g0 < groups; g0 += GMAX) {
+        if (!REGS && pos) load_pos(g0);
+        make(g0, true);
+    }
     if (n <= a.budget) {
         if (t == 0) ws[0] = 0;
         return;
     }
-    int64_t recent = INT64_MAX;   // positions from here on are protected
-    if (a.pos && a.n_recent) {
-        int m = INT32_MIN;
-        for (int j = t; j < n; j += 1024) m = max(m, a.pos[base + j]);
-        for (int o = 32; o; o >>= 1) m = max(m, __shfl_xor(m, o));
-        if ((t & 63) == 0) red[t >> 6] = m;
-        __syncthreads();
-        m = red[0];
-        for (int i = 1; i < 16; ++i) m = max(m, red[i]);
-        recent = (int64_t)m + 1 - a.n_recent;
-    }
-    uint32_t key = 0, known = 0;
-    int want = keep;   // of the keys that agree with `key` in the known bits, how many of the largest stay
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        __syncthreads();
-        if (t < 256) hist[t] = 0;
-        __syncthreads();
-        for (int j = t; j < n; j += 1024) {
-            const uint32_t k = evict_key(a, base, j, recent);
-            if ((k & known) == key) atomicAdd(&hist[k >> shift & 255], 1);
+    // f(group, slot, key, whether there is one) over the wave's groups in order
+    auto each = [&](auto f) {
+        for (int g0 = 0; g0 < groups; g0 += GMAX) {
+            if constexpr (!REGS) {
+                if (pos) load_pos(g0);
+                make(g0, false);
+            }
+#pragma unroll
+            for (int g = 0; g < GMAX; ++g)
+                if (g0 + g < groups) {
+                    const uint32_t j = first + 64 * (g0 + g);
+                    f(g0 + g, j, keys[g], j <= end);
+                }
         }
-        __syncthreads();
-        if (t < 64) {   // from the largest digit down: the digit in which the count passes `want`
-            int v[4], sum = 0;
-            for (int i = 0; i < 4; ++i) sum += v[i] = hist[255 - 4 * t - i];
+    };
+    int all;
+    wave_scan<WAVES>(guarded, red, all);
+    uint32_t key = 0xFFFFFFFFu;
+    int want = keep;   // how many slots of exactly `key` stay, the lowest ones; all with a larger key stay
+    if (all < keep) {
+        want = keep - all;
+        key = 0;
+        uint32_t known = 0;
+#pragma unroll 1
+        for (int p = 0; p < 3; ++p) {
+            const int shift = p == 0 ? 21 : p == 1 ? 10 : 0, mask = p == 2 ? 1023 : 2047;
+            __syncthreads();
+#pragma unroll
+            for (int b = 0; b < BINS; ++b) hist[64 * WAVES * b + t] = 0;
+            __syncthreads();
+            each([&](int, uint32_t, uint32_t k, bool in) {
+                if (in && k != 0xFFFFFFFFu && (k & known) == key) atomicAdd(&hist[k >> shift & mask], 1);
+            });
+            __syncthreads();
+            // from the largest digit down, BINS of them a thread: the digit in which the count passes `want`
+            const int d0 = 2047 - BINS * t;
+            int v[BINS], sum = 0;
+#pragma unroll
+            for (int b = 0; b < BINS; ++b) sum += v[b] = hist[d0 - b];
             int x = sum;
             for (int o = 1; o < 64; o <<= 1) {
                 const int y = __shfl_up(x, o);
-                if (t >= o) x += y;
+                if (lane >= o) x += y;
             }
-            int above = x - sum;
-            if (above < want && x >= want)
-                for (int i = 0; i < 4; ++i) {
-                    if (above + v[i] >= want) {
-                        pick[0] = 255 - 4 * t - i;
-                        pick[1] = want - above;
-                        break;
-                    }
-                    above += v[i];
-                }
+            int total;
+            int above = wave_scan<WAVES>(__builtin_amdgcn_readlane(x, 63), red, total) + x - sum;
+            if (above < want && above + sum >= want) {
+                int d = d0;
+#pragma unroll
+                for (int b = 0; b + 1 < BINS; ++b)
+                    if (d == d0 - b && above + v[b] < want) above += v[b], --d;
+                pick[0] = d;
+                pick[1] = want - above;
+            }
+            __syncthreads();
+            key |= (uint32_t)pick[0] << shift;
+            known |= (uint32_t)mask << shift;
+            want = pick[1];
         }
-        __syncthreads();
-        key |= (uint32_t)pick[0] << shift;
-        known |= 255u << shift;
-        want = pick[1];
     }
-    // want: how many slots of exactly `key` stay, the lowest ones
-    const int per = (n + 1023) / 1024, j0 = min(n, t * per), j1 = min(n, j0 + per);
+    // every slot's fate, in slot order: f(group, slot, holes' ballot, movers' ballot)
+    const uint64_t lower = (1ull << lane) - 1;
     int ties = 0, total;
-    for (int j = j0; j < j1; ++j) ties += evict_key(a, base, j, recent) == key;
-    const int tie0 = block_scan(ties, red, total);
-    int holes = 0, movers = 0, tie = tie0;
-    for (int j = j0; j < j1; ++j) {
-        const uint32_t k = evict_key(a, base, j, recent);
-        const bool stay = k > key || (k == key && tie++ < want);
-        holes += !stay && j < a.budget;
-        movers += stay && j >= a.budget;
-    }
-    int hole = block_scan(holes, red, total), mover = block_scan(movers, red, total);
+    each([&](int, uint32_t, uint32_t k, bool in) { ties += __popcll(__ballot(in && k == key)); });
+    const int tie0 = wave_scan<WAVES>(ties, red, total);
+    auto fates = [&](auto f) {
+        int tie = tie0;
+        each([&](int g, uint32_t j, uint32_t k, bool in) {
+            const uint64_t eq = __ballot(in && k == key);
+            const bool stay = in && (k > key || (k == key && tie + __popcll(eq & lower) < want));
+            tie += __popcll(eq);
+            f(g, j, __ballot(in && !stay && j < (uint32_t)a.budget), __ballot(stay && j >= (uint32_t)a.budget));
+        });
+    };
+    int holes = 0, movers = 0;
+    fates([&](int g, uint32_t, uint64_t ho, uint64_t mo) {
+        holes += __popcll(ho), movers += __popcll(mo);
+        if (REGS && lane == 0) fate[wave * GMAX + g][0] = ho, fate[wave * GMAX + g][1] = mo;
+    });
+    holes = wave_scan<WAVES>(holes, red, total);
+    movers = wave_scan<WAVES>(movers, red, total);
     if (t == 0) ws[0] = total;
     int *src = ws + 4, *dst = src + evict_most(c.max_len, a.budget);
-    tie = tie0;
-    for (int j = j0; j < j1; ++j) {
-        const uint32_t k = evict_key(a, base, j, recent);
-        const bool stay = k > key || (k == key && tie++ < want);
-        if (!stay && j < a.budget) dst[hole++] = j;
-        if (stay && j >= a.budget) src[mover++] = j;
-    }
+    auto put = [&](uint32_t j, uint64_t ho, uint64_t mo) {
+        if (ho >> lane & 1) dst[holes + __popcll(ho & lower)] = j;
+        if (mo >> lane & 1) src[movers + __popcll(mo & lower)] = j;
+        holes += __popcll(ho), movers += __popcll(mo);
+    };
+    if constexpr (REGS)
+        for (int g = 0; g < groups; ++g) put(first + 64 * g, fate[wave * GMAX + g][0], fate[wave * GMAX + g][1]);
+    else
+        fates([&](int, uint32_t j, uint64_t ho, uint64_t mo) { put(j, ho, mo); });
 }
 
-// The moves: sources are slots >= budget and destinations slots < budget, so no row is both.
-__global__ __launch_bounds__(256) void k_evict_move(KvDev c, EvictDev a, int D) {
+// The moves: sources are slots >= budget and destinations slots < budget, so no row is both. D / 8 lanes a row, four rows at a
+// time: their places, then eight loads, then the stores. Bound by HBM on rows of 2 D bytes.
+template <int D>
+__global__ __launch_bounds__(256) void k_evict_move(KvDev c, EvictDev a) {
+    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+    constexpr int PC = D / 8, ROWS = 256 / PC;
     const int h = blockIdx.y, s = blockIdx.z;
     const size_t hd = (size_t)s * c.n_kv + h, base = hd * c.max_len;
     const int *ws = a.ws + hd * evict_words(c.max_len, a.budget);
     const int moves = ws[0], *src = ws + 4, *dst = src + evict_most(c.max_len, a.budget);
     if (h == 0 && blockIdx.x == 0 && threadIdx.x == 0) a.len_out[s] = min(ws[1], a.budget);
-    const int row = D / 8;
-    for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < (int64_t)moves * row; x += (int64_t)gridDim.x * 256) {
-        const int i = (int)(x / row), e = (int)(x % row) * 8, j0 = src[i], j1 = dst[i];
-        const int64_t from = slot_offset(c, s, j0), to = slot_offset(c, s, j1);
-        if (from >= 0 && to >= 0) {
-            const size_t o = (size_t)h * c.head_stride + e;
-            const uint4 k = *(const uint4 *)(c.k + from + o), v = *(const uint4 *)(c.v + from + o);
-            *(uint4 *)(c.k + to + o) = k;
-            *(uint4 *)(c.v + to + o) = v;
+    const int r0 = threadIdx.x / PC, e = threadIdx.x % PC;
+    const size_t o = (size_t)h * c.head_stride + 8 * e;
+    for (int i0 = 4 * ROWS * blockIdx.x + r0; i0 < moves; i0 += 4 * ROWS * gridDim.x) {
+        int j0[4], j1[4];
+        int64_t from[4], to[4];
+        u4 k[4], v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int i = min(i0 + u * ROWS, moves - 1);   // (the last one once more is harmless)
+            j0[u] = src[i], j1[u] = dst[i];
         }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) from[u] = slot_offset(c, s, j0[u]), to[u] = slot_offset(c, s, j1[u]);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int64_t f = max(from[u], (int64_t)0);
+            k[u] = *(const u4 *)(c.k + f + o);
+            v[u] = *(const u4 *)(c.v + f + o);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (from[u] >= 0 && to[u] >= 0) {
+                *(u4 *)(c.k + to[u] + o) = k[u];
+                *(u4 *)(c.v + to[u] + o) = v[u];
+            }
         if (e == 0) {
-            a.score_out[base + j1] = a.score[base + j0];
-            if (a.pos) a.pos_out[base + j1] = a.pos[base + j0];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                a.score_out[base + j1[u]] = a.score[base + j0[u]];
+                if (a.pos) a.pos_out[base + j1[u]] = a.pos[base + j0[u]];
+            }
         }
     }
 }
 
 int launch_kv_evict(const KvDev &c, int D, const p8x_evict_args &p, hipStream_t st) {
     const EvictDev a{p.budget, p.n_sink, p.n_recent, p.score, p.score_out, p.pos, p.pos_out, p.len_out, (int *)p.workspace};
-    k_evict_select<<<dim3(c.n_kv, c.n_seq), 1024, 0, st>>>(c, a);
-    const int64_t pieces = (int64_t)evict_most(c.max_len, a.budget) * (D / 8);
-    const int nb = (int)std::max<int64_t>(1, std::min<int64_t>((pieces + 255) / 256, 512));
-    k_evict_move<<<dim3(nb, c.n_kv, c.n_seq), 256, 0, st>>>(c, a, D);
+    const dim3 heads(c.n_kv, c.n_seq);
+    if (c.max_len <= 4 * 4 * 64) k_evict_select<4, 4, true><<<heads, 64 * 4, 0, st>>>(c, a);
+    else if (c.max_len <= 16 * 4 * 64) k_evict_select<16, 4, true><<<heads, 64 * 16, 0, st>>>(c, a);
+    else if (c.max_len <= 16 * 32 * 64) k_evict_select<16, 32, true><<<heads, 64 * 16, 0, st>>>(c, a);
+    else k_evict_select<16, 16, false><<<heads, 64 * 16, 0, st>>>(c, a);
+    const int64_t rows = 4 * (256 / (D / 8));   // of a workgroup at a time
+    const int nb = (int)std::max<int64_t>(1, std::min<int64_t>(((int64_t)evict_most(c.max_len, a.budget) + rows - 1) / rows, 1024));
+    const dim3 grid(nb, c.n_kv, c.n_seq);
+    if (D == 64) k_evict_move<64><<<grid, 256, 0, st>>>(c, a);
+    else if (D == 128) k_evict_move<128><<<grid, 256, 0, st>>>(c, a);
+    else k_evict_move<256><<<grid, 256, 0, st>>>(c, a);
     return hip_check(hipGetLastError(), "p8x_kv_evict launch");
 }
 
