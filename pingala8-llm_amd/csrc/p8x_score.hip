@@ -54,6 +54,38 @@ __global__ __launch_bounds__(64 * kScoreWaves) void k_score(ScoreJob J) {
     int rb = 0;
     do {   // once without rows: scores decay
         const int rt = min(RB / 16, (rows - rb + 15) / 16);
+        // the wave's tiles from tb on: offsets of its next 64 halves, a lane each, and keys one tile ahead, the first before
+        // the rows are laid out
+        int tb = t0 + wave, lo = 0, hi = 0, many = 0;
+        uint4v kf[2][C], kn[2][C];
+        float next = 0.0f;
+        auto half = [&](int i) { return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, i) << 32 | (uint32_t)__builtin_amdgcn_readlane(lo, i)); };
+        // tile i's keys into kn; a lane past the last slot reads the half's first, whose column is then not written
+        auto fetch = [&](int i) {
+            const int slot = 32 * (tb + kScoreWaves * i);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int64_t o = half(2 * i + x);
+                if (o >= 0) {
+                    const uint16_t *at = kp + o + (slot + 16 * x + ln < n ? ko : 8 * g);
+#pragma unroll
+                    for (int k = 0; k < C; ++k) kn[x][k] = *(const uint4v *)(at + 32 * k);
+                }
+            }
+            if (lane < 32 && slot + lane < n && !rb) next = J.score[base + slot + lane];
+        };
+        auto ahead = [&](int tb) {
+            if (tb >= min(t1, ctx)) return;
+            const int t = tb + kScoreWaves * (lane >> 1), slot = 32 * t + 16 * (lane & 1);
+            const int64_t off = t < min(t1, ctx) && slot < n ? slot_offset(c, s, slot) : -1;
+            lo = (int)off, hi = (int)(off >> 32), many = min(32, (min(t1, ctx) - tb + kScoreWaves - 1) / kScoreWaves);
+            fetch(0);
+        };
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int k = 0; k < C; ++k) kn[x][k] = uint4v{0, 0, 0, 0};
+        ahead(tb);
         if (rb) __syncthreads();
         for (int r = threadIdx.x; r < 16 * rt; r += 64 * kScoreWaves) {
             const int row = rb + r, i = row / d.G;
@@ -88,7 +120,6 @@ __global__ __launch_bounds__(64 * kScoreWaves) void k_score(ScoreJob J) {
         }
         __syncthreads();
 
-        uint4v kf[2][C];
         // the tile's weights, summed over the rows: lane l < 32 has slot l's. hide: bit i of byte t set where row 4 g + i of
         // the row tile does not see the lane's slot of half t
         auto sum_rows = [&](bool draft, int tj0, int tj1) {
@@ -130,27 +161,17 @@ __global__ __launch_bounds__(64 * kScoreWaves) void k_score(ScoreJob J) {
             }
         };
 
-        for (int tb = t0 + wave; tb < min(t1, ctx); tb += 32 * kScoreWaves) {
-            // offsets of the wave's next 64 halves, a lane each
-            int64_t off = -1;
-            {
-                const int t = tb + kScoreWaves * (lane >> 1), slot = 32 * t + 16 * (lane & 1);
-                if (t < min(t1, ctx) && slot < n) off = slot_offset(c, s, slot);
-            }
-            const int lo = (int)off, hi = (int)(off >> 32), many = min(32, (min(t1, ctx) - tb + kScoreWaves - 1) / kScoreWaves);
-            auto half = [&](int i) { return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, i) << 32 | (uint32_t)__builtin_amdgcn_readlane(lo, i)); };
+        for (; tb < min(t1, ctx); ahead(tb += 32 * kScoreWaves)) {
             for (int i = 0; i < many; ++i) {
                 const int slot = 32 * (tb + kScoreWaves * i);
-                const int64_t h0 = half(2 * i), h1 = half(2 * i + 1);
-                const bool on0 = h0 >= 0 && slot + ln < n, on1 = h1 >= 0 && slot + 16 + ln < n;
-                const float before = lane < 32 && slot + lane < n && !rb ? J.score[base + slot + lane] : 0.0f;
+                const float before = next;
 #pragma unroll
-                for (int k = 0; k < C; ++k) {
-                    kf[0][k] = on0 ? *(const uint4v *)(kp + h0 + ko + 32 * k) : uint4v{0, 0, 0, 0};
-                    kf[1][k] = on1 ? *(const uint4v *)(kp + h1 + ko + 32 * k) : uint4v{0, 0, 0, 0};
-                }
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int k = 0; k < C; ++k) kf[x][k] = kn[x][k];
+                if (i + 1 < many) fetch(i + 1);
                 float w = rt > 0 ? sum_rows(false, 0, 0) : 0.0f;
-                if ((lane < 16 ? h0 : h1) < 0) w = 0.0f;
+                if ((lane < 16 ? half(2 * i) : half(2 * i + 1)) < 0) w = 0.0f;
                 put(slot, n, true, w, before);
             }
         }
