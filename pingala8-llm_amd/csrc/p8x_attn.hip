@@ -171,6 +171,7 @@ struct Wave {
                     q[a][0][k] = w;
                 }
             }
+            c2[a] = fmaxf(c2[a], 0x1p-149f);   // of a scale of 0, or one that underflows: hidden scores, -inf, stay so
         }
     }
 

@@ -109,3 +109,12 @@ def test_null_structs():
 def test_nothing_to_do_is_no_error():
     p8x.NormResidual(0, 32, h=A, x=A).run()
     attn(cache(), drafts(n_tokens=0, max_tokens=0)).run()
+
+
+def test_slot_strides_beyond_offsets_within_a_page():
+    """attention and scores keep a slot's offset in its half page in 32 bits"""
+    big = dict(slot_stride=1 << 26, head_stride=128, page_stride=1 << 31)
+    for make in (attn, score):
+        with pytest.raises(p8x.P8xError) as e:
+            make(cache(**big), drafts()).run()
+        assert e.value.code == p8x.P8X_ERR_UNSUPPORTED if hasattr(e.value, "code") else "2^26" in str(e.value)
