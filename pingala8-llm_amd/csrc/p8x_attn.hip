@@ -258,7 +258,7 @@ struct Wave {
                 float v = fmaxf(mx[a], __shfl_xor(mx[a], 16));
                 v = fmaxf(v, __shfl_xor(v, 32));
                 v = fmaxf(v, m[a]);
-                const float al = v == -INFINITY || m[a] == v ? 1.0f : exp2f(m[a] - v);
+                const float al = v == -INFINITY || m[a] == v ? 1.0f : __builtin_amdgcn_exp2f(m[a] - v);
                 m[a] = v;
                 l[a] *= al;
 #pragma unroll
@@ -384,7 +384,7 @@ __device__ __forceinline__ void store2_agent(float *p, float a, float b) {
 struct Part { float4v v; float m, l; };   // four elements of a row
 __device__ __forceinline__ void add_part(Part &a, const Part &b) {
     const float mn = fmaxf(a.m, b.m), mb = mn == -INFINITY ? 0.0f : mn;
-    const float f0 = exp2f(a.m - mb), f1 = exp2f(b.m - mb);
+    const float f0 = __builtin_amdgcn_exp2f(a.m - mb), f1 = __builtin_amdgcn_exp2f(b.m - mb);
     a.m = mn;
     a.l = a.l * f0 + b.l * f1;
     a.v = a.v * f0 + b.v * f1;
@@ -709,31 +709,52 @@ __global__ __launch_bounds__(64 * attn_waves(D, SHARE)) void k_attn(AttnJob J) {
                     h1 = left > 16 ? slot_offset(c, s, 32 * t + 16) : -1;
                     for (int a = 0; a < NT; ++a) see[a] = ((1u << left) - 1) & ((h0 >= 0 ? 0xFFFFu : 0) | (h1 >= 0 ? 0xFFFF0000u : 0));
                 }
+                // slots that are not there: the tile's first, hidden, and zeros among the values
+                auto put_v = [&](int j, bool on, const uint32_t *v) {
 #pragma unroll
-                for (int b = 0; b < 2; ++b)
+                    for (int e = 0; e < W::VW; ++e) w.vf[j][e] = on ? v[e] : 0;
+                };
+                if (draft) {
 #pragma unroll
-                    for (int k = 0; k < W::C; ++k) {
-                        uint4v v = {0, 0, 0, 0};
-                        if (16 * b + ln < left) {
-                            if (draft) v = draft8(d.k, (size_t)(q.first + j0 + 16 * b + ln) * d.ld_kv + (size_t)h * d.hs_kv + 32 * k + 8 * g, d.kv_f32, BF);
-                            else if ((b ? h1 : h0) >= 0) v = *(const uint4v *)(kp + (b ? h1 : h0) + ko + 32 * k);
-                        }
-                        w.kf[b][k] = v;
+                    for (int b = 0; b < 2; ++b) {
+                        const int jj = 16 * b + ln < left ? 16 * b + ln : 0;
+                        const size_t at = (size_t)(q.first + j0 + jj) * d.ld_kv + (size_t)h * d.hs_kv + 8 * g;
+#pragma unroll
+                        for (int k = 0; k < W::C; ++k) w.kf[b][k] = draft8(d.k, at + 32 * k, d.kv_f32, BF);
                     }
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int jj = (j < 4 ? 0 : 12) + 4 * g + j;
-                    const size_t at = (size_t)(q.first + j0 + jj) * d.ld_kv + (size_t)h * d.hs_kv + DV * ln;
-                    const int64_t hb = j < 4 ? h0 : h1;
+                    for (int j = 0; j < 8; ++j) {
+                        const int jj = (j < 4 ? 0 : 12) + 4 * g + j;
+                        const size_t at = (size_t)(q.first + j0 + (jj < left ? jj : 0)) * d.ld_kv + (size_t)h * d.hs_kv + DV * ln;
+                        uint32_t v[W::VW];
+                        if constexpr (W::VW == 2) {
+                            if (d.kv_f32) {
+                                const float4v f = *(const float4v *)((const float *)d.v + at);
+                                v[0] = pack2<BF>(f[0], f[1]), v[1] = pack2<BF>(f[2], f[3]);
+                            } else {
+                                *(uint2v *)v = *(const uint2v *)((const uint16_t *)d.v + at);
+                            }
+                        } else {
 #pragma unroll
-                    for (int e = 0; e < W::VW; ++e) {
-                        uint32_t v = 0;
-                        if (jj < left && hb >= 0) {
-                            if (!draft) v = *(const uint32_t *)(vp + hb + vo + (j & 3) * ss + 2 * e);
-                            else if (d.kv_f32) v = pack2<BF>(((const float *)d.v)[at + 2 * e], ((const float *)d.v)[at + 2 * e + 1]);
-                            else v = *(const uint32_t *)((const uint16_t *)d.v + at + 2 * e);
+                            for (int e = 0; e < W::VW; e += 4) *(uint4v *)(v + e) = draft8(d.v, at + 2 * e, d.kv_f32, BF);
                         }
-                        w.vf[j][e] = v;
+                        put_v(j, jj < left, v);
+                    }
+                } else {
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) {
+                        const int64_t hb = b ? h1 : h0;
+                        const uint32_t o = 16 * b + ln < left ? ko : 8 * g;
+#pragma unroll
+                        for (int k = 0; k < W::C; ++k) w.kf[b][k] = *(const uint4v *)(kp + max(hb, (int64_t)0) + o + 32 * k);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const int jj = (j < 4 ? 0 : 12) + 4 * g + j;
+                        const int64_t hb = j < 4 ? h0 : h1;
+                        uint32_t v[W::VW];
+                        w.load_v1(vp + max(hb, (int64_t)0) + (jj < left ? vo + (j & 3) * ss : DV * ln), v);
+                        put_v(j, jj < left && hb >= 0, v);
                     }
                 }
                 uint32_t odd = 0;
@@ -819,7 +840,7 @@ __global__ __launch_bounds__(64 * attn_waves(D, SHARE)) void k_attn(AttnJob J) {
                 Part p{float4v{0, 0, 0, 0}, m, 0.0f};
                 for (int k = 0; k < SW; ++k) {
                     const int wv = k * RW + rg;
-                    const float f = exp2f(pm[wv * R16 + rr] - mb);
+                    const float f = __builtin_amdgcn_exp2f(pm[wv * R16 + rr] - mb);
                     p.l += f * pl[wv * R16 + rr];
                     p.v += f * *(const float4v *)(sh + ((size_t)wv * R16 + rr) * LD + e);
                 }
