@@ -96,6 +96,7 @@ struct EvictDev {
     int *ws;
 };
 
+constexpr uint32_t kSafeKey = 0xFFFFFFFFu;
 // A slot's key: kept slots are those of the largest keys. Protected ones are above every score, NaN below.
 __device__ __forceinline__ uint32_t score_key(float f) {
     if (f != f) return 0;
@@ -118,15 +119,14 @@ __device__ __forceinline__ int wave_scan(int v, int *red, int &total) {
 
 // One workgroup of WAVES waves a key/value head. Each wave has a contiguous range of the slots, in groups of 64, a slot a lane:
 // the budget-th largest key by three passes of 11, 11 and 10 bits over counts in LDS (protected slots are counted apart), then
-// every slot's fate in slot order, by ballots, which wait in LDS for the numbers of holes and movers before them. REGS: up to
-// 64 WAVES GMAX slots, whose keys stay in registers; else each pass reads scores and positions again, GMAX groups at a time, and
-// the ballots are taken again. Bound by one compute unit's issue rate (some 100 instructions a group of 64) and, for few slots, by
-// the latency of the passes.
-template <int WAVES, int GMAX, bool REGS>
+// every slot's fate in slot order, by ballots. KEEP: up to 64 KEEP slots a wave, whose keys stay in LDS, each lane its own;
+// else (0) every pass makes them again from scores and positions. Loops are rolled, U groups a turn: a workgroup runs each
+// pass once, and with all groups unrolled it waited for instructions most of the time. Bound by the latency of the passes.
+template <int WAVES, int U, int KEEP>
 __global__ __launch_bounds__(64 * WAVES) void k_evict_select(KvDev c, EvictDev a) {
     constexpr int BINS = 2048 / (64 * WAVES);   // of a thread
     __shared__ int hist[2048], red[WAVES], pick[2];
-    __shared__ uint64_t fate[REGS ? WAVES * GMAX : 1][2];
+    extern __shared__ uint32_t kept[];   // KEEP: [wave][group][lane]
     const int h = blockIdx.x, s = blockIdx.y, t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const size_t hd = (size_t)s * c.n_kv + h, base = hd * c.max_len;
     const int n = __builtin_amdgcn_readfirstlane(seq_len(c, s)), keep = min(n, a.budget);
@@ -141,24 +141,25 @@ __global__ __launch_bounds__(64 * WAVES) void k_evict_select(KvDev c, EvictDev a
     const float *score = a.score + base;
     const int *pos = a.pos ? a.pos + base : nullptr;
     const bool copy_s = a.score_out != a.score, copy_p = pos && a.pos_out != a.pos;
-    uint32_t keys[GMAX];
-    // positions of groups g0 .. into keys, every load before the first use
-    auto load_pos = [&](int g0) {
+    uint32_t *const mine = kept + wave * KEEP * 64 + lane;
+    // v[u] of group g0 + u, all loads before the first use; a lane past the last slot reads that one
+    auto fetch = [&](int g0, const uint32_t *from, uint32_t (&v)[U]) {
 #pragma unroll
-        for (int g = 0; g < GMAX; ++g)
-            if (g0 + g < groups) keys[g] = (uint32_t)pos[min(first + 64 * (g0 + g), end)];
+        for (int u = 0; u < U; ++u) v[u] = from[min(first + 64 * (g0 + u), end)];
     };
     int m = INT32_MIN;   // the largest position; positions of slots that stay in place to pos_out
     if (pos)
-        for (int g0 = 0; g0 < groups; g0 += GMAX) {
-            load_pos(g0);
+#pragma unroll 1
+        for (int g0 = 0; g0 < groups; g0 += U) {
+            uint32_t v[U];
+            fetch(g0, (const uint32_t *)pos, v);
 #pragma unroll
-            for (int g = 0; g < GMAX; ++g)
-                if (g0 + g < groups) {
-                    m = max(m, (int)keys[g]);
-                    const uint32_t j = first + 64 * (g0 + g);
-                    if (copy_p && j < (uint32_t)keep) a.pos_out[base + j] = (int)keys[g];
-                }
+            for (int u = 0; u < U; ++u) {
+                const uint32_t j = first + 64 * (g0 + u);
+                m = max(m, (int)v[u]);
+                if (KEEP && g0 + u < groups) mine[64 * (g0 + u)] = v[u];
+                if (copy_p && g0 + u < groups && j < (uint32_t)keep) a.pos_out[base + j] = (int)v[u];
+            }
         }
     int64_t recent = INT64_MAX;   // positions from here on are protected
     if (pos && a.n_recent && n > a.budget) {
@@ -169,52 +170,61 @@ __global__ __launch_bounds__(64 * WAVES) void k_evict_select(KvDev c, EvictDev a
         for (int o = WAVES / 2; o; o >>= 1) m = max(m, __shfl_xor(m, o));
         recent = (int64_t)m + 1 - a.n_recent;
     }
-    // keys of groups g0 .. over the positions in them; FIRST: the scores of slots that stay in place to score_out
-    int guarded = 0;
-    auto make = [&](int g0, bool first_time) {
+    // keys of groups g0 .. g0 + U - 1 from scores, and positions from LDS or memory
+    auto make = [&](int g0, uint32_t (&k)[U], uint32_t (&sc)[U], bool kept_pos) {
+        uint32_t p[U];
+        fetch(g0, (const uint32_t *)score, sc);
+        if (pos) {
+            if (kept_pos)
 #pragma unroll
-        for (int b = 0; b < GMAX; b += 8) {
-            float sc[8];
+                for (int u = 0; u < U; ++u) p[u] = mine[64 * min(g0 + u, groups - 1)];
+            else fetch(g0, (const uint32_t *)pos, p);
+        }
 #pragma unroll
-            for (int g = b; g < b + 8 && g < GMAX; ++g)
-                if (g0 + g < groups) sc[g - b] = score[min(first + 64 * (g0 + g), end)];
-#pragma unroll
-            for (int g = b; g < b + 8 && g < GMAX; ++g)
-                if (g0 + g < groups) {
-                    const uint32_t j = first + 64 * (g0 + g);
-                    const bool safe = pos && ((int)keys[g] < a.n_sink || (int)keys[g] >= recent);
-                    if (first_time && copy_s && j < (uint32_t)keep) a.score_out[base + j] = sc[g - b];
-                    keys[g] = safe ? 0xFFFFFFFFu : score_key(sc[g - b]);
-                    if (first_time) guarded += __popcll(__ballot(safe && j <= end));
-                }
+        for (int u = 0; u < U; ++u) {
+            const bool safe = pos && ((int)p[u] < a.n_sink || (int)p[u] >= recent);
+            k[u] = safe ? kSafeKey : score_key(__builtin_bit_cast(float, sc[u]));
         }
     };
-    for (int g0 = 0; g0 < groups; g0 += GMAX) {
-        if (!REGS && pos) load_pos(g0);
-        make(g0, true);
+    int guarded = 0;   // protected slots; the scores of slots that stay in place go to score_out
+#pragma unroll 1
+    for (int g0 = 0; g0 < groups; g0 += U) {
+        uint32_t k[U], sc[U];
+        make(g0, k, sc, KEEP > 0);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (g0 + u < groups) {
+                const uint32_t j = first + 64 * (g0 + u);
+                if (KEEP) mine[64 * (g0 + u)] = k[u];
+                if (copy_s && j < (uint32_t)keep) a.score_out[base + j] = __builtin_bit_cast(float, sc[u]);
+                guarded += __popcll(__ballot(k[u] == kSafeKey && j <= end));
+            }
     }
     if (n <= a.budget) {
         if (t == 0) ws[0] = 0;
         return;
     }
-    // f(group, slot, key, whether there is one) over the wave's groups in order
+    // f(slot, key, whether there is one) over the wave's groups in order
     auto each = [&](auto f) {
-        for (int g0 = 0; g0 < groups; g0 += GMAX) {
-            if constexpr (!REGS) {
-                if (pos) load_pos(g0);
-                make(g0, false);
+#pragma unroll 1
+        for (int g0 = 0; g0 < groups; g0 += U) {
+            uint32_t k[U], sc[U];
+            if constexpr (KEEP) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) k[u] = mine[64 * min(g0 + u, groups - 1)];
+            } else {
+                make(g0, k, sc, false);
             }
 #pragma unroll
-            for (int g = 0; g < GMAX; ++g)
-                if (g0 + g < groups) {
-                    const uint32_t j = first + 64 * (g0 + g);
-                    f(g0 + g, j, keys[g], j <= end);
-                }
+            for (int u = 0; u < U; ++u) {
+                const uint32_t j = first + 64 * (g0 + u);
+                f(j, k[u], g0 + u < groups && j <= end);
+            }
         }
     };
     int all;
     wave_scan<WAVES>(guarded, red, all);
-    uint32_t key = 0xFFFFFFFFu;
+    uint32_t key = kSafeKey;
     int want = keep;   // how many slots of exactly `key` stay, the lowest ones; all with a larger key stay
     if (all < keep) {
         want = keep - all;
@@ -227,8 +237,8 @@ __global__ __launch_bounds__(64 * WAVES) void k_evict_select(KvDev c, EvictDev a
 #pragma unroll
             for (int b = 0; b < BINS; ++b) hist[64 * WAVES * b + t] = 0;
             __syncthreads();
-            each([&](int, uint32_t, uint32_t k, bool in) {
-                if (in && k != 0xFFFFFFFFu && (k & known) == key) atomicAdd(&hist[k >> shift & mask], 1);
+            each([&](uint32_t, uint32_t k, bool in) {
+                if (in && k != kSafeKey && (k & known) == key) atomicAdd(&hist[k >> shift & mask], 1);
             });
             __syncthreads();
             // from the largest digit down, BINS of them a thread: the digit in which the count passes `want`
@@ -257,38 +267,40 @@ __global__ __launch_bounds__(64 * WAVES) void k_evict_select(KvDev c, EvictDev a
             want = pick[1];
         }
     }
-    // every slot's fate, in slot order: f(group, slot, holes' ballot, movers' ballot)
+    // every slot's fate, in slot order: f(slot, holes' ballot, movers' ballot)
     const uint64_t lower = (1ull << lane) - 1;
     int ties = 0, total;
-    each([&](int, uint32_t, uint32_t k, bool in) { ties += __popcll(__ballot(in && k == key)); });
+    each([&](uint32_t, uint32_t k, bool in) { ties += __popcll(__ballot(in && k == key)); });
     const int tie0 = wave_scan<WAVES>(ties, red, total);
     auto fates = [&](auto f) {
         int tie = tie0;
-        each([&](int g, uint32_t j, uint32_t k, bool in) {
+        each([&](uint32_t j, uint32_t k, bool in) {
             const uint64_t eq = __ballot(in && k == key);
             const bool stay = in && (k > key || (k == key && tie + __popcll(eq & lower) < want));
             tie += __popcll(eq);
-            f(g, j, __ballot(in && !stay && j < (uint32_t)a.budget), __ballot(stay && j >= (uint32_t)a.budget));
+            f(j, __ballot(in && !stay && j < (uint32_t)a.budget), __ballot(stay && j >= (uint32_t)a.budget));
         });
     };
     int holes = 0, movers = 0;
-    fates([&](int g, uint32_t, uint64_t ho, uint64_t mo) {
-        holes += __popcll(ho), movers += __popcll(mo);
-        if (REGS && lane == 0) fate[wave * GMAX + g][0] = ho, fate[wave * GMAX + g][1] = mo;
-    });
+    fates([&](uint32_t, uint64_t ho, uint64_t mo) { holes += __popcll(ho), movers += __popcll(mo); });
     holes = wave_scan<WAVES>(holes, red, total);
     movers = wave_scan<WAVES>(movers, red, total);
     if (t == 0) ws[0] = total;
     int *src = ws + 4, *dst = src + evict_most(c.max_len, a.budget);
-    auto put = [&](uint32_t j, uint64_t ho, uint64_t mo) {
+    fates([&](uint32_t j, uint64_t ho, uint64_t mo) {
         if (ho >> lane & 1) dst[holes + __popcll(ho & lower)] = j;
         if (mo >> lane & 1) src[movers + __popcll(mo & lower)] = j;
         holes += __popcll(ho), movers += __popcll(mo);
-    };
-    if constexpr (REGS)
-        for (int g = 0; g < groups; ++g) put(first + 64 * g, fate[wave * GMAX + g][0], fate[wave * GMAX + g][1]);
-    else
-        fates([&](int, uint32_t j, uint64_t ho, uint64_t mo) { put(j, ho, mo); });
+    });
+}
+
+template <int WAVES, int U, int KEEP>
+static int evict_select(const KvDev &c, const EvictDev &a, hipStream_t st) {
+    constexpr int lds = 4 * 64 * WAVES * KEEP;
+    static const hipError_t e = hipFuncSetAttribute((const void *)k_evict_select<WAVES, U, KEEP>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (e != hipSuccess) return hip_check(e, "p8x_kv_evict LDS");
+    k_evict_select<WAVES, U, KEEP><<<dim3(c.n_kv, c.n_seq), 64 * WAVES, lds, st>>>(c, a);
+    return P8X_OK;
 }
 
 // The moves: sources are slots >= budget and destinations slots < budget, so no row is both. D / 8 lanes a row, four rows at a
@@ -339,11 +351,11 @@ __global__ __launch_bounds__(256) void k_evict_move(KvDev c, EvictDev a) {
 
 int launch_kv_evict(const KvDev &c, int D, const p8x_evict_args &p, hipStream_t st) {
     const EvictDev a{p.budget, p.n_sink, p.n_recent, p.score, p.score_out, p.pos, p.pos_out, p.len_out, (int *)p.workspace};
-    const dim3 heads(c.n_kv, c.n_seq);
-    if (c.max_len <= 4 * 4 * 64) k_evict_select<4, 4, true><<<heads, 64 * 4, 0, st>>>(c, a);
-    else if (c.max_len <= 16 * 4 * 64) k_evict_select<16, 4, true><<<heads, 64 * 16, 0, st>>>(c, a);
-    else if (c.max_len <= 16 * 32 * 64) k_evict_select<16, 32, true><<<heads, 64 * 16, 0, st>>>(c, a);
-    else k_evict_select<16, 16, false><<<heads, 64 * 16, 0, st>>>(c, a);
+    const int rc = c.max_len <= 4 * 4 * 64     ? evict_select<4, 4, 4>(c, a, st)
+                   : c.max_len <= 16 * 4 * 64  ? evict_select<16, 4, 4>(c, a, st)
+                   : c.max_len <= 16 * 32 * 64 ? evict_select<16, 8, 32>(c, a, st)
+                                               : evict_select<16, 8, 0>(c, a, st);
+    if (rc) return rc;
     const int64_t rows = 4 * (256 / (D / 8));   // of a workgroup at a time
     const int nb = (int)std::max<int64_t>(1, std::min<int64_t>(((int64_t)evict_most(c.max_len, a.budget) + rows - 1) / rows, 1024));
     const dim3 grid(nb, c.n_kv, c.n_seq);
