@@ -204,10 +204,10 @@ __global__ __launch_bounds__(64 * WAVES) void k_evict_select(KvDev c, EvictDev a
         if (t == 0) ws[0] = 0;
         return;
     }
-    // f(slot, key, whether there is one) over the wave's groups in order
-    auto each = [&](auto f) {
+    // f(group, slot, key, whether there is one) over groups g0 .. g1 - 1 of the wave in order
+    auto each = [&](int g0, int g1, auto f) {
 #pragma unroll 1
-        for (int g0 = 0; g0 < groups; g0 += U) {
+        for (; g0 < g1; g0 += U) {
             uint32_t k[U], sc[U];
             if constexpr (KEEP) {
 #pragma unroll
@@ -218,7 +218,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_evict_select(KvDev c, EvictDev a
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const uint32_t j = first + 64 * (g0 + u);
-                f(j, k[u], g0 + u < groups && j <= end);
+                f(g0 + u, j, k[u], g0 + u < g1 && j <= end);
             }
         }
     };
@@ -237,7 +237,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_evict_select(KvDev c, EvictDev a
 #pragma unroll
             for (int b = 0; b < BINS; ++b) hist[64 * WAVES * b + t] = 0;
             __syncthreads();
-            each([&](uint32_t, uint32_t k, bool in) {
+            each(0, groups, [&](int, uint32_t, uint32_t k, bool in) {
                 if (in && k != kSafeKey && (k & known) == key) atomicAdd(&hist[k >> shift & mask], 1);
             });
             __syncthreads();
@@ -267,31 +267,71 @@ __global__ __launch_bounds__(64 * WAVES) void k_evict_select(KvDev c, EvictDev a
             want = pick[1];
         }
     }
-    // every slot's fate, in slot order: f(slot, holes' ballot, movers' ballot)
-    const uint64_t lower = (1ull << lane) - 1;
-    int ties = 0, total;
-    each([&](uint32_t, uint32_t k, bool in) { ties += __popcll(__ballot(in && k == key)); });
-    const int tie0 = wave_scan<WAVES>(ties, red, total);
-    auto fates = [&](auto f) {
-        int tie = tie0;
-        each([&](uint32_t j, uint32_t k, bool in) {
-            const uint64_t eq = __ballot(in && k == key);
-            const bool stay = in && (k > key || (k == key && tie + __popcll(eq & lower) < want));
-            tie += __popcll(eq);
-            f(j, __ballot(in && !stay && j < (uint32_t)a.budget), __ballot(stay && j >= (uint32_t)a.budget));
+    // Every slot's fate, 64 groups at a time: lane i has the ballots of group c0 + i, so that what goes on in the slots' order
+    // is a scan over lanes.
+    uint64_t more, same;   // keys above and at `key`
+    auto sweep = [&](int c0) {
+        more = same = 0;
+        each(c0, min(groups, c0 + 64), [&](int g, uint32_t, uint32_t k, bool in) {
+            const uint64_t up = __ballot(in && k > key), eq = __ballot(in && k == key);
+            if (lane == g - c0) more = up, same = eq;
         });
     };
-    int holes = 0, movers = 0;
-    fates([&](uint32_t, uint64_t ho, uint64_t mo) { holes += __popcll(ho), movers += __popcll(mo); });
+    auto scan = [&](int v) {   // over lanes, own included
+        for (int o = 1; o < 64; o <<= 1) {
+            const int y = __shfl_up(v, o);
+            if (lane >= o) v += y;
+        }
+        return v;
+    };
+    const bool once = groups <= 64;   // the ballots stay
+    int ties = 0, total;
+#pragma unroll 1
+    for (int c0 = 0; c0 < groups; c0 += 64) {
+        sweep(c0);
+        ties += __builtin_amdgcn_readlane(scan(__popcll(same)), 63);
+    }
+    const int tie0 = wave_scan<WAVES>(ties, red, total);
+    int tie, holes = 0, movers = 0;
+    uint64_t ho, mo;   // of the lane's group: slots below the budget that go, slots above it that stay
+    auto fates = [&](int c0) {
+        if (!once) sweep(c0);
+        const int cnt = __popcll(same), upto = tie + scan(cnt), left = want - (upto - cnt);
+        tie = __builtin_amdgcn_readlane(upto, 63);
+        uint64_t go = left >= cnt ? 0 : same;   // of the slots at `key`: all but the lowest `left`
+        for (int i = 0; i < left && go; ++i) go &= go - 1;
+        const uint64_t stay = more | (same & ~go);
+        const int64_t j = ((int64_t)wave * groups + c0 + lane) * 64, in = n - j, low = a.budget - j;   // the group's first slot
+        const uint64_t there = c0 + lane >= groups || in <= 0 ? 0 : in >= 64 ? ~0ull : (1ull << in) - 1;
+        const uint64_t below = low <= 0 ? 0 : low >= 64 ? ~0ull : (1ull << low) - 1;
+        ho = there & below & ~stay;
+        mo = there & stay & ~below;
+    };
+    tie = tie0;
+#pragma unroll 1
+    for (int c0 = 0; c0 < groups; c0 += 64) {
+        fates(c0);
+        holes += __builtin_amdgcn_readlane(scan(__popcll(ho)), 63), movers += __builtin_amdgcn_readlane(scan(__popcll(mo)), 63);
+    }
     holes = wave_scan<WAVES>(holes, red, total);
     movers = wave_scan<WAVES>(movers, red, total);
     if (t == 0) ws[0] = total;
     int *src = ws + 4, *dst = src + evict_most(c.max_len, a.budget);
-    fates([&](uint32_t j, uint64_t ho, uint64_t mo) {
-        if (ho >> lane & 1) dst[holes + __popcll(ho & lower)] = j;
-        if (mo >> lane & 1) src[movers + __popcll(mo & lower)] = j;
-        holes += __popcll(ho), movers += __popcll(mo);
-    });
+    const uint64_t lower = (1ull << lane) - 1;
+    tie = tie0;
+#pragma unroll 1
+    for (int c0 = 0; c0 < groups; c0 += 64) {
+        if (!once) fates(c0);
+        const int hs = holes + scan(__popcll(ho)), ms = movers + scan(__popcll(mo)), h0 = hs - __popcll(ho), m0 = ms - __popcll(mo);
+        holes = __builtin_amdgcn_readlane(hs, 63), movers = __builtin_amdgcn_readlane(ms, 63);
+        for (int i = 0; i < min(64, groups - c0); ++i) {
+            auto of = [&](uint64_t v) { return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), i) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, i); };
+            const uint64_t gh = of(ho), gm = of(mo);
+            const uint32_t j = first + 64 * (c0 + i);
+            if (gh >> lane & 1) dst[__builtin_amdgcn_readlane(h0, i) + __popcll(gh & lower)] = j;
+            if (gm >> lane & 1) src[__builtin_amdgcn_readlane(m0, i) + __popcll(gm & lower)] = j;
+        }
+    }
 }
 
 template <int WAVES, int U, int KEEP>
@@ -353,7 +393,7 @@ int launch_kv_evict(const KvDev &c, int D, const p8x_evict_args &p, hipStream_t 
     const EvictDev a{p.budget, p.n_sink, p.n_recent, p.score, p.score_out, p.pos, p.pos_out, p.len_out, (int *)p.workspace};
     const int rc = c.max_len <= 4 * 4 * 64     ? evict_select<4, 4, 4>(c, a, st)
                    : c.max_len <= 16 * 4 * 64  ? evict_select<16, 4, 4>(c, a, st)
-                   : c.max_len <= 16 * 32 * 64 ? evict_select<16, 8, 32>(c, a, st)
+                   : c.max_len <= 16 * 32 * 64 ? evict_select<16, 16, 32>(c, a, st)
                                                : evict_select<16, 8, 0>(c, a, st);
     if (rc) return rc;
     const int64_t rows = 4 * (256 / (D / 8));   // of a workgroup at a time

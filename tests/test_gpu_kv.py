@@ -154,6 +154,13 @@ def test_evict_long():
     run_evict(Case([70001], [0], fused=False, heads=1, kv=1, D=64, page=64, seed=3), 333, 0, 0, "ties", with_pos=False)
 
 
+@pytest.mark.parametrize("kind", ["skewed", "ties", "equal", "odd"])
+@pytest.mark.parametrize("lens,budget,recent", [([4097, 5000], 4096, 64), ([20011, 31], 77, 9), ([32700, 9000], 16001, 0)])
+def test_evict_of_thousands(lens, budget, recent, kind):
+    """rows whose keys a workgroup holds in shared memory, many groups of 64 a wave"""
+    run_evict(Case(lens, [0, 0], fused=False, heads=1, kv=1, D=64, page=64, seed=8), budget, 3, recent, kind)
+
+
 def test_evict_in_place_without_positions_and_pages_outside():
     run_evict(Case([300, 200], [0, 0], fused=False, seed=4), 128, 4, 16, "skewed", in_place=True)
     run_evict(Case([300, 90], [0, 0], fused=False, seed=5, table=False, layout="slot", cache=BF16), 100, with_pos=False)
