@@ -16,7 +16,7 @@
 //
 // Work: the 32-slot tiles of all (sequence, head, row tile) segments in a row, an equal share for each of one workgroup a
 // compute unit. Where the shares can be cut at the segments' ends without more workgroups or longer shares they are (each
-// segment that a workgroup visits costs it about 8 us of latency: queries, sums through LDS, records); else a share may
+// segment that a workgroup visits costs it some 8 us of latency: queries, sums through LDS, records); else a share may
 // span segments. A segment of several workgroups leaves records (sums, maximum, sum of weights) that the last of them
 // joins in order, or, where they are many, a second launch.
 #include <hip/hip_runtime.h>
@@ -43,7 +43,8 @@ struct AttnJob {
     unsigned *count;   // arrivals of a segment's workgroups, 0 between calls
     float *part;       // two records a workgroup: rows x D sums, then rows x (m, l)
     int2 *where;       // of a segment: first workgroup, workgroups (for a join launch)
-    int rw, rt, least; // row waves of a workgroup; row tiles of a sequence at most; units a workgroup takes at least
+    int rw, rt, least; // row waves of a workgroup; row tiles of a sequence at most; units a workgroup takes at least: a tile a wave (twice or
+                       // four times that: 15.4 to 18.2 and 20.6 us for one token over 1001 slots)
     int split;         // unit: a tile; 0: a whole segment (no records)
     int join;          // records are joined by a launch of their own
     int nwg;
@@ -881,16 +882,26 @@ __global__ __launch_bounds__(64 * attn_waves(D, SHARE)) void k_attn(AttnJob J) {
     }
 }
 
-// Rows of a wave and row waves of a workgroup. Up to 32 rows: 16 or 32 in every wave (16 with queries of several parts or rows
-// of 256 elements, whose operands fill the registers), the waves take slots in turn. More: 4 or 8 waves share K and V through
-// LDS, each with 16 or 32 of the rows.
-constexpr size_t kJoinBytes = 96 << 10;   // records of a segment of more bytes than this are joined by a launch of their own
+// Rows of a wave and row waves of a workgroup. Few rows: 16 or 32 in every wave (16 with queries of several parts or rows of
+// 256 elements, whose operands fill the registers), at most two row waves, the other waves take slots in turn; up to two
+// such row tiles, each reading K and V for itself. More rows: 8 waves (4 of twice the registers for rows of 256) share K and V
+// through LDS, each with 16 or 32 of the rows. us, few-rows form then sharing (2 sequences x 32767 slots x 8 heads, 65535 for
+// head_dim 64, 16383 for 256; bf16, in brackets f32 queries):
+//   head_dim   64: 64 rows 78 (101) and 104 (116), 96 rows 105 (146) and 107 (123)
+//   head_dim  128: 64 rows 77 (88) and 78 (91), 96 rows 98 (125) and 79 (93), 256 rows 174 (310) and 117 (171)
+//   head_dim  256: 64 rows (86.5) and (83.5), 96 rows (121) and (109)
+// hence above 64 rows, above 32 of 256 elements. 32 rows a wave against 16 where both fit: 105 to 130 us at 512 rows, 4
+// sequences x 16383 slots.
+// Records of a segment of more than kJoinBytes are joined by a launch of their own, else by the segment's last
+// workgroup: 118.8 to 126.5 us at 32 rows and 32 records (530 KB), 22.5 to 32.6 at 8190 slots; the other way 14.8 to
+// 16.3 at 4 rows and 5 records (10 KB).
+constexpr size_t kJoinBytes = 96 << 10;
 struct AttnPlan { int nt, rw, rows_wg, rt, share; size_t segs, rec_bytes, head_bytes; };
 static AttnPlan attn_plan(const KvDev &c, const DraftDev &d, int D) {
     AttnPlan p;
     const int rows = d.max_tokens * d.G;
-    if (rows > 32) {
-        p.share = rows <= 64 || D == 256 ? 4 : 8;
+    if (rows > (D == 256 ? 32 : 64)) {
+        p.share = D == 256 ? 4 : 8;
         p.nt = rows > 16 * p.share && !d.q_f32 && D < 256 ? 2 : 1;
         p.rw = p.share;
     } else {
@@ -919,6 +930,8 @@ static int attn_run(const AttnJob &J, int rows_wg, hipStream_t st) {
     if (e != hipSuccess) return hip_check(e, "p8x_attn_tree LDS");
     k_attn<D, BF, QF, NT, SHARE><<<J.nwg, 64 * waves, lds, st>>>(J);
     const dim3 heads(0, J.rt, J.c.n_seq * J.c.n_kv);
+    // eight threads to four elements where a segment has many records: 22.7 to 26.0 us at 32 records of 32 rows, but 114 to 104 at 8
+    // of 256
     if (J.join && J.nwg > 12 * (int)(heads.y * heads.z)) k_attn_join<D, BF, QF, 8><<<dim3((rows_wg * (D / 4) + 31) / 32, heads.y, heads.z), 256, 0, st>>>(J, rows_wg);
     else if (J.join) k_attn_join<D, BF, QF, 1><<<dim3((rows_wg * (D / 4) + 255) / 256, heads.y, heads.z), 256, 0, st>>>(J, rows_wg);
     return hip_check(hipGetLastError(), "p8x_attn_tree launch");
@@ -926,14 +939,11 @@ static int attn_run(const AttnJob &J, int rows_wg, hipStream_t st) {
 
 template <int D, bool BF, bool QF>
 static int attn_form(const AttnJob &J, const AttnPlan &p, hipStream_t st) {
-    if constexpr (D < 256) {
-        if constexpr (!QF) {
-            if (p.share == 8 && p.nt == 2) return attn_run<D, BF, QF, 2, 8>(J, p.rows_wg, st);
-            if (!p.share && p.nt == 2) return attn_run<D, BF, QF, 2, 0>(J, p.rows_wg, st);
-        }
-        if (p.share == 8) return attn_run<D, BF, QF, 1, 8>(J, p.rows_wg, st);
+    constexpr int SHARED = D == 256 ? 4 : 8;
+    if constexpr (D < 256 && !QF) {
+        if (p.nt == 2) return p.share ? attn_run<D, BF, QF, 2, SHARED>(J, p.rows_wg, st) : attn_run<D, BF, QF, 2, 0>(J, p.rows_wg, st);
     }
-    return p.share ? attn_run<D, BF, QF, 1, 4>(J, p.rows_wg, st) : attn_run<D, BF, QF, 1, 0>(J, p.rows_wg, st);
+    return p.share ? attn_run<D, BF, QF, 1, SHARED>(J, p.rows_wg, st) : attn_run<D, BF, QF, 1, 0>(J, p.rows_wg, st);
 }
 
 template <int D>
