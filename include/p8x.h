@@ -308,6 +308,8 @@ typedef struct p8x_kv_cache {
     const int32_t *pages; size_t ld_pages;   /* NULL: sequence s lies in page s */
     const int32_t *len;             /* [n_seq] slots in use, clamped to 0 .. max_len */
     int max_len;                    /* slots a sequence can hold; also the row length of score and pos arrays */
+    /* p8x_attn_tree and p8x_kv_score: slot_stride below 2^26; p8x_attn_tree: fewer than 2^29 tiles of 32 slots over all heads
+     * and row tiles, else P8X_ERR_UNSUPPORTED */
 } p8x_kv_cache;
 
 /* Drafted tokens as a layer's products leave them: sequence s has tokens first[s] .. first[s + 1] - 1 (at most

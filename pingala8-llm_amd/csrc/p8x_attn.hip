@@ -18,7 +18,14 @@
 // compute unit. Where the shares can be cut at the segments' ends without more workgroups or longer shares they are (each
 // segment that a workgroup visits costs it some 8 us of latency: queries, sums through LDS, records); else a share may
 // span segments. A segment of several workgroups leaves records (sums, maximum, sum of weights) that the last of them
-// joins in order, or, where they are many, a second launch.
+// joins in order, or, where they are many, a second launch. (Shares that always span segments: 118 to 125 us at one sequence of
+// 131071 slots, 106 to 111 at four trees of 64, 73 either way at 16 sequences.)
+//
+// What bounds it: HBM for few rows (8 tokens x 4 heads over 131071 slots x 8 heads, 537 MB: 117 us, 4.6 TB/s with the join; 16
+// sequences, 301 MB: 73 us, 4.1 TB/s, the ends of 128 segments included). For many rows the VALU and matrix instructions
+// of a tile: 256 rows by 32 slots take a compute unit 1.8 us, where K and V would take 1 from HBM (4 x 64 tokens x 32
+// heads over 46484 slots, 43.7 GFLOP: 102 us, 430 TFLOP/s). One token over 1001 slots: 14.5 us of latency: 2 the shares, 3.5 the
+// first tile, 2.5 its products (instructions come from memory too), 4 the waves' sums, 3 the join.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -30,7 +37,8 @@ namespace p8x {
 // Waves of a workgroup, one of which a compute unit holds: 8 of 256 registers a lane, or 4 of 512 for rows of 256 elements.
 // SHARE: the waves that share K and V through LDS, 0 for none.
 __host__ __device__ constexpr int attn_waves(int D, int share) { return share ? share : D == 256 ? 4 : 8; }
-constexpr float kLazy = 8.0f;   // log2 of how far a weight may exceed 1 before its row's maximum moves
+// log2 of how far a weight may exceed 1 before its row's maximum moves (0: 106 to 116 us at 256 rows a workgroup)
+constexpr float kLazy = 8.0f;
 // tiles that a workgroup's waves share through LDS at a time
 __host__ __device__ constexpr int stage_tiles(int D) { return D == 256 ? 1 : 2; }
 constexpr int kStages = 4;   // stages in LDS: one in use, the others on their way

@@ -3,7 +3,7 @@
 //
 // One workgroup a row, the row in registers between its one read and its one write; two sums through LDS (three or four
 // with layer norms: mean, then the sum of squares about it). Bound by HBM for many rows and by the launch and
-// three memory round trips for few.
+// three memory round trips for few: 1500 rows of 5120 with a gate (138 MB) 32.5 us, 4.25 TB/s; one row of 4096 4.0 us.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -171,7 +171,7 @@ static void norm_run(const NormDev &J, int nt, bool vec, hipStream_t st) {
 
 int launch_norm_residual(const p8x_norm_args &a, hipStream_t st) {
     const NormDev J{a};
-    // four at a time: rows and pointers allow it
+    // four at a time where rows and pointers allow it (one at a time: 60 us for 33 at 1500 rows of 5120, 6.5 for 4.2 at one of 4096)
     bool vec = a.C % 4 == 0;
     auto four = [&](const void *p, int dtype, size_t ld) {
         if (p && ((uintptr_t)p % (dtype == P8X_F32 ? 16 : 8) || (a.n > 1 && ld % 4))) vec = false;
@@ -182,8 +182,8 @@ int launch_norm_residual(const p8x_norm_args &a, hipStream_t st) {
     four(a.x, a.x_dtype, a.ldx);
     if (a.y) four(a.gate, a.gate_dtype, a.ld_gate);
     for (const float *w : {a.w_post, a.b_post, a.w_pre, a.b_pre}) four(w, P8X_F32, 0);
-    // few rows: as many threads as groups of four, for the shortest chain; many: 256 threads, so that several rows' loads and
-    // sums overlap on a compute unit
+    // few rows: as many threads as groups of four, for the shortest chain (256 rows of 4096: 4.7 us, 5.7 with 256 threads); many:
+    // 256 threads, so that several rows' loads and sums overlap on a compute unit (1500 rows of 5120: 33.3 us, 36.8 with 1024)
     const int groups = (a.C + 3) / 4, most = a.n <= num_cus() ? 1024 : 256;
     int nt = std::min(most, (groups + 63) / 64 * 64);
     while ((groups + nt - 1) / nt > 8) nt *= 2;
