@@ -625,6 +625,13 @@ __global__ __launch_bounds__(64 * attn_waves(D, SHARE)) void k_attn(AttnJob J) {
             auto place = [&](int t) { return lds + ((t - t0) / ST % kStages) * 2 * STAGE + 32 * ((t - t0) % ST) * W::ROW; };
 #pragma unroll 1
             for (int st = -1; st < 1; ++st) arrive(st);   // (-1: the first loads)
+            // the next tile's pages, read with its K: a wait for them after V's reads would be one for V
+            int pg[2];
+            auto pages = [&](int t) {
+                const int *p = paged[(t - t0) / ST % 8] + 2 * ((t - t0) % ST);
+                pg[0] = p[0], pg[1] = p[1];
+            };
+            pages(t0);
             w.lds_k(place(t0));
             uint32_t odd[2] = {0, 0};
             // One body for all tiles, so that the sums stay in their registers. V of a tile and K of the next come from LDS while the
@@ -636,7 +643,7 @@ __global__ __launch_bounds__(64 * attn_waves(D, SHARE)) void k_attn(AttnJob J) {
                 w.qk(x);
                 __builtin_amdgcn_sched_barrier(0);
                 w.lds_v(place(t) + STAGE);
-                uint32_t in = (paged[st % 8][2 * i] ? 0xFFFFu : 0) | (paged[st % 8][2 * i + 1] ? 0xFFFF0000u : 0);
+                uint32_t in = (pg[0] ? 0xFFFFu : 0) | (pg[1] ? 0xFFFF0000u : 0);
                 in = t < ctx ? __builtin_amdgcn_readfirstlane(in) & (left >= 32 ? 0xFFFFFFFFu : (1u << left) - 1) : 0;
                 if (t >= ctx) {
                     const uint32_t o = (uint32_t)__ballot(lane < 32 && odd_row[st % 8][32 * i + lane]);
@@ -645,6 +652,7 @@ __global__ __launch_bounds__(64 * attn_waves(D, SHARE)) void k_attn(AttnJob J) {
                 }
                 if (t + 1 < t1) {
                     if (i == ST - 1) arrive(st + 1);
+                    pages(t + 1);
                     w.lds_k(place(t + 1));
                 }
                 __builtin_amdgcn_sched_barrier(0);
