@@ -24,7 +24,7 @@
 // What bounds it: HBM for few rows (8 tokens x 4 heads over 131071 slots x 8 heads, 537 MB: 117 us, 4.6 TB/s with the join; 16
 // sequences, 301 MB: 73 us, 4.1 TB/s, the ends of 128 segments included). For many rows the VALU and matrix instructions
 // of a tile: 256 rows by 32 slots take a compute unit 1.8 us, where K and V would take 1 from HBM (4 x 64 tokens x 32
-// heads over 46484 slots, 43.7 GFLOP: 102 us, 430 TFLOP/s). One token over 1001 slots: 14.5 us of latency: 2 the shares, 3.5 the
+// heads over 46484 slots, 43.7 GFLOP: 101 us, 430 TFLOP/s). One token over 1001 slots: 14.5 us of latency: 2 the shares, 3.5 the
 // first tile, 2.5 its products (instructions come from memory too), 4 the waves' sums, 3 the join.
 #include <hip/hip_runtime.h>
 
