@@ -332,7 +332,8 @@ typedef struct p8x_drafts {
  * P8X_F32 queries are multiplied in f32 accuracy (as sums of 16-bit parts), 16-bit ones as they are; the weights are
  * rounded to no less than 16 bits either way, sums are f32.
  * workspace: device memory that splits a sequence over workgroups (NULL or too little: fewer of them), zeroed
- * once by the caller before its first use and left zeroed where it has to be; calls that may overlap need one each.
+ * once by the caller before its first use and left zeroed where it has to be, for calls of any shape in turn; calls that
+ * may overlap need one each.
  * p8x_attn_workspace: bytes beyond which more do not help for this shape. */
 #define P8X_MAX_DRAFT 64
 int p8x_attn_tree(const p8x_kv_cache *c, const p8x_drafts *d, void *out, size_t ld_out, size_t head_stride_out, float *lse,

@@ -912,6 +912,9 @@ __global__ __launch_bounds__(64 * attn_waves(D, SHARE)) void k_attn(AttnJob J) {
 // workgroup: 118.8 to 126.5 us at 32 rows and 32 records (530 KB), 22.5 to 32.6 at 8190 slots; the other way 14.8 to
 // 16.3 at 4 rows and 5 records (10 KB).
 constexpr size_t kJoinBytes = 96 << 10;
+// The workspace starts with as many counters whatever the shape, so that calls of other shapes, which write
+// places and records behind them, leave them zero; more segments are joined by a launch.
+constexpr size_t kCounters = 4096;
 struct AttnPlan { int nt, rw, rows_wg, rt, share; size_t segs, rec_bytes, head_bytes; };
 static AttnPlan attn_plan(const KvDev &c, const DraftDev &d, int D) {
     AttnPlan p;
@@ -928,7 +931,7 @@ static AttnPlan attn_plan(const KvDev &c, const DraftDev &d, int D) {
     p.rows_wg = 16 * p.nt * p.rw;
     p.rt = (rows + p.rows_wg - 1) / p.rows_wg;
     p.segs = (size_t)c.n_seq * c.n_kv * p.rt;
-    p.head_bytes = (12 * p.segs + 8 + 255) / 256 * 256;   // counters, then places
+    p.head_bytes = 4 * kCounters + (8 * p.segs + 255) / 256 * 256;   // counters, then places
     p.rec_bytes = 4 * (size_t)p.rows_wg * (D + 2);
     return p;
 }
@@ -974,7 +977,7 @@ int launch_attn_tree(const KvDev &c, const DraftDev &d, int D, void *out, size_t
     const size_t most = p.segs * ((size_t)(c.max_len + 31) / 32 + 2);   // tiles
     if (most >= (1u << 29)) return set_error(P8X_ERR_UNSUPPORTED, "p8x_attn_tree: %zu tiles of 32 slots (fewer than 2^29)", most);
     if (c.slot_stride >= (1u << 26)) return set_error(P8X_ERR_UNSUPPORTED, "p8x_attn_tree: slot_stride %zu (below 2^26)", c.slot_stride);
-    AttnJob J{c, d, out, ldo, hso, lse, (unsigned *)ws, (float *)((char *)ws + p.head_bytes), (int2 *)((char *)ws + (4 * p.segs + 7) / 8 * 8), p.rw, p.rt, attn_waves(D, p.share) / p.rw, 1, 0, 0};
+    AttnJob J{c, d, out, ldo, hso, lse, (unsigned *)ws, (float *)((char *)ws + p.head_bytes), (int2 *)((char *)ws + 4 * kCounters), p.rw, p.rt, attn_waves(D, p.share) / p.rw, 1, 0, 0};
     const size_t room = ws_bytes > p.head_bytes ? (ws_bytes - p.head_bytes) / (2 * p.rec_bytes) : 0;   // workgroups with records
     int nwg = (int)std::min<size_t>(num_cus(), room);
     if (nwg < 16 || p.segs / p.rt > 65535 || p.rt > 65535) {   // whole segments then
@@ -985,7 +988,7 @@ int launch_attn_tree(const KvDev &c, const DraftDev &d, int D, void *out, size_t
     J.nwg = nwg;
     // records of a segment, about, that one workgroup would join
     const size_t rows = std::min((size_t)d.max_tokens * d.G, (size_t)p.rows_wg), each = J.split ? nwg / p.segs * rows * (D + 2) * 4 : 0;
-    J.join = J.split && (p.share || each > kJoinBytes);
+    J.join = J.split && (p.share || each > kJoinBytes || p.segs > kCounters);
     return D == 64 ? attn_types<64>(J, p, st) : D == 128 ? attn_types<128>(J, p, st) : attn_types<256>(J, p, st);
 }
 

@@ -92,6 +92,33 @@ def test_sequences_beyond_the_work_of_one_wave_of_workgroups():
     check_attn(c, *run_attn(c))
 
 
+def test_one_workspace_for_calls_of_any_shape():
+    """in turn: few segments with many records, many with few, rows shared through LDS, more segments than counters"""
+    cases = [Case([6000], [3], heads=4, kv=1, D=128, seed=120), Case([150 + s for s in range(60)], [2] * 60, heads=4, kv=2, D=64, seed=121),
+             Case([3000, 64], [40, 40], heads=4, kv=2, seed=122), Case([5 + s % 90 for s in range(1100)], [1] * 1100, heads=4, kv=4, D=64, seed=123)]
+    calls, most = [], 0
+    for c in cases:
+        cache, d, out = c.make_cache(), c.drafts(), c.dev(np.zeros((c.n, c.H, c.D), np.float32))
+        own = p8x.AttnTree(cache, out, **d)
+        most = max(most, own._args[-1])
+        own.run()
+        p8x.synchronize()
+        calls.append((c, cache, d, out, out.to_numpy(np.float32, (c.n, c.H, c.D)).copy()))
+    ws = p8x.DeviceBuffer(most)
+    ws.fill(0)
+    for size in (most, most // 5):
+        for i in (0, 1, 2, 0, 3, 1, 0, 2, 1):
+            c, cache, d, out, want = calls[i]
+            out.fill(0x7F)
+            p8x.AttnTree(cache, out, workspace=ws, workspace_bytes=size, **d).run()
+            p8x.synchronize()
+            got = out.to_numpy(np.float32, want.shape)
+            # (another split in a smaller workspace: sums in another order)
+            assert np.abs(got - want).max() <= (0 if size == most else 1e-5), (i, size)
+    for c, _, _, _, want in calls[:3]:
+        check_attn(c, want, None)
+
+
 def test_calls_on_a_stream_of_their_own():
     """every call ordered by the stream that it is given, with uploads on that stream just before"""
     c = Case([300, 64], [5, 40], heads=4, kv=2, seed=117, cache=BF16, q=BF16)
