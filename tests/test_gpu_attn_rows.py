@@ -92,6 +92,47 @@ def test_sequences_beyond_the_work_of_one_wave_of_workgroups():
     check_attn(c, *run_attn(c))
 
 
+def test_large_offsets():
+    """a pool whose second page lies past 2^32 bytes and 2^31 elements: rows shared through LDS, then append and eviction"""
+    D, page, n, toks, budget = 64, 64, 100, 40, 90
+    stride = (1 << 31) + 4096
+    c = Case([n], [toks], seed=118, D=D, kv=1, heads=2, page=page, max_len=192, cache=F16, q=F32)
+    c.pages = np.array([[1, 0, 2]], np.int32)
+    rng = np.random.default_rng(1)
+    for pool in (c.kb, c.vb):
+        pool[:3] = rng.standard_normal(pool[:3].shape).astype(np.float16).view(np.uint16)
+    ref, rl = c.attention()
+    big = [p8x.DeviceBuffer(2 * (2 * stride + page * D)) for _ in range(2)]
+    for b, pool in zip(big, (c.kb, c.vb)):
+        for p in range(3):
+            a = np.ascontiguousarray(pool[p])
+            p8x.hip_check(p8x.hip().hipMemcpy(b.addr + 2 * stride * p, a.ctypes.data, a.nbytes, p8x.H2D), "copy")
+    lend = c.dev(np.array([n], np.int32))
+    cache = p8x.KvCache(F16, 1, 1, D, big[0], big[1], page_stride=stride, head_stride=page * D, slot_stride=D, page_size=page, n_pages=3, len=lend,
+                        max_len=192, pages=c.dev(c.pages), ld_pages=3)
+    out, lse, d = c.dev(np.zeros((toks, 2, D), np.float32)), c.dev(np.zeros((toks, 2), np.float32)), c.drafts()
+    p8x.AttnTree(cache, out, lse=lse, **d).run()
+    p8x.KvAppend(cache, len_out=lend, **d).run()
+    score = rng.random((1, 1, 192)).astype(np.float32)
+    sd = c.dev(score)
+    p8x.KvEvict(cache, budget, score=sd, len_out=lend).run()
+    p8x.synchronize()
+    assert np.abs(out.to_numpy(np.float32, ref.shape) - ref).max() < 1e-4 and np.abs(lse.to_numpy(np.float32, rl.shape) - rl).max() < 1e-4
+    assert lend.to_numpy(np.int32, (1,))[0] == budget
+    kept = np.zeros(n + toks, bool)
+    kept[np.argsort(-score[0, 0, :n + toks], kind="stable")[:budget]] = True
+    at = np.arange(budget)
+    at[np.flatnonzero(~kept[:budget])] = np.flatnonzero(kept[budget:]) + budget
+    for b, pool, new in zip(big, (c.kb, c.vb), (c.knb, c.vnb)):
+        rows = np.concatenate([[c.row(pool, 0, j)[0] for j in range(n)], np.ascontiguousarray(new[:, 0]).astype(np.float16).view(np.uint16)])[at]
+        for j in range(budget):
+            p, o = c.place(0, j)
+            got = np.zeros(D, np.uint16)
+            p8x.hip_check(p8x.hip().hipMemcpy(got.ctypes.data, b.addr + 2 * (stride * p + o * D), got.nbytes, p8x.D2H), "copy")
+            assert np.array_equal(got, rows[j]), j
+        b.free()
+
+
 def test_one_workspace_for_calls_of_any_shape():
     """in turn: few segments with many records, many with few, rows shared through LDS, more segments than counters"""
     cases = [Case([6000], [3], heads=4, kv=1, D=128, seed=120), Case([150 + s for s in range(60)], [2] * 60, heads=4, kv=2, D=64, seed=121),
