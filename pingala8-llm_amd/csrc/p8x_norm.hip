@@ -69,11 +69,12 @@ __device__ __forceinline__ float block_sum(float v, float *red) {
     return t;
 }
 
-// 1 / (1 + e^-g) to a few units in the last place: 2^(t + r), t + r = -g log2 e to more than f32
+// 1 / (1 + e^-g) to a few units in the last place: 2^(t + r), t + r = -g log2 e to more than f32. Where 2^t is 0 or infinite, r is
+// of no use, and infinite or NaN where t itself has overflowed.
 __device__ __forceinline__ float sigmoid(float g) {
     const float t = g * -1.44269502f, r = fmaf(g, -1.44269502f, -t) + g * -1.92596299e-8f;
     const float e = __builtin_amdgcn_exp2f(t);
-    return __builtin_amdgcn_rcpf(1.0f + (e < INFINITY ? fmaf(e, r * 0.693147182f, e) : e));
+    return __builtin_amdgcn_rcpf(1.0f + (e > 0.0f && e < INFINITY ? fmaf(e, r * 0.693147182f, e) : e));
 }
 
 // NV groups of four elements a thread, strided by the workgroup's width; Y32, H32, G32: y, h, gate are f32 (VEC).
