@@ -329,8 +329,10 @@ typedef struct p8x_drafts {
 /* out = softmax(scale q k) v over the slots of the token's sequence and the drafted tokens its mask shows, out in q's
  * type, lse [n_tokens][n_heads] = log of the sum of exp (NULL: not stored). A token that sees nothing gets 0 and
  * lse -inf; what a mask hides does not reach the token, be it infinite or NaN. At most P8X_MAX_DRAFT tokens a sequence.
- * P8X_F32 queries are multiplied in f32 accuracy (as sums of 16-bit parts), 16-bit ones as they are; the weights are
- * rounded to no less than 16 bits either way, sums are f32.
+ * P8X_F32 queries are multiplied in f32 accuracy (as sums of 16-bit parts), 16-bit ones as they are; sums are f32. A weight is
+ * held to 2^-17 of itself or better, or, on a P8X_F16 cache, to 2^-19 (P8X_F32 queries: 2^-22) of the largest weight in its 32
+ * slots where that is more, however far those are below others. A value that is infinite or NaN makes the elements of
+ * the tokens that see it infinite or NaN.
  * workspace: device memory that splits a sequence over workgroups (NULL or too little: fewer of them), zeroed
  * once by the caller before its first use and left zeroed where it has to be, for calls of any shape in turn; calls that
  * may overlap need one each.

@@ -9,10 +9,15 @@
 //   A = V^T: from memory, lane (m, g) takes D / 16 elements of its group's 8 slots and transposes them in registers (one
 //   v_perm a dword), output tile t's row m then is element (D / 16) m + t; from LDS, ds_read_b64_tr_b16 transposes blocks
 //   of 4 slots by 16 elements, and row m is element 16 t + m.
-// Softmax: the running maximum m of a row only moves when a score exceeds it by 2^8 in the weight, seen by each lane for
-// itself, so that the usual tile needs no exchange between lanes and no rescaling; sums l stay in their lanes until the
-// end. Weights stand relative to m, times 2^7 for fp16 (subnormals), and enter the product as two 16-bit parts (three for
-// f32 queries on a bf16 cache), so that their rounding does not show in out.
+// Softmax: the reference m of a row, to which its weights are relative, only moves when a score exceeds it by 2^8 in the weight, seen
+// by each lane for itself, so that the usual tile needs no exchange between lanes and no rescaling; sums l stay in their
+// lanes until the end. Weights enter the product as two 16-bit parts (three for f32 queries on a bf16 cache). bf16 parts have
+// the range of f32: a weight keeps 16 bits or more. fp16 parts end at 2^-24: weights stand there times 2^7, and where the largest
+// of a row's weights in a tile is below 2^-12 (2^-10 for f32 queries), as in a tail beside slots that take nearly all, m
+// moves down to it, which the f32 sums have the range for (up to 2^64: what is further below is below 2^-64 of the result).
+// So a weight is held to 2^-17 of itself or 2^-19 (2^-22) of the largest of its tile. (Without moving down, weights e^-15 below
+// the largest were off by 1.4e-3 of themselves, at e^-26 by 10%. Moving from 2^-8 on, the usual spread of scores moves it back and
+// forth: 138 to 146 us at 256 rows of 64, 2 x 65535 slots.)
 //
 // Work: the 32-slot tiles of all (sequence, head, row tile) segments in a row, an equal share for each of one workgroup a
 // compute unit. Where the shares can be cut at the segments' ends without more workgroups or longer shares they are (each
@@ -37,8 +42,9 @@ namespace p8x {
 // Waves of a workgroup, one of which a compute unit holds: 8 of 256 registers a lane, or 4 of 512 for rows of 256 elements.
 // SHARE: the waves that share K and V through LDS, 0 for none.
 __host__ __device__ constexpr int attn_waves(int D, int share) { return share ? share : D == 256 ? 4 : 8; }
-// log2 of how far a weight may exceed 1 before its row's maximum moves (0: 106 to 116 us at 256 rows a workgroup)
-constexpr float kLazy = 8.0f;
+// log2 of how far a weight may exceed 1 before its row's reference moves up (0: 106 to 116 us at 256 rows a workgroup), and of the
+// sums beyond which it does not move down
+constexpr float kUp = 8.0f, kRoom = 64.0f;
 // tiles that a workgroup's waves share through LDS at a time
 __host__ __device__ constexpr int stage_tiles(int D) { return D == 256 ? 1 : 2; }
 constexpr int kStages = 4;   // stages in LDS: one in use, the others on their way
@@ -138,6 +144,7 @@ struct Wave {
     static __device__ __forceinline__ int fv(int row) { return PC < 16 ? (row >> 1 & 3) << 1 : (row & 7) << 1; }
     static constexpr int QP = QF ? (BF ? 3 : 2) : 1, PP = QF && BF ? 3 : 2;   // 16-bit parts of a query and of a weight
     static constexpr float kBias = BF ? 0.0f : 7.0f;
+    static constexpr float kDown = QF ? 10.0f : 12.0f;   // (fp16) log2 of how far below 1 a tile's largest weight may be
     uint4v q[NT][QP][C];
     float4v o[NT][DV];
     float m[NT], l[NT], c2[NT];
@@ -255,18 +262,39 @@ struct Wave {
     // scores to weights: x[a][j] of slot j of the lane's eight (-inf: hidden)
     __device__ __forceinline__ void softmax(float (&x)[NT][8]) {
         float mx[NT];
-        bool move = false;
+        bool far = false;   // one comparison a tile and row, what follows from it only then
 #pragma unroll
         for (int a = 0; a < NT; ++a) {
-            mx[a] = top(top(top(top(x[a][0], x[a][1]), x[a][2]), top(x[a][3], x[a][4])), top(top(x[a][5], x[a][6]), x[a][7])) * c2[a];
-            move |= mx[a] > m[a] + kLazy;
+            mx[a] = top(top(top(top(x[a][0], x[a][1]), x[a][2]), top(x[a][3], x[a][4])), top(top(x[a][5], x[a][6]), x[a][7]));
+            const float d = fmaf(mx[a], c2[a], -m[a]);
+            far |= BF ? d > kUp : fabsf(d + 0.5f * (kDown - kUp)) > 0.5f * (kDown + kUp);
         }
-        if (__any(move)) {
+        bool move = __any(far);
+        uint64_t down = 0;
+        if (!BF && move) {   // up where one of a row's lanes is, down where all four are
+            uint64_t up = 0;
 #pragma unroll
             for (int a = 0; a < NT; ++a) {
-                float v = fmaxf(mx[a], __shfl_xor(mx[a], 16));
+                const float d = fmaf(mx[a], c2[a], -m[a]);
+                const uint64_t low = __ballot(d < -kDown && d > -INFINITY), two = low & low >> 32;
+                up |= __ballot(d > kUp);
+                down |= two & two >> 16 & 0xFFFF;
+            }
+            move = up | down;
+        }
+        if (move) {
+#pragma unroll
+            for (int a = 0; a < NT; ++a) {
+                float v = mx[a] * c2[a];
+                v = fmaxf(v, __shfl_xor(v, 16));
                 v = fmaxf(v, __shfl_xor(v, 32));
-                v = fmaxf(v, m[a]);
+                float least = m[a];   // what the reference may become
+                if (down) {
+                    float s = fmaxf(l[a], __shfl_xor(l[a], 16));
+                    s = fmaxf(s, __shfl_xor(s, 32));
+                    if (v - m[a] < -kDown && v > -INFINITY) least = fminf(m[a], m[a] - (kRoom - __log2f(s)));
+                }
+                v = fmaxf(v, least);
                 const float al = v == -INFINITY || m[a] == v ? 1.0f : __builtin_amdgcn_exp2f(m[a] - v);
                 m[a] = v;
                 l[a] *= al;
