@@ -973,8 +973,8 @@ template <int D, bool BF, bool QF, int NT, int SHARE>
 static int attn_run(const AttnJob &J, int rows_wg, hipStream_t st) {
     constexpr int waves = attn_waves(D, SHARE);
     constexpr int lds = SHARE ? kStages * 2 * 32 * stage_tiles(D) * 2 * D : waves * 16 * NT * (D + 4 + 2) * 4;
-    static const hipError_t e = hipFuncSetAttribute((const void *)k_attn<D, BF, QF, NT, SHARE>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    if (e != hipSuccess) return hip_check(e, "p8x_attn_tree LDS");
+    static OncePerDevice once;
+    if (int rc = allow_lds(once, (const void *)k_attn<D, BF, QF, NT, SHARE>, lds, "p8x_attn_tree LDS")) return rc;
     k_attn<D, BF, QF, NT, SHARE><<<J.nwg, 64 * waves, lds, st>>>(J);
     const dim3 heads(0, J.rt, J.c.n_seq * J.c.n_kv);
     // eight threads to four elements where a segment has many records: 22.7 to 26.0 us at 32 records of 32 rows, but 114 to 104 at 8

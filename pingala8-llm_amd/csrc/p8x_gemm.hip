@@ -679,22 +679,11 @@ int reserve_mul_mat(const p8x_tensor *t, int n_max) {
     return P8X_OK;
 }
 
-// k_mm_finish keeps a row of the output (up to 128 KB) in dynamic LDS. The attribute that allows it is per device:
-// set once on each device this process launches on (callers on several threads serialize here).
+// k_mm_finish keeps a row of the output (up to 128 KB) in dynamic LDS.
 static int finish_lds_attribute() {
-    int dev = 0;
-    int rc = hip_check(hipGetDevice(&dev), "k_mm_finish attribute: hipGetDevice");
-    if (rc) return rc;
-    static std::mutex mu;
-    static std::vector<char> done;
-    std::lock_guard<std::mutex> lock(mu);
-    if ((size_t)dev >= done.size()) done.resize((size_t)dev + 1, 0);
-    if (done[dev]) return P8X_OK;
-    if ((rc = hip_check(hipFuncSetAttribute((const void *)k_mm_finish<float>, hipFuncAttributeMaxDynamicSharedMemorySize, 131072), "k_mm_finish attribute")) ||
-        (rc = hip_check(hipFuncSetAttribute((const void *)k_mm_finish<uint16_t>, hipFuncAttributeMaxDynamicSharedMemorySize, 131072), "k_mm_finish attribute")))
-        return rc;
-    done[dev] = 1;
-    return P8X_OK;
+    static OncePerDevice f32, f16;
+    const int rc = allow_lds(f32, (const void *)k_mm_finish<float>, 131072, "k_mm_finish attribute");
+    return rc ? rc : allow_lds(f16, (const void *)k_mm_finish<uint16_t>, 131072, "k_mm_finish attribute");
 }
 
 // the launches of one prompt GEMM with its workspace given: xr >= N K fp16, wmm >= the plane bytes (unused when the

@@ -41,6 +41,12 @@ int num_cus() {
     return cus;
 }
 
+int allow_lds(OncePerDevice &once, const void *kernel, int bytes, const char *what) {
+    int dev = 0;
+    if (int rc = hip_check(hipGetDevice(&dev), what)) return rc;
+    return once.run(dev, [&] { return hip_check(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes), what); });
+}
+
 static int nw_tile(uint32_t m) { return nw_of((int)(m >> 29)); }
 
 void side_offsets(size_t n, size_t rows, size_t K, size_t nd, size_t off[6]) {

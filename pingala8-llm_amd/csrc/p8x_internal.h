@@ -8,6 +8,7 @@
 
 #include "../../include/p8x.h"
 #include "p8x_format.h"
+#include "p8x_once.h"
 
 namespace p8x {
 struct GemvJob;
@@ -121,6 +122,8 @@ int upload_job(p8x_tensor *t);
 int scratch_resolve(int device);
 
 int num_cus();
+// lets a kernel have `bytes` of dynamic LDS on the current device (the attribute is per device); once: of this kernel
+int allow_lds(OncePerDevice &once, const void *kernel, int bytes, const char *what);
 // offsets of the side regions of an n-byte slot, top-down from its end (vrn_offsets, CPU.patch:33-40):
 // delta, c16, prm, pinv, signs, trailer
 void side_offsets(size_t n, size_t rows, size_t K, size_t nd, size_t off[6]);

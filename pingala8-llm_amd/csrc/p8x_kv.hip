@@ -339,8 +339,8 @@ __global__ __launch_bounds__(64 * WAVES) void k_evict_select(KvDev c, EvictDev a
 template <int WAVES, int U, int KEEP>
 static int evict_select(const KvDev &c, const EvictDev &a, hipStream_t st) {
     constexpr int lds = 4 * 64 * WAVES * KEEP;
-    static const hipError_t e = hipFuncSetAttribute((const void *)k_evict_select<WAVES, U, KEEP>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    if (e != hipSuccess) return hip_check(e, "p8x_kv_evict LDS");
+    static OncePerDevice once;
+    if (int rc = allow_lds(once, (const void *)k_evict_select<WAVES, U, KEEP>, lds, "p8x_kv_evict LDS")) return rc;
     k_evict_select<WAVES, U, KEEP><<<dim3(c.n_kv, c.n_seq), 64 * WAVES, lds, st>>>(c, a);
     return P8X_OK;
 }
