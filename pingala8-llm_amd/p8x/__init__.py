@@ -973,11 +973,22 @@ def _drafts(cache, n_tokens, max_tokens, first, k=None, v=None, kv_dtype=F32, ld
                    _address(mask), n_heads, _address(q), q_dtype, n_heads * D if ld_q is None else ld_q, head_stride_q, scale)
 
 
+def _workspace_bytes(name, workspace, nbytes):
+    """how much of a caller's workspace a call may use: of a buffer all of it where nothing is said"""
+    if isinstance(workspace, DeviceBuffer):
+        if nbytes is not None and nbytes > workspace.nbytes:
+            raise P8xError(f"{name}: workspace_bytes {nbytes} of a buffer of {workspace.nbytes}")
+        return workspace.nbytes if nbytes is None else nbytes
+    if workspace and nbytes is None:
+        raise P8xError(f"{name}: a workspace given as an address needs workspace_bytes")
+    return nbytes or 0
+
+
 class AttnTree(_Call):
     """Attention of drafted tokens over the cache and each other (p8x_attn_tree); drafts: the fields of p8x_drafts by
-    name. Without a workspace of the caller's it keeps one of its own."""
+    name. Without a workspace of the caller's it keeps one of its own (0: none, whole sequences a workgroup)."""
 
-    def __init__(self, cache, out, lse=None, ld_out=None, head_stride_out=0, workspace=None, workspace_bytes=0, **drafts):
+    def __init__(self, cache, out, lse=None, ld_out=None, head_stride_out=0, workspace=None, workspace_bytes=None, **drafts):
         d = _drafts(cache, **drafts)
         if workspace is None:
             workspace_bytes = lib().p8x_attn_workspace(ctypes.byref(cache.c), ctypes.byref(d))
@@ -985,6 +996,7 @@ class AttnTree(_Call):
                 workspace = DeviceBuffer(workspace_bytes)
                 workspace.fill(0)
                 synchronize()
+        workspace_bytes = _workspace_bytes("p8x_attn_tree", workspace, workspace_bytes)
         super().__init__("p8x_attn_tree", (ctypes.byref(cache.c), ctypes.byref(d), _address(out), d.n_heads * cache.head_dim if ld_out is None else ld_out,
                                            head_stride_out, _address(lse), _address(workspace), workspace_bytes), (cache, d, drafts, out, lse, workspace))
 
@@ -1012,10 +1024,11 @@ class KvEvict(_Call):
     """The cache cut to a budget (p8x_kv_evict). Without a workspace of the caller's it keeps one of its own."""
 
     def __init__(self, cache, budget, score, len_out, score_out=None, pos=None, pos_out=None, n_sink=0, n_recent=0, workspace=None,
-                 workspace_bytes=0):
+                 workspace_bytes=None):
         if workspace is None:
             workspace_bytes = lib().p8x_kv_evict_workspace(ctypes.byref(cache.c), budget)
             workspace = DeviceBuffer(workspace_bytes)
+        workspace_bytes = _workspace_bytes("p8x_kv_evict", workspace, workspace_bytes)
         a = EvictArgs(budget, n_sink, n_recent, _address(score), _address(score if score_out is None else score_out), _address(pos),
                       _address(pos if pos_out is None else pos_out), _address(len_out), _address(workspace), workspace_bytes)
         super().__init__("p8x_kv_evict", (ctypes.byref(cache.c), ctypes.byref(a)), (cache, a, score, score_out, pos, pos_out, len_out, workspace))
