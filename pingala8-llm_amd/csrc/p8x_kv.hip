@@ -106,8 +106,9 @@ __device__ __forceinline__ uint32_t score_key(float f) {
 }
 
 // sums of v over the waves before this one, and over all; v is the wave's
-template <int WAVES>
+constexpr int kSelectWaves = 16;
 __device__ __forceinline__ int wave_scan(int v, int *red, int &total) {
+    constexpr int WAVES = kSelectWaves;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     __syncthreads();
     if (lane == 0) red[wave] = v;
@@ -118,15 +119,15 @@ __device__ __forceinline__ int wave_scan(int v, int *red, int &total) {
     return __builtin_amdgcn_readfirstlane(before);
 }
 
-// One workgroup of WAVES waves a key/value head. Each wave has a contiguous range of the slots, in groups of 64, a slot a lane:
+// One workgroup of 16 waves a key/value head. Each wave has a contiguous range of the slots, in groups of 64, a slot a lane:
 // the budget-th largest key by three passes of 11, 11 and 10 bits over counts in LDS (protected slots are counted apart), then
 // every slot's fate in slot order, by ballots. KEEP: up to 64 KEEP slots a wave, whose keys stay in LDS, each lane its own;
 // else (0) every pass makes them again from scores and positions. Loops are rolled, U groups a turn: a workgroup runs each
 // pass once, and with all groups unrolled it waited for instructions most of the time. Bound by the latency of the passes on
-// one compute unit a head: 32767 slots 43 us (memory 13, counts 15, fates 10), 1008 slots 10.
-template <int WAVES, int U, int KEEP>
-__global__ __launch_bounds__(64 * WAVES) void k_evict_select(KvDev c, EvictDev a) {
-    constexpr int BINS = 2048 / (64 * WAVES);   // of a thread
+// one compute unit a head: 32767 slots 43 us (memory 13, counts 15, fates 10).
+template <int U, int KEEP>
+__global__ __launch_bounds__(64 * kSelectWaves) void k_evict_select(KvDev c, EvictDev a) {
+    constexpr int WAVES = kSelectWaves, BINS = 2048 / (64 * WAVES);   // of a thread
     __shared__ int hist[2048], red[WAVES], pick[2];
     extern __shared__ uint32_t kept[];   // KEEP: [wave][group][lane]
     const int h = blockIdx.x, s = blockIdx.y, t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -225,7 +226,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_evict_select(KvDev c, EvictDev a
         }
     };
     int all;
-    wave_scan<WAVES>(guarded, red, all);
+    wave_scan(guarded, red, all);
     uint32_t key = kSafeKey;
     int want = keep;   // how many slots of exactly `key` stay, the lowest ones; all with a larger key stay
     if (all < keep) {
@@ -254,7 +255,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_evict_select(KvDev c, EvictDev a
                 if (lane >= o) x += y;
             }
             int total;
-            int above = wave_scan<WAVES>(__builtin_amdgcn_readlane(x, 63), red, total) + x - sum;
+            int above = wave_scan(__builtin_amdgcn_readlane(x, 63), red, total) + x - sum;
             if (above < want && above + sum >= want) {
                 int d = d0;
 #pragma unroll
@@ -293,7 +294,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_evict_select(KvDev c, EvictDev a
         sweep(c0);
         ties += __builtin_amdgcn_readlane(scan(__popcll(same)), 63);
     }
-    const int tie0 = wave_scan<WAVES>(ties, red, total);
+    const int tie0 = wave_scan(ties, red, total);
     int tie, holes = 0, movers = 0;
     uint64_t ho, mo;   // of the lane's group: slots below the budget that go, slots above it that stay
     auto fates = [&](int c0) {
@@ -315,8 +316,8 @@ __global__ __launch_bounds__(64 * WAVES) void k_evict_select(KvDev c, EvictDev a
         fates(c0);
         holes += __builtin_amdgcn_readlane(scan(__popcll(ho)), 63), movers += __builtin_amdgcn_readlane(scan(__popcll(mo)), 63);
     }
-    holes = wave_scan<WAVES>(holes, red, total);
-    movers = wave_scan<WAVES>(movers, red, total);
+    holes = wave_scan(holes, red, total);
+    movers = wave_scan(movers, red, total);
     if (t == 0) ws[0] = total;
     int *src = ws + 4, *dst = src + evict_most(c.max_len, a.budget);
     const uint64_t lower = (1ull << lane) - 1;
@@ -336,12 +337,147 @@ __global__ __launch_bounds__(64 * WAVES) void k_evict_select(KvDev c, EvictDev a
     }
 }
 
-template <int WAVES, int U, int KEEP>
+// The same for rows of at most 64 K slots a wave and 16 waves, whose keys stay in registers, K a lane: four digits of 8 bits, each
+// with counts of its own and one barrier (every wave finds the digit for itself), then ties and fates by ballots. Bound by the
+// latency of its seven barriers and of the scans between them: 1008 slots 12.2 us with the moves, 4000 16.7.
+template <int K>
+__global__ __launch_bounds__(1024) void k_evict_short(KvDev c, EvictDev a) {
+    __shared__ int hist[4][256], red[3][16];
+    const int h = blockIdx.x, s = blockIdx.y, t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), waves = blockDim.x >> 6;
+    const size_t hd = (size_t)s * c.n_kv + h, base = hd * c.max_len;
+    const int n = __builtin_amdgcn_readfirstlane(seq_len(c, s)), keep = min(n, a.budget);
+    int *ws = a.ws + hd * evict_words(c.max_len, a.budget);
+    if (t == 0) ws[1] = n;
+    if (n == 0) {
+        if (t == 0) ws[0] = 0;
+        return;
+    }
+    const int j0 = wave * K * 64 + lane;   // the lane's slots: j0 + 64 g
+    int p[K] = {};
+    float sc[K];
+#pragma unroll
+    for (int g = 0; g < K; ++g) {
+        const int j = min(j0 + 64 * g, n - 1);
+        sc[g] = a.score[base + j];
+        if (a.pos) p[g] = a.pos[base + j];
+    }
+    for (int i = t; i < 1024; i += blockDim.x) hist[0][i] = 0;
+    // slots that stay in place, to the outputs
+#pragma unroll
+    for (int g = 0; g < K; ++g)
+        if (j0 + 64 * g < keep) {
+            if (a.score_out != a.score) a.score_out[base + j0 + 64 * g] = sc[g];
+            if (a.pos && a.pos_out != a.pos) a.pos_out[base + j0 + 64 * g] = p[g];
+        }
+    if (n <= a.budget) {
+        if (t == 0) ws[0] = 0;
+        return;
+    }
+    // sum of the values that the waves put into r, before this wave's and of all
+    auto across = [&](const int *r, int &total) {
+        int v = lane < waves ? r[lane & 15] : 0, before = lane < wave ? v : 0;
+        for (int o = 8; o; o >>= 1) before += __shfl_xor(before, o), v += __shfl_xor(v, o);
+        total = __builtin_amdgcn_readfirstlane(v);
+        return __builtin_amdgcn_readfirstlane(before);
+    };
+    const bool latest = a.pos && a.n_recent;
+    if (latest) {
+        int m = p[0];
+#pragma unroll
+        for (int g = 1; g < K; ++g) m = max(m, p[g]);
+        for (int o = 32; o; o >>= 1) m = max(m, __shfl_xor(m, o));
+        if (lane == 0) red[0][wave] = m;
+    }
+    __syncthreads();
+    int64_t recent = INT64_MAX;   // positions from here on are protected
+    if (latest) {
+        int m = red[0][min(lane & 15, waves - 1)];
+        for (int o = 8; o; o >>= 1) m = max(m, __shfl_xor(m, o));
+        recent = (int64_t)m + 1 - a.n_recent;
+    }
+    uint32_t k[K];
+#pragma unroll
+    for (int g = 0; g < K; ++g) k[g] = a.pos && (p[g] < a.n_sink || p[g] >= recent) ? kSafeKey : score_key(sc[g]);
+    uint32_t key = 0;
+    int want = keep;   // of the keys that agree with `key` in the digits known, how many of the largest stay
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+        const int shift = 24 - 8 * d;
+#pragma unroll
+        for (int g = 0; g < K; ++g) {
+            const uint32_t dig = k[g] >> shift & 255;
+            if (j0 + 64 * g < n && (d == 0 || k[g] >> (shift + 8 & 31) == key >> (shift + 8 & 31))) {
+                // the first lane adds all that have its digit (many slots have the same score, of nothing)
+                const uint64_t same = __ballot(dig == (uint32_t)__builtin_amdgcn_readfirstlane(dig));
+                if (!(same >> lane & 1)) atomicAdd(&hist[d][dig], 1);
+                else if (!(same & ((1ull << lane) - 1))) atomicAdd(&hist[d][dig], __popcll(same));
+            }
+        }
+        __syncthreads();
+        // from the largest digit down, four of them a lane: the one in which the count passes `want`
+        const int4 v = *(const int4 *)&hist[d][252 - 4 * lane];
+        const int sum = v.x + v.y + v.z + v.w;
+        int x = sum;
+        for (int o = 1; o < 64; o <<= 1) {
+            const int y = __shfl_up(x, o);
+            if (lane >= o) x += y;
+        }
+        int above = x - sum, dig = 255 - 4 * lane;
+        const int f = __ffsll((unsigned long long)__ballot(x >= want)) - 1;
+        if (above + v.w < want) {
+            above += v.w, --dig;
+            if (above + v.z < want) {
+                above += v.z, --dig;
+                if (above + v.y < want) above += v.y, --dig;
+            }
+        }
+        key |= (uint32_t)__builtin_amdgcn_readlane(dig, f) << shift;
+        want -= __builtin_amdgcn_readlane(above, f);
+    }
+    // want: how many slots of exactly `key` stay, the lowest ones
+    uint64_t same[K];
+    int ties = 0, total;
+#pragma unroll
+    for (int g = 0; g < K; ++g) same[g] = __ballot(j0 + 64 * g < n && k[g] == key), ties += __popcll(same[g]);
+    if (lane == 0) red[1][wave] = ties;
+    __syncthreads();
+    int tie = across(red[1], total);
+    const uint64_t lower = (1ull << lane) - 1;
+    uint64_t ho[K], mo[K];   // slots below the budget that go, slots above it that stay
+    int counts = 0;          // of the former, and of the latter in the upper half
+#pragma unroll
+    for (int g = 0; g < K; ++g) {
+        const int j = j0 + 64 * g;
+        const bool stay = k[g] > key || (k[g] == key && tie + __popcll(same[g] & lower) < want);
+        tie += __popcll(same[g]);
+        ho[g] = __ballot(j < n && !stay && j < a.budget), mo[g] = __ballot(j < n && stay && j >= a.budget);
+        counts += __popcll(ho[g]) + (__popcll(mo[g]) << 16);
+    }
+    if (lane == 0) red[2][wave] = counts;
+    __syncthreads();
+    const int before = across(red[2], total);
+    if (t == 0) ws[0] = total & 0xFFFF;
+    int *src = ws + 4, *dst = src + evict_most(c.max_len, a.budget);
+    int hole = before & 0xFFFF, mover = before >> 16;
+#pragma unroll
+    for (int g = 0; g < K; ++g) {
+        if (ho[g] >> lane & 1) dst[hole + __popcll(ho[g] & lower)] = j0 + 64 * g;
+        if (mo[g] >> lane & 1) src[mover + __popcll(mo[g] & lower)] = j0 + 64 * g;
+        hole += __popcll(ho[g]), mover += __popcll(mo[g]);
+    }
+}
+
+template <int U, int KEEP>
 static int evict_select(const KvDev &c, const EvictDev &a, hipStream_t st) {
-    constexpr int lds = 4 * 64 * WAVES * KEEP;
+    constexpr int lds = 4 * 64 * kSelectWaves * KEEP;
     static OncePerDevice once;
-    if (int rc = allow_lds(once, (const void *)k_evict_select<WAVES, U, KEEP>, lds, "p8x_kv_evict LDS")) return rc;
-    k_evict_select<WAVES, U, KEEP><<<dim3(c.n_kv, c.n_seq), 64 * WAVES, lds, st>>>(c, a);
+    if (int rc = allow_lds(once, (const void *)k_evict_select<U, KEEP>, lds, "p8x_kv_evict LDS")) return rc;
+    k_evict_select<U, KEEP><<<dim3(c.n_kv, c.n_seq), 64 * kSelectWaves, lds, st>>>(c, a);
+    return P8X_OK;
+}
+template <int K>
+static int evict_short(const KvDev &c, const EvictDev &a, hipStream_t st) {
+    k_evict_short<K><<<dim3(c.n_kv, c.n_seq), (c.max_len + 64 * K - 1) / (64 * K) * 64, 0, st>>>(c, a);
     return P8X_OK;
 }
 
@@ -394,14 +530,14 @@ __global__ __launch_bounds__(256) void k_evict_move(KvDev c, EvictDev a) {
 
 int launch_kv_evict(const KvDev &c, int D, const p8x_evict_args &p, hipStream_t st) {
     const EvictDev a{p.budget, p.n_sink, p.n_recent, p.score, p.score_out, p.pos, p.pos_out, p.len_out, (int *)p.workspace};
-    // The batch of loads fits the groups a wave has, and a workgroup more waves only from where they have work (both calls): 4
-    // waves 14.6 us and 16 waves 17.0 at 1008 slots; batches of 4 and 8 21.1 and 23.2 at 4000; of 8 and 16 24.4 and 29.3 at 6000;
-    // keys in LDS 86 and read again 100 at 32767.
-    const int rc = c.max_len <= 4 * 4 * 64     ? evict_select<4, 4, 4>(c, a, st)
-                   : c.max_len <= 16 * 4 * 64  ? evict_select<16, 4, 4>(c, a, st)
-                   : c.max_len <= 16 * 8 * 64  ? evict_select<16, 8, 8>(c, a, st)
-                   : c.max_len <= 16 * 32 * 64 ? evict_select<16, 16, 32>(c, a, st)
-                                               : evict_select<16, 8, 0>(c, a, st);
+    // Keys in registers up to 8 a lane, as few as fit (both calls, us): 2, 4 and 8 a lane 13.4, 13.7 and 16.1 at 2000 slots; 4 and 8
+    // 15.4 and 16.8 at 3000; 1 and 2 the same at 1008. With k_evict_select instead 14.6 at 1008 slots, 18.1 at 2000, 20.8 at 4000, 24.5 for 19.7
+    // at 6000. There keys in LDS 86 and read again 100 at 32767.
+    const int rc = c.max_len <= 1024 * 2       ? evict_short<2>(c, a, st)
+                   : c.max_len <= 1024 * 4     ? evict_short<4>(c, a, st)
+                   : c.max_len <= 1024 * 8     ? evict_short<8>(c, a, st)
+                   : c.max_len <= 16 * 32 * 64 ? evict_select<16, 32>(c, a, st)
+                                               : evict_select<8, 0>(c, a, st);
     if (rc) return rc;
     const int64_t rows = 4 * (256 / (D / 8));   // of a workgroup at a time
     const int nb = (int)std::max<int64_t>(1, std::min<int64_t>(((int64_t)evict_most(c.max_len, a.budget) + rows - 1) / rows, 1024));
