@@ -269,8 +269,9 @@ typedef struct p8x_batch_info { int njobs, ncols, class_set, units, split_jobs, 
 int p8x_gemv_batch_info(const p8x_gemv_batch *b, p8x_batch_info *out);
 
 /* ---- between the linears: norms, cache, attention of drafted tokens ---------------------------------------- */
-/* No counterpart in the reference (ggml's own kernels run there): what a decode step over drafted tokens needs beside
- * p8x_mul_mat_vec and p8x_mul_mat, for hosts that have no other kernels for it. All calls are asynchronous on the
+/* No counterpart in the reference (ggml's own kernels run there): norms with residual, the cache and its attention for a
+ * decode step over drafted tokens, beside p8x_mul_mat_vec and p8x_mul_mat, for hosts that have no other kernels for them (not
+ * here: rotary embedding, norms of single heads in a q, k, v row). All calls are asynchronous on the
  * stream, allocate nothing, record kernel launches only and are deterministic; they keep nothing between calls. The
  * structs are read during the call, what they point to is device memory. Fields left 0 / NULL take the stated default. */
 enum { P8X_NORM_NONE = 0, P8X_NORM_RMS = 1, P8X_NORM_LAYER = 2 };

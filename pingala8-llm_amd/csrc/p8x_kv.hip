@@ -361,7 +361,7 @@ __global__ __launch_bounds__(1024) void k_evict_short(KvDev c, EvictDev a) {
         sc[g] = a.score[base + j];
         if (a.pos) p[g] = a.pos[base + j];
     }
-    for (int i = t; i < 1024; i += blockDim.x) hist[0][i] = 0;
+    for (int i = t; i < 1024; i += blockDim.x) hist[i >> 8][i & 255] = 0;
     // slots that stay in place, to the outputs
 #pragma unroll
     for (int g = 0; g < K; ++g)

@@ -123,8 +123,8 @@ __global__ __launch_bounds__(64 * kScoreWaves) void k_score(ScoreJob J) {
         }
         __syncthreads();
 
-        // the tile's weights, summed over the rows: lane l < 32 has slot l's. hide: bit i of byte t set where row 4 g + i of
-        // the row tile does not see the lane's slot of half t
+        // the tile's weights, summed over the rows: lane l < 32 has slot l's. draft: the slots are drafted tokens, of which a row
+        // counts those that its mask shows; tj0, tj1: the token of the lane's slot in either half
         auto sum_rows = [&](bool draft, int tj0, int tj1) {
             float w0 = 0.0f, w1 = 0.0f;
             for (int r = 0; r < rt; ++r) {
