@@ -332,8 +332,8 @@ typedef struct p8x_drafts {
  * lse -inf; what a mask hides does not reach the token, be it infinite or NaN. At most P8X_MAX_DRAFT tokens a sequence.
  * P8X_F32 queries are multiplied in f32 accuracy (as sums of 16-bit parts), 16-bit ones as they are; sums are f32. A weight is
  * held to 2^-17 of itself or better, or, on a P8X_F16 cache, to 2^-19 (P8X_F32 queries: 2^-22) of the largest weight in its 32
- * slots where that is more, however far those are below others. A value that is infinite or NaN makes the elements of
- * the tokens that see it infinite or NaN.
+ * slots where that is more, however far those are below others. An infinite or NaN key or value reaches the tokens that see it
+ * as infinities or NaN, also where the formula would give an infinity (values) or a weight of 0 (keys). out overlaps no input.
  * workspace: device memory that splits a sequence over workgroups (NULL or too little: fewer of them), zeroed
  * once by the caller before its first use and left zeroed where it has to be, for calls of any shape in turn; calls that
  * may overlap need one each.
