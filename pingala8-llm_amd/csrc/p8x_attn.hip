@@ -271,14 +271,14 @@ struct Wave {
         }
         bool move = __any(far);
         uint64_t down = 0;
-        if (!BF && move) {   // up where one of a row's lanes is, down where all four are
+        if (!BF && move) {   // up where one of a row's lanes is, down where all four are (or see nothing, but one does)
             uint64_t up = 0;
 #pragma unroll
             for (int a = 0; a < NT; ++a) {
                 const float d = fmaf(mx[a], c2[a], -m[a]);
-                const uint64_t low = __ballot(d < -kDown && d > -INFINITY), two = low & low >> 32;
+                const uint64_t low = __ballot(d < -kDown), two = low & low >> 32, some = __ballot(d > -INFINITY), of2 = some | some >> 32;
                 up |= __ballot(d > kUp);
-                down |= two & two >> 16 & 0xFFFF;
+                down |= two & two >> 16 & (of2 | of2 >> 16) & 0xFFFF;
             }
             move = up | down;
         }

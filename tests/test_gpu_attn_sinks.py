@@ -15,11 +15,11 @@ from test_gpu_attn import run_attn
 pytestmark = pytest.mark.gpu
 
 
-def levels_case(level, value, toks, heads, kv, D, cache, q, seed, spread=0.0):
+def levels_case(level, value, toks, heads, kv, D, cache, q, seed, spread=0.0, page=64):
     """level [n]: how far a slot's score is above the drafted tokens' (spread: plus a normal of that size), value [n]: of what size
     its value is. A drafted token's value is that of the last slot."""
     n = len(level)
-    c = Case([n], [toks], heads=heads, kv=kv, D=D, cache=cache, q=q, fused=False, seed=seed, page=64, mask="chain")
+    c = Case([n], [toks], heads=heads, kv=kv, D=D, cache=cache, q=q, fused=False, seed=seed, page=page, mask="chain")
     rng = np.random.default_rng(seed)
     qv = 0.05 * rng.standard_normal((c.n, heads, D))
     qv[:, :, 0], qv[:, :, 1] = 8.0, 1.0
