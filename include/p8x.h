@@ -269,9 +269,10 @@ typedef struct p8x_batch_info { int njobs, ncols, class_set, units, split_jobs, 
 int p8x_gemv_batch_info(const p8x_gemv_batch *b, p8x_batch_info *out);
 
 /* ---- between the linears: norms, cache, attention of drafted tokens ---------------------------------------- */
-/* No counterpart in the reference (ggml's own kernels run there): norms with residual, the cache and its attention for a
- * decode step over drafted tokens, beside p8x_mul_mat_vec and p8x_mul_mat, for hosts that have no other kernels for them (not
- * here: rotary embedding, norms of single heads in a q, k, v row). All calls are asynchronous on the
+/* No counterpart in the reference (ggml's own kernels run there): norms with residual, rotary positions, the cache and its
+ * attention for prompts and for a decode step over drafted tokens, beside p8x_mul_mat_vec and p8x_mul_mat, for hosts that have
+ * no other kernels for them. A prompt: p8x_mul_mat (q, k, v), p8x_kv_append_rope, p8x_attn_prompt, p8x_mul_mat (o). A tree of drafts:
+ * p8x_mul_mat_vec, p8x_rope in place, p8x_attn_tree, then p8x_kv_score and p8x_kv_append of the rotated keys. All calls are asynchronous on the
  * stream, allocate nothing, record kernel launches only and are deterministic; they keep nothing between calls. The
  * structs are read during the call, what they point to is device memory. Fields left 0 / NULL take the stated default. */
 enum { P8X_NORM_NONE = 0, P8X_NORM_RMS = 1, P8X_NORM_LAYER = 2 };
@@ -372,6 +373,66 @@ typedef struct p8x_evict_args {
 } p8x_evict_args;
 int p8x_kv_evict(const p8x_kv_cache *c, const p8x_evict_args *a, void *stream);
 size_t p8x_kv_evict_workspace(const p8x_kv_cache *c, int budget);
+
+/* Rotary positions. A head x of a token at position p becomes
+ *   v = x, or x / sqrt(mean(x^2) + eps) w of the whole head (w_q, w_k [head_dim]; NULL: no norm), then
+ *   y_a = amplitude (v_a cos t - v_b sin t), y_b = amplitude (v_b cos t + v_a sin t), t = 2 pi p freq[i] / 2^64
+ * for the pairs i < n_rot / 2, (a, b) = (i, i + n_rot / 2) (P8X_ROPE_HALF) or (2 i, 2 i + 1) (P8X_ROPE_PAIRS); elements from n_rot on
+ * pass as v. freq holds turns a position as fractions of 2^64, so that the angle of any int32 position is exact to 2^-32 of a
+ * turn. Sums and products in f32. */
+enum { P8X_ROPE_HALF = 0, P8X_ROPE_PAIRS = 1 };
+typedef struct p8x_rotation {
+    int layout, n_rot;              /* n_rot a multiple of 8, 0 .. head_dim */
+    const uint64_t *freq;           /* [n_rot / 2] on the device, 16-byte aligned (p8x_rope_frequencies) */
+    float amplitude;                /* no default: 0 makes zeros */
+    const float *w_q, *w_k; float eps;   /* w 16-byte aligned */
+} p8x_rotation;
+
+/* Host: freq[i] of theta_i = base^(-2 i / n_rot) (/ factors[i], where given) radians a position, scaled for contexts beyond the
+ * `original` length: P8X_ROPE_LINEAR theta / factor; P8X_ROPE_BANDS theta / factor where the pair makes fewer than `low` turns in
+ * `original` positions, theta where more than `high`, linear in the turns between; P8X_ROPE_YARN theta / factor from the pair that
+ * makes `low` turns on, theta up to the one that makes `high`, linear in the pair's index between (both rounded outwards), and
+ * amplitude 0.1 ln(factor) + 1 (for factor > 1; else, and for the other kinds, 1). amplitude may be NULL. */
+enum { P8X_ROPE_PLAIN = 0, P8X_ROPE_LINEAR = 1, P8X_ROPE_BANDS = 2, P8X_ROPE_YARN = 3 };
+typedef struct p8x_rope_scaling {
+    int kind;
+    double base, factor, original, low, high;   /* base > 0 (for P8X_ROPE_YARN > 1); factor > 0 but for P8X_ROPE_PLAIN; BANDS, YARN: original > 0, 0 < low < high */
+    const double *factors;          /* host, [n_rot / 2], > 0; NULL: 1 */
+} p8x_rope_scaling;
+int p8x_rope_frequencies(const p8x_rope_scaling *s, int n_rot, uint64_t *freq, float *amplitude);
+
+/* n heads of token rows, rows ld elements and heads head_stride (0: head_dim) apart, P8X_F32 | P8X_F16 | P8X_BF16, to rows of any
+ * of these types. 16-byte aligned, strides multiples of 8 (4 for P8X_F32). out may be x with the same type and strides;
+ * else it overlaps no input. */
+typedef struct p8x_heads {
+    int n;
+    const void *x; int dtype; size_t ld, head_stride;
+    void *out; int out_dtype; size_t ld_out, head_stride_out;
+} p8x_heads;
+/* The rotation of n_tokens rows of queries and keys (either NULL: none; w_q and w_k of r are theirs) at positions pos[token].
+ * head_dim a multiple of 8, 8 .. 256. */
+int p8x_rope(const p8x_rotation *r, int n_tokens, int head_dim, const int32_t *pos, const p8x_heads *q, const p8x_heads *k, void *stream);
+
+/* p8x_kv_append of all tokens (the fields of d that it reads, any number of tokens) with their keys rotated on the way, and
+ * their queries q (NULL: none) rotated to q->out: one pass over the products of a layer. Positions are at[token] (NULL: the slot that the
+ * token takes), and are stored to pos (NULL: not stored). Tokens past max_len are dropped (their queries are rotated). Rows of q->out of no sequence
+ * are left as they are. */
+int p8x_kv_append_rope(const p8x_kv_cache *c, const p8x_drafts *d, const p8x_rotation *r, const int32_t *at, const p8x_heads *q, int32_t *pos,
+                       int32_t *len_out, void *stream);
+
+/* Causal attention of new tokens that are in the cache already (p8x_kv_append_rope, p8x_kv_append; c->len counts them): of the nt
+ * tokens of a sequence of n slots, token i sees slots 0 .. n - nt + i. out = softmax(scale q k) v, lse [n_tokens][n_heads] = log of the
+ * sum of exp (NULL: not stored). Any number of tokens a sequence; of d first, n_tokens, max_tokens, q and scale are read, mask is
+ * NULL. P8X_F32 queries are multiplied and weighed in f32 accuracy (as sums of 16-bit parts), to out of any type; 16-bit ones as they are, with
+ * weights rounded to the cache's type, to out of either 16-bit type. Sums are f32. A token that sees no slot (no page, a length below nt), or only scores
+ * of -inf, gets 0 and lse -inf; what a token does not see does not reach it, be it infinite or NaN; what it sees of them reaches it as infinities or NaN.
+ * A weight is held to half a step of its type, or on a P8X_F16 cache to 2^-17 (P8X_F32 queries: 2^-22) of the largest weight of its row
+ * in 64 slots where that is more. out overlaps no input; rows of no sequence are left as they are.
+ * workspace: device memory, any contents, 16-byte aligned, that splits long contexts of few tokens over workgroups (NULL or too little: fewer
+ * of them, or none); calls that may overlap need one each. p8x_attn_prompt_workspace: bytes beyond which more do not help. */
+int p8x_attn_prompt(const p8x_kv_cache *c, const p8x_drafts *d, void *out, int out_dtype, size_t ld_out, size_t head_stride_out, float *lse,
+                    void *workspace, size_t workspace_bytes, void *stream);
+size_t p8x_attn_prompt_workspace(const p8x_kv_cache *c, const p8x_drafts *d);
 
 /* ---- native model files (GGUF): slot bytes for p8x_prepare ----------------------------------------------- */
 /* The host side of the reference's model loader for VR tensors (llama_model_loader::vr_native_init and

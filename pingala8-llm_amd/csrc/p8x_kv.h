@@ -22,7 +22,20 @@ struct DraftDev {
     float scale;
 };
 
-// launchers (p8x_norm.hip, p8x_attn.hip, p8x_kv.hip); arguments checked by p8x_kv_host.cpp
+// head rows in and out, and what turns them (p8x_heads, p8x_rotation after the host's checks)
+struct HeadsDev {
+    const void *x; size_t ld, hs;
+    void *out; size_t ldo, hso;
+    int n, dtype, out_dtype;
+};
+struct TurnDev {
+    const uint64_t *freq;
+    const float *w_q, *w_k;
+    float amp, eps;
+    int pairs, n_rot;
+};
+
+// launchers (p8x_norm.hip, p8x_attn.hip, p8x_kv.hip, p8x_rope.hip, p8x_prompt.hip); arguments checked by p8x_kv_host.cpp
 int launch_norm_residual(const p8x_norm_args &a, hipStream_t st);
 int launch_attn_tree(const KvDev &c, const DraftDev &d, int head_dim, void *out, size_t ldo, size_t hso, float *lse, void *ws, size_t ws_bytes,
                      hipStream_t st);
@@ -31,6 +44,13 @@ int launch_kv_score(const KvDev &c, const DraftDev &d, int head_dim, const uint6
                     float *score_out, hipStream_t st);
 int launch_kv_append(const KvDev &c, const DraftDev &d, int head_dim, const uint64_t *accept, const int32_t *at, int32_t *pos, int32_t *len_out,
                      hipStream_t st);
+int launch_append_len(const KvDev &c, const DraftDev &d, const uint64_t *accept, int32_t *len_out, hipStream_t st);
+int launch_rope(const TurnDev &r, int n_tokens, int head_dim, const int32_t *pos, const HeadsDev &q, const HeadsDev &k, hipStream_t st);
+int launch_kv_append_rope(const KvDev &c, const DraftDev &d, int head_dim, const TurnDev &r, const int32_t *at, const HeadsDev &q, int kv_dtype,
+                          int32_t *pos, int32_t *len_out, hipStream_t st);
+int launch_attn_prompt(const KvDev &c, const DraftDev &d, int head_dim, void *out, int out_dtype, size_t ldo, size_t hso, float *lse, void *ws,
+                       size_t ws_bytes, hipStream_t st);
+size_t attn_prompt_workspace(const KvDev &c, const DraftDev &d, int head_dim);
 int launch_kv_evict(const KvDev &c, int head_dim, const p8x_evict_args &a, hipStream_t st);
 size_t kv_evict_workspace(const KvDev &c, int budget);
 

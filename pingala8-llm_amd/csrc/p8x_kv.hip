@@ -78,8 +78,13 @@ int launch_kv_append(const KvDev &c, const DraftDev &d, int D, const uint64_t *a
     const int64_t pieces = (int64_t)(D / 8) * 2 * c.n_kv * d.max_tokens;
     const int nb = (int)std::max<int64_t>(1, std::min<int64_t>((pieces + 1023) / 1024, 1024));
     if (d.n_tokens && d.max_tokens) k_append<<<dim3(nb, c.n_seq), 1024, 0, st>>>(c, d, D, accept, at, pos, in_place && nb > 1 ? nullptr : len_out);
-    if (len_out && ((in_place && nb > 1) || !(d.n_tokens && d.max_tokens))) k_append_len<<<(c.n_seq + 63) / 64, 64, 0, st>>>(c, d, accept, len_out);
+    if (len_out && ((in_place && nb > 1) || !(d.n_tokens && d.max_tokens))) return launch_append_len(c, d, accept, len_out, st);
     return hip_check(hipGetLastError(), "p8x_kv_append launch");
+}
+
+int launch_append_len(const KvDev &c, const DraftDev &d, const uint64_t *accept, int32_t *len_out, hipStream_t st) {
+    k_append_len<<<(c.n_seq + 63) / 64, 64, 0, st>>>(c, d, accept, len_out);
+    return hip_check(hipGetLastError(), "append length launch");
 }
 
 // ---- evict ------------------------------------------------------------------------------------------------

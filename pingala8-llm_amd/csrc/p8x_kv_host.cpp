@@ -2,6 +2,8 @@
 // checks, and the structs of p8x.h as kernel arguments.
 #include <hip/hip_runtime.h>
 
+#include <cmath>
+
 #include "p8x_kv.h"
 
 namespace p8x {
@@ -65,6 +67,35 @@ int check_drafts(const char *fn, const p8x_kv_cache *c, const p8x_drafts *d, boo
         if (!(d->scale - d->scale == 0.0f)) return set_error(P8X_ERR_ARG, "%s: scale is not finite", fn);
         o.G = d->n_heads / c->n_kv;
     }
+    return P8X_OK;
+}
+
+// the rotation of heads of D elements
+int check_rotation(const char *fn, const p8x_rotation *r, int D, TurnDev &o) {
+    if (!r) return set_error(P8X_ERR_ARG, "%s: null rotation", fn);
+    if (r->layout != P8X_ROPE_HALF && r->layout != P8X_ROPE_PAIRS) return set_error(P8X_ERR_ARG, "%s: layout %d", fn, r->layout);
+    if (r->n_rot < 0 || r->n_rot > D) return set_error(P8X_ERR_ARG, "%s: n_rot %d of head_dim %d", fn, r->n_rot, D);
+    if (r->n_rot % 8) return set_error(P8X_ERR_UNSUPPORTED, "%s: n_rot %d (a multiple of 8)", fn, r->n_rot);
+    if (r->n_rot && !r->freq) return set_error(P8X_ERR_ARG, "%s: null freq", fn);
+    if (!aligned(r->freq, 16) || !aligned(r->w_q, 16) || !aligned(r->w_k, 16)) return set_error(P8X_ERR_ARG, "%s: freq, w_q and w_k 16-byte aligned", fn);
+    if (!(r->amplitude - r->amplitude == 0.0f)) return set_error(P8X_ERR_ARG, "%s: amplitude is not finite", fn);
+    o = {r->freq, r->w_q, r->w_k, r->amplitude, r->eps, r->layout == P8X_ROPE_PAIRS, r->n_rot};
+    return P8X_OK;
+}
+
+// head rows in and out; null: none
+int check_heads(const char *fn, const p8x_heads *h, int D, HeadsDev &o) {
+    o = {};
+    if (!h || h->n == 0) return P8X_OK;
+    if (h->n < 0) return set_error(P8X_ERR_ARG, "%s: %d heads", fn, h->n);
+    if (h->n > 65535) return set_error(P8X_ERR_UNSUPPORTED, "%s: %d heads (at most 65535)", fn, h->n);
+    if (!h->x || !h->out) return set_error(P8X_ERR_ARG, "%s: null heads x or out", fn);
+    if (!is_float(h->dtype) || !is_float(h->out_dtype)) return set_error(P8X_ERR_ARG, "%s: heads dtypes %d %d", fn, h->dtype, h->out_dtype);
+    o = {h->x, h->ld, h->head_stride ? h->head_stride : (size_t)D, h->out, h->ld_out, h->head_stride_out ? h->head_stride_out : (size_t)D, h->n, h->dtype, h->out_dtype};
+    if (!rows_ok(o.x, o.dtype, o.ld, o.hs, o.n, D) || !rows_ok(o.out, o.out_dtype, o.ldo, o.hso, o.n, D))
+        return set_error(P8X_ERR_ARG, "%s: heads' rows 16-byte aligned, strides %zu %zu to %zu %zu", fn, o.ld, o.hs, o.ldo, o.hso);
+    if (o.x == o.out && (o.dtype != o.out_dtype || o.ld != o.ldo || o.hs != o.hso))
+        return set_error(P8X_ERR_ARG, "%s: heads in place with another type or strides", fn);
     return P8X_OK;
 }
 
@@ -146,6 +177,103 @@ int p8x_kv_append(const p8x_kv_cache *c, const p8x_drafts *d, const uint64_t *ac
     if (!rc) rc = check_drafts(fn, c, d, true, true, false, accept ? P8X_MAX_DRAFT : 0, q);
     if (rc) return rc;
     return launch_kv_append(k, q, c->head_dim, accept, at, pos, len_out, (hipStream_t)stream);
+}
+
+int p8x_rope_frequencies(const p8x_rope_scaling *s, int n_rot, uint64_t *freq, float *amplitude) {
+    const char *fn = "p8x_rope_frequencies";
+    if (!s || (n_rot && !freq)) return set_error(P8X_ERR_ARG, "%s: null arguments", fn);
+    if (n_rot < 0 || n_rot % 2) return set_error(P8X_ERR_ARG, "%s: n_rot %d", fn, n_rot);
+    auto positive = [](double v) { return v > 0 && v - v == 0; };
+    const bool ends = s->kind == P8X_ROPE_BANDS || s->kind == P8X_ROPE_YARN;
+    if (s->kind < P8X_ROPE_PLAIN || s->kind > P8X_ROPE_YARN || !positive(s->base) || (s->kind == P8X_ROPE_YARN && s->base <= 1) ||
+        (s->kind != P8X_ROPE_PLAIN && !positive(s->factor)) || (ends && (!positive(s->original) || !positive(s->low) || !positive(s->high) || s->low >= s->high)))
+        return set_error(P8X_ERR_ARG, "%s: kind %d base %g factor %g original %g low %g high %g", fn, s->kind, s->base, s->factor, s->original, s->low, s->high);
+    const double pi2 = 6.283185307179586476925;
+    // the (fractional) pair that makes so many turns in the original length: original theta_i = 2 pi turns
+    auto pair_of = [&](double turns) { return n_rot * std::log(s->original / (turns * pi2)) / (2 * std::log(s->base)); };
+    double lo = 0, hi = 0;
+    if (s->kind == P8X_ROPE_YARN) {
+        lo = std::fmax(0.0, std::floor(pair_of(s->high)));
+        hi = std::fmin(n_rot - 1.0, std::ceil(pair_of(s->low)));
+    }
+    for (int i = 0; i < n_rot / 2; ++i) {
+        double th = std::pow(s->base, -2.0 * i / n_rot);
+        if (s->factors) {
+            if (!positive(s->factors[i])) return set_error(P8X_ERR_ARG, "%s: factors[%d] %g", fn, i, s->factors[i]);
+            th /= s->factors[i];
+        }
+        double far = 0;   // how much of the pair is divided by the factor
+        if (s->kind == P8X_ROPE_LINEAR) far = 1;
+        else if (s->kind == P8X_ROPE_BANDS) far = (s->high - s->original * th / pi2) / (s->high - s->low);
+        else if (s->kind == P8X_ROPE_YARN) far = (i - lo) / std::fmax(hi - lo, 0.001);
+        far = std::fmin(1.0, std::fmax(0.0, far));
+        if (far > 0) th = far * (th / s->factor) + (1 - far) * th;
+        const double turns = th / pi2, part = turns - std::floor(turns);   // whole turns do nothing
+        if (!(turns - turns == 0)) return set_error(P8X_ERR_ARG, "%s: pair %d turns %g a position", fn, i, turns);
+        const double scaled = std::nearbyint(std::ldexp(part, 64));
+        freq[i] = scaled >= 18446744073709551616.0 ? 0 : (uint64_t)scaled;
+    }
+    if (amplitude) *amplitude = s->kind == P8X_ROPE_YARN && s->factor > 1 ? (float)(0.1 * std::log(s->factor) + 1) : 1.0f;
+    return P8X_OK;
+}
+
+int p8x_rope(const p8x_rotation *r, int n_tokens, int head_dim, const int32_t *pos, const p8x_heads *q, const p8x_heads *k, void *stream) {
+    const char *fn = "p8x_rope";
+    TurnDev t;
+    HeadsDev hq, hk;
+    if (n_tokens < 0) return set_error(P8X_ERR_ARG, "%s: n_tokens %d", fn, n_tokens);
+    if (head_dim < 8 || head_dim > 256 || head_dim % 8) return set_error(P8X_ERR_UNSUPPORTED, "%s: head_dim %d (a multiple of 8, 8 .. 256)", fn, head_dim);
+    int rc = check_rotation(fn, r, head_dim, t);
+    if (!rc) rc = check_heads(fn, q, head_dim, hq);
+    if (!rc) rc = check_heads(fn, k, head_dim, hk);
+    if (rc) return rc;
+    if (!hq.n && !hk.n) return set_error(P8X_ERR_ARG, "%s: neither q nor k", fn);
+    if (n_tokens == 0) return P8X_OK;
+    if (!pos) return set_error(P8X_ERR_ARG, "%s: null pos", fn);
+    return launch_rope(t, n_tokens, head_dim, pos, hq, hk, (hipStream_t)stream);
+}
+
+int p8x_kv_append_rope(const p8x_kv_cache *c, const p8x_drafts *d, const p8x_rotation *r, const int32_t *at, const p8x_heads *q, int32_t *pos,
+                       int32_t *len_out, void *stream) {
+    const char *fn = "p8x_kv_append_rope";
+    KvDev k;
+    DraftDev t;
+    TurnDev turn;
+    HeadsDev h;
+    int rc = check_cache(fn, c, k);
+    if (!rc) rc = check_drafts(fn, c, d, true, true, false, 0, t);
+    if (!rc) rc = check_rotation(fn, r, c->head_dim, turn);
+    if (!rc) rc = check_heads(fn, q, c->head_dim, h);
+    if (rc) return rc;
+    return launch_kv_append_rope(k, t, c->head_dim, turn, at, h, d->kv_dtype, pos, len_out, (hipStream_t)stream);
+}
+
+int p8x_attn_prompt(const p8x_kv_cache *c, const p8x_drafts *d, void *out, int out_dtype, size_t ld_out, size_t head_stride_out, float *lse,
+                    void *workspace, size_t workspace_bytes, void *stream) {
+    const char *fn = "p8x_attn_prompt";
+    KvDev k;
+    DraftDev q;
+    int rc = check_cache(fn, c, k);
+    if (!rc) rc = check_drafts(fn, c, d, false, false, true, 0, q);
+    if (rc) return rc;
+    if (d->mask) return set_error(P8X_ERR_ARG, "%s: a mask (its tokens see all before them)", fn);
+    if (!is_float(out_dtype)) return set_error(P8X_ERR_ARG, "%s: out dtype %d", fn, out_dtype);
+    if (!d->n_tokens || !d->max_tokens) return P8X_OK;
+    if (out_dtype == P8X_F32 && d->q_dtype != P8X_F32) return set_error(P8X_ERR_UNSUPPORTED, "%s: f32 out of 16-bit queries", fn);
+    const size_t hs = head_stride_out ? head_stride_out : (size_t)c->head_dim;
+    if (!out || !rows_ok(out, out_dtype, ld_out, hs, d->n_heads, c->head_dim))
+        return set_error(P8X_ERR_ARG, "%s: out rows 16-byte aligned, strides %zu %zu", fn, ld_out, hs);
+    if (workspace && !aligned(workspace, 16)) return set_error(P8X_ERR_ARG, "%s: workspace 16-byte aligned", fn);
+    return launch_attn_prompt(k, q, c->head_dim, out, out_dtype, ld_out, hs, lse, workspace, workspace ? workspace_bytes : 0, (hipStream_t)stream);
+}
+
+size_t p8x_attn_prompt_workspace(const p8x_kv_cache *c, const p8x_drafts *d) {
+    KvDev k;
+    DraftDev q;
+    if (check_cache("p8x_attn_prompt_workspace", c, k) || check_drafts("p8x_attn_prompt_workspace", c, d, false, false, false, 0, q)) return 0;
+    if (d->n_heads < 1 || d->n_heads % c->n_kv || !d->n_tokens || !d->max_tokens) return 0;
+    q.G = d->n_heads / c->n_kv;
+    return attn_prompt_workspace(k, q, c->head_dim);
 }
 
 size_t p8x_kv_evict_workspace(const p8x_kv_cache *c, int budget) {

@@ -19,6 +19,8 @@ ACT_Q8_128, ACT_Q8_1, ACT_X16 = 0, 1, 2
 MM_NONE, MM_ROW_GROUP, MM_FUSED, MM_DECODED = 0, 1, 2, 3   # kernels of a prompt GEMM (mul_mat_plan)
 NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2
 GATE_LINEAR, GATE_SIGMOID = 0, 1
+ROPE_HALF, ROPE_PAIRS = 0, 1
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BANDS, ROPE_YARN = 0, 1, 2, 3
 MAX_DRAFT = 64   # drafted tokens of a sequence
 GEMV_KERNEL_AUTO, GEMV_KERNEL_DOT4, GEMV_KERNEL_MFMA = 0, 1, 2   # p8x_gemv_batch_create_ex
 MAX_COLS = 8
@@ -37,7 +39,7 @@ EXPORTS = [
     "p8x_dequantize_rows", "p8x_vec_dot_rows", "p8x_encode_defaults", "p8x_encode_tensor", "p8x_encode_free",
     "p8x_encode_factor", "p8x_encode_alloc", "p8x_step_create", "p8x_step_create_act", "p8x_step_run", "p8x_step_check", "p8x_step_info",
     "p8x_step_release", "p8x_norm_residual", "p8x_attn_tree", "p8x_attn_workspace", "p8x_kv_score", "p8x_kv_append", "p8x_kv_evict",
-    "p8x_kv_evict_workspace",
+    "p8x_kv_evict_workspace", "p8x_rope_frequencies", "p8x_rope", "p8x_kv_append_rope", "p8x_attn_prompt", "p8x_attn_prompt_workspace",
 ]
 
 
@@ -118,6 +120,20 @@ class EvictArgs(ctypes.Structure):
                 ("len_out", ctypes.c_void_p), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)]
 
 
+class RotationC(ctypes.Structure):
+    _fields_ = [("layout", ctypes.c_int), ("n_rot", ctypes.c_int), ("freq", ctypes.c_void_p), ("amplitude", ctypes.c_float),
+                ("w_q", ctypes.c_void_p), ("w_k", ctypes.c_void_p), ("eps", ctypes.c_float)]
+
+
+class RopeScaling(ctypes.Structure):
+    _fields_ = [("kind", ctypes.c_int)] + [(f, ctypes.c_double) for f in ("base", "factor", "original", "low", "high")] + [("factors", ctypes.c_void_p)]
+
+
+class HeadsC(ctypes.Structure):
+    _fields_ = [("n", ctypes.c_int), ("x", ctypes.c_void_p), ("dtype", ctypes.c_int), ("ld", ctypes.c_size_t), ("head_stride", ctypes.c_size_t),
+                ("out", ctypes.c_void_p), ("out_dtype", ctypes.c_int), ("ld_out", ctypes.c_size_t), ("head_stride_out", ctypes.c_size_t)]
+
+
 _lib = None
 
 
@@ -195,6 +211,12 @@ def lib():
     L.p8x_attn_workspace.argtypes = [cache, drafts]; L.p8x_attn_workspace.restype = sz
     L.p8x_kv_score.argtypes = [cache, drafts, vp, vp, f, vp, vp, vp]
     L.p8x_kv_append.argtypes = [cache, drafts, vp, vp, vp, vp, vp]
+    turn, heads = ctypes.POINTER(RotationC), ctypes.POINTER(HeadsC)
+    L.p8x_rope_frequencies.argtypes = [ctypes.POINTER(RopeScaling), i, vp, ctypes.POINTER(f)]
+    L.p8x_rope.argtypes = [turn, i, i, vp, heads, heads, vp]
+    L.p8x_kv_append_rope.argtypes = [cache, drafts, turn, vp, heads, vp, vp, vp]
+    L.p8x_attn_prompt.argtypes = [cache, drafts, vp, i, sz, sz, vp, vp, sz, vp]
+    L.p8x_attn_prompt_workspace.argtypes = [cache, drafts]; L.p8x_attn_prompt_workspace.restype = sz
     L.p8x_kv_evict.argtypes = [cache, ctypes.POINTER(EvictArgs), vp]
     L.p8x_kv_evict_workspace.argtypes = [cache, i]; L.p8x_kv_evict_workspace.restype = sz
     _lib = L
@@ -1032,3 +1054,71 @@ class KvEvict(_Call):
         a = EvictArgs(budget, n_sink, n_recent, _address(score), _address(score if score_out is None else score_out), _address(pos),
                       _address(pos if pos_out is None else pos_out), _address(len_out), _address(workspace), workspace_bytes)
         super().__init__("p8x_kv_evict", (ctypes.byref(cache.c), ctypes.byref(a)), (cache, a, score, score_out, pos, pos_out, len_out, workspace))
+
+
+def rope_frequencies(n_rot, base=10000.0, kind=ROPE_PLAIN, factor=1.0, original=0.0, low=1.0, high=32.0, factors=None):
+    """(frequencies of a Rotation, uint64 [n_rot / 2], to be brought to the device; its amplitude) (p8x_rope_frequencies)"""
+    freq, amplitude = np.zeros(max(0, n_rot // 2), np.uint64), ctypes.c_float()
+    if factors is not None:
+        factors = np.ascontiguousarray(factors, np.float64)
+        if factors.shape != (n_rot // 2,):
+            raise P8xError(f"p8x_rope_frequencies: {factors.shape} factors of {n_rot // 2} pairs")
+    s = RopeScaling(kind, base, factor, original, low, high, None if factors is None else factors.ctypes.data)
+    check(lib().p8x_rope_frequencies(ctypes.byref(s), n_rot, freq.ctypes.data, ctypes.byref(amplitude)), "p8x_rope_frequencies")
+    return freq, amplitude.value
+
+
+class Rotation:
+    """How heads turn with their positions, and their norms before (p8x_rotation)."""
+
+    def __init__(self, n_rot, freq, layout=ROPE_HALF, amplitude=1.0, w_q=None, w_k=None, eps=1e-6):
+        self.c = RotationC(layout, n_rot, _address(freq), amplitude, _address(w_q), _address(w_k), eps)
+        self._keep = (freq, w_q, w_k)
+
+
+def _heads(D, n, x, dtype, ld, head_stride, out, out_dtype, ld_out, head_stride_out):
+    """p8x_heads; out None: in place"""
+    ld = n * D if ld is None else ld
+    if out is None:
+        out, out_dtype, ld_out, head_stride_out = x, dtype, ld, head_stride
+    return HeadsC(n, _address(x), dtype, ld, head_stride, _address(out), out_dtype, n * D if ld_out is None else ld_out, head_stride_out)
+
+
+class Rope(_Call):
+    """Queries and keys of n tokens normed and rotated (p8x_rope), in place where no q_out, k_out is given."""
+
+    def __init__(self, rotation, n, head_dim, pos, n_heads=0, q=None, q_dtype=F32, ld_q=None, head_stride_q=0, q_out=None, q_out_dtype=F32, ld_q_out=None,
+                 head_stride_q_out=0, n_kv=0, k=None, k_dtype=F32, ld_k=None, head_stride_k=0, k_out=None, k_out_dtype=F32, ld_k_out=None,
+                 head_stride_k_out=0):
+        hq = _heads(head_dim, n_heads, q, q_dtype, ld_q, head_stride_q, q_out, q_out_dtype, ld_q_out, head_stride_q_out)
+        hk = _heads(head_dim, n_kv, k, k_dtype, ld_k, head_stride_k, k_out, k_out_dtype, ld_k_out, head_stride_k_out)
+        super().__init__("p8x_rope", (ctypes.byref(rotation.c), n, head_dim, _address(pos), ctypes.byref(hq), ctypes.byref(hk)),
+                         (rotation, pos, hq, hk, q, q_out, k, k_out))
+
+
+class KvAppendRope(_Call):
+    """All tokens' keys, normed and rotated, and values into the cache, their queries rotated to q_out (p8x_kv_append_rope; without
+    n_heads no queries, without q_out in place); drafts: the fields of p8x_drafts by name."""
+
+    def __init__(self, cache, rotation, at=None, pos=None, len_out=None, n_heads=0, q=None, q_dtype=F32, ld_q=None, head_stride_q=0, q_out=None,
+                 q_out_dtype=F32, ld_q_out=None, head_stride_q_out=0, **drafts):
+        d = _drafts(cache, **drafts)
+        hq = _heads(cache.head_dim, n_heads, q, q_dtype, ld_q, head_stride_q, q_out, q_out_dtype, ld_q_out, head_stride_q_out)
+        super().__init__("p8x_kv_append_rope", (ctypes.byref(cache.c), ctypes.byref(d), ctypes.byref(rotation.c), _address(at), ctypes.byref(hq), _address(pos),
+                                                _address(len_out)), (cache, d, drafts, rotation, at, hq, q, q_out, pos, len_out))
+
+
+class AttnPrompt(_Call):
+    """Causal attention of new tokens that are in the cache already (p8x_attn_prompt); drafts: the fields of p8x_drafts by name.
+    Without a workspace of the caller's it keeps one of its own."""
+
+    def __init__(self, cache, out, out_dtype=None, lse=None, ld_out=None, head_stride_out=0, workspace=None, workspace_bytes=None, **drafts):
+        d = _drafts(cache, **drafts)
+        if workspace is None:
+            workspace_bytes = lib().p8x_attn_prompt_workspace(ctypes.byref(cache.c), ctypes.byref(d))
+            if workspace_bytes:
+                workspace = DeviceBuffer(workspace_bytes)
+        workspace_bytes = _workspace_bytes("p8x_attn_prompt", workspace, workspace_bytes)
+        super().__init__("p8x_attn_prompt", (ctypes.byref(cache.c), ctypes.byref(d), _address(out), d.q_dtype if out_dtype is None else out_dtype,
+                                             d.n_heads * cache.head_dim if ld_out is None else ld_out, head_stride_out, _address(lse), _address(workspace),
+                                             workspace_bytes), (cache, d, drafts, out, lse, workspace))
