@@ -1,4 +1,4 @@
-// p8x_attn.h -- operands of the matrix-core products with queries and cached keys (p8x_attn.hip, p8x_score.hip).
+// p8x_attn.h -- operands of the matrix-core products with queries and cached keys (p8x_attn.hip, p8x_score.hip, p8x_prompt.hip).
 #pragma once
 #include "p8x_kv.h"
 
@@ -79,6 +79,23 @@ __device__ __forceinline__ float load_split(const float *q, bool on, float f, fl
         f = ldexpf(f, -ex);
     }
     return f;
+}
+
+// Whether a dword holds a 16-bit infinity or NaN, and the dword without them.
+template <bool BF>
+__device__ __forceinline__ bool take_odd(uint32_t &w) {
+    constexpr uint32_t inf = BF ? 0x7F80u : 0x7C00u;
+    const bool lo = (w & inf) == inf, hi = (w >> 16 & inf) == inf;
+    w &= (lo ? 0 : 0xFFFFu) | (hi ? 0 : 0xFFFF0000u);
+    return lo || hi;
+}
+
+// 16 bytes a lane from base + off to LDS at `to` + 16 lane, without a wait. Written by hand: the compiler, which knows no other
+// wait than for all of these, would put one before every read of LDS. M0 holds `to` while the load is issued; five wait
+// states lie between it, or a VALU write of the base, and the load. Nothing is loaded into registers.
+__device__ __forceinline__ void load_lds(const uint16_t *base, uint32_t off, uint32_t to) {
+    uint32_t m0;
+    __asm__ volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0" : "=&s"(m0) : "v"(off), "s"(base), "s"(to) : "memory");
 }
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;

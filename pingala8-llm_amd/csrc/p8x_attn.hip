@@ -390,15 +390,6 @@ struct Wave {
     }
 };
 
-// Whether a dword holds a 16-bit infinity or NaN, and the dword without them.
-template <bool BF>
-__device__ __forceinline__ bool take_odd(uint32_t &w) {
-    constexpr uint32_t inf = BF ? 0x7F80u : 0x7C00u;
-    const bool lo = (w & inf) == inf, hi = (w >> 16 & inf) == inf;
-    w &= (lo ? 0 : 0xFFFFu) | (hi ? 0 : 0xFFFF0000u);
-    return lo || hi;
-}
-
 // which of the drafted tokens j0 .. j0 + 31 the lane's rows see
 template <int NT>
 __device__ __forceinline__ void draft_mask(const DraftDev &d, const Seq &q, int j0, int row0, int rows, int ln, uint32_t (&see)[NT]) {
@@ -490,14 +481,6 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnJob J, int rows_wg) {
         for (int k = 1; k < SUB; ++k) add_part(p, sh[k][threadIdx.x % PIECES]);
     }
     if (on) store_row<D, BF, QF>(J, q.first, h, rt * rows_wg + r, e, p);
-}
-
-// 16 bytes a lane from base + off to LDS at `to` + 16 lane, without a wait. Written by hand: the compiler, which knows no other
-// wait than for all of these, would put one before every read of LDS. M0 holds `to` while the load is issued; five wait
-// states lie between it, or a VALU write of the base, and the load. Nothing is loaded into registers.
-__device__ __forceinline__ void load_lds(const uint16_t *base, uint32_t off, uint32_t to) {
-    uint32_t m0;
-    __asm__ volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0" : "=&s"(m0) : "v"(off), "s"(base), "s"(to) : "memory");
 }
 
 // SHARE: the waves' rows are many; each tile of K and V is brought to LDS once for all of them, three stages of tiles

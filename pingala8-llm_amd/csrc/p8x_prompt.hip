@@ -1,4 +1,19 @@
 // p8x_prompt.hip -- causal attention of new tokens over the cache that holds them (p8x_attn_prompt).
+//
+// Rows: the (token, head of the group) pairs of a sequence and key/value head, token-major, so that the rows of a workgroup
+// end at about the same slot and share K and V. A wave has 32 NR rows; tiles of 64 slots (32 where head_dim is 256) come to LDS
+// asynchronously, once for the workgroup, in a ring of stages. Products on v_mfma_f32_32x32x16, transposed throughout so that
+// nothing passes through LDS between the two:
+//   S^T [slot][row] = K Q^T: A = K (lane m = lane % 32 is the slot, 8 elements at 8 (lane / 32)), B = Q, kept in registers; of its
+//   result lane (row, g) has slots 8 (i / 4) + 4 g + i % 4 of 32. The weights in that place are, as they are, B operands of
+//   O^T [element][row] = V^T P^T when the operand's k index 8 g + j stands for slot 4 g + j (j < 4) or 8 + 4 g + j - 4 of 16;
+//   A = V^T by ds_read_b64_tr_b16, which transposes blocks of 4 slots by 16 elements.
+// Softmax: the weights of a tile are relative to the row's reference m of the tiles before. Their sum, which is needed anyway,
+// tells whether that was good: where it is beyond 2^8 (or NaN, or there is no reference yet) the tile's largest score becomes the
+// reference, the sums are scaled and the weights made again, so that the usual tile needs no maximum and no exchange between lanes.
+// 16-bit queries take weights of one 16-bit part, f32 ones of two (fp16) or three (bf16); sums are of the unrounded weights. fp16
+// parts end at 2^-24: weights stand there times 2^7, and where a tile's largest is below 2^-10, as in a tail beside slots that
+// take nearly all, m moves down to it, for which f32 sums have the range.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -7,72 +22,604 @@
 
 namespace p8x {
 
+typedef float float16v __attribute__((ext_vector_type(16)));
+
+template <bool BF>
+__device__ __forceinline__ float16v mfma32(uint4v a, uint4v b, float16v c) {
+    if constexpr (BF) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bhalf8, a), __builtin_bit_cast(bhalf8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+}
+
+// log2 of how far a tile's weights may add up beyond 1 before the reference moves up, and of how large the f32 sums may become
+// by its moving down
+constexpr float kUp = 8.0f, kRoom = 64.0f;
+constexpr int kStages = 4;   // in LDS: two in use (K of the next tile, V of this one), the others on their way
+__host__ __device__ constexpr int tile_slots(int D) { return D == 256 ? 32 : 64; }
+
 struct PromptJob {
     KvDev c;
     DraftDev d;
     void *out; size_t ldo, hso; int out_dtype;
     float *lse;
-    int D;
+    float *part;   // a record of each workgroup of a split segment: rows x D sums, then rows x (m, l)
+    int heads_wg;  // workgroups of a key/value head
+    int split, least;   // segments may be split over workgroups, into parts of at least so many tiles
 };
 
-// One workgroup a token and head, 256 slots at a time: a thread the score of one slot, then an element of the sums.
-__global__ __launch_bounds__(256) void k_prompt_simple(PromptJob J) {
-    __shared__ float q[256], p[256], red[4];
-    __shared__ int64_t at[256];
+// the sequences' share of a head's workgroups: sequence s has rts row tiles (segments) of at most `tiles` tiles of slots, each
+// cut into `parts`
+struct PromptSeq { int nt, n, first, rts, tiles, parts; };
+
+__device__ __forceinline__ int wave_total(int v) {
+    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+    return __builtin_amdgcn_readfirstlane(v);
+}
+
+template <int ROWS, int TS>
+__device__ __forceinline__ PromptSeq prompt_seq(const PromptJob &J, int s, int per) {
+    PromptSeq q{};
+    if (s >= J.c.n_seq) return q;
+    q.nt = seq_tokens(J.d, s, q.first);
+    q.n = seq_len(J.c, s);
+    q.rts = (int)(((int64_t)q.nt * J.d.G + ROWS - 1) / ROWS);
+    q.tiles = (q.n + TS - 1) / TS;
+    q.parts = per ? max(1, (q.tiles + per - 1) / per) : 1;
+    return q;
+}
+
+// tiles of a part, the least that fits a head's workgroups (0: segments whole)
+template <int ROWS, int TS>
+__device__ __forceinline__ int prompt_per(const PromptJob &J) {
+    if (!J.split) return 0;
+    const int lane = threadIdx.x & 63;
+    auto over = [&](auto f) {   // f(sequence) summed
+        int t = 0;
+        for (int s0 = 0; s0 < J.c.n_seq; s0 += 64) t += wave_total(f(s0 + lane));
+        return t;
+    };
+    const int tiles = over([&](int s) { const PromptSeq q = prompt_seq<ROWS, TS>(J, s, 0); return q.rts * q.tiles; });
+    int per = max(J.least, (tiles + J.heads_wg - 1) / J.heads_wg);
+    // (there are at least twice as many workgroups as segments: twice the first `per` always fits)
+    while (over([&](int s) { const PromptSeq q = prompt_seq<ROWS, TS>(J, s, per); return q.rts * q.parts; }) > J.heads_wg) per += (per + 7) / 8;
+    return per;
+}
+
+// The segment x (of a head's, all sequences' in a row; `part` of it when they are counted in parts): its sequence's numbers, s = -1
+// behind the last
+template <int ROWS, int TS>
+__device__ __forceinline__ PromptSeq prompt_find(const PromptJob &J, int per, bool in_parts, int x, int &s, int &rt, int &part) {
+    const int lane = threadIdx.x & 63;
+    int base = 0;
+    s = -1, rt = part = 0;
+    PromptSeq r{};
+    for (int s0 = 0; s0 < J.c.n_seq; s0 += 64) {
+        const PromptSeq q = prompt_seq<ROWS, TS>(J, s0 + lane, per);
+        const int v = q.rts * (in_parts ? q.parts : 1);
+        int y = v;
+        for (int o = 1; o < 64; o <<= 1) {
+            const int z = __shfl_up(y, o);
+            if (lane >= o) y += z;
+        }
+        const uint64_t in = __ballot(base + y > x);
+        if (in) {
+            const int f = __ffsll((unsigned long long)in) - 1;
+            auto of = [&](int a) { return __builtin_amdgcn_readlane(a, f); };
+            r = PromptSeq{of(q.nt), of(q.n), of(q.first), of(q.rts), of(q.tiles), of(q.parts)};
+            s = s0 + f;
+            const int i = x - base - of(y - v);
+            part = in_parts ? i % r.parts : 0;
+            rt = r.rts - 1 - (in_parts ? i / r.parts : i);   // the longest first
+            return r;
+        }
+        base += __builtin_amdgcn_readlane(y, 63);
+    }
+    return r;
+}
+
+template <int D>
+__device__ __forceinline__ void store_out(const PromptJob &J, int first, int h, int row, int e, float4v v, float m, float l, float bias) {
+    const int G = J.d.G, i = row / G, head = h * G + row - i * G;
+    v *= l == 0.0f ? 0.0f : 1.0f / l;
+    const size_t at = (size_t)(first + i) * J.ldo + (size_t)head * J.hso + e;
+    if (J.out_dtype == P8X_F32) *(float4v *)((float *)J.out + at) = v;
+    else if (J.out_dtype == P8X_BF16) *(uint2v *)((uint16_t *)J.out + at) = uint2v{pack2<true>(v[0], v[1]), pack2<true>(v[2], v[3])};
+    else *(uint2v *)((uint16_t *)J.out + at) = uint2v{pack2<false>(v[0], v[1]), pack2<false>(v[2], v[3])};
+    if (e == 0 && J.lse) J.lse[(size_t)(first + i) * J.c.n_kv * G + head] = l == 0.0f ? -INFINITY : (m - bias + __log2f(l)) * kLn2;
+}
+
+template <int D, bool BF, bool QF, int NR, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void k_prompt(PromptJob J) {
+    constexpr int TS = tile_slots(D), SUB = TS / 32, C = D / 16, DT = D / 32, KS = TS / 16, PC = D / 8, ROW = 2 * D, ROWS = 32 * NR * WAVES;
+    constexpr int QP = QF ? (BF ? 3 : 2) : 1, PP = QP;
+    constexpr float kBias = BF ? 0.0f : 7.0f;
+    // (fp16) log2 of a lane's sum of weights below which the tile's largest is looked up, and of that one below which m moves down
+    constexpr float kLow = QF ? 5.0f : 10.0f, kDown = 10.0f;
+    extern __shared__ float4v sh4[];
+    constexpr bool PING = WAVES == 8;
+    __shared__ int paged[8][KS];   // whether a stage's 16 slots have a page
+    __shared__ int odd_row[8][TS], any_odd[8][WAVES];   // slots with infinities or NaN among their values, of stages that some rows see in part; whether a wave found any
     const KvDev &c = J.c;
     const DraftDev &d = J.d;
-    const int t = threadIdx.x, D = J.D, head = blockIdx.y, h = head / d.G, s = blockIdx.z;
-    int first;
-    const int nt = seq_tokens(d, s, first), n = seq_len(c, s);
-    auto across = [&](float v, bool top) {
-        for (int o = 32; o; o >>= 1) v = top ? fmaxf(v, __shfl_xor(v, o)) : v + __shfl_xor(v, o);
-        __syncthreads();
-        if ((t & 63) == 0) red[t >> 6] = v;
-        __syncthreads();
-        return top ? fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])) : red[0] + red[1] + red[2] + red[3];
-    };
-    for (int i = blockIdx.x; i < nt; i += gridDim.x) {
-        const int see = max(0, n - nt + i + 1);   // slots
-        __syncthreads();
-        if (t < D) q[t] = load_as_f32(d.q, d.q_f32 ? P8X_F32 : c.bf16 ? P8X_BF16 : P8X_F16, (size_t)(first + i) * d.ld_q + (size_t)head * d.hs_q + t);
-        float m = -INFINITY, l = 0, o = 0;
-        for (int j0 = 0; j0 < see; j0 += 256) {
-            __syncthreads();
-            const int j = j0 + t;
-            const int64_t off = j < see ? slot_offset(c, s, j) : -1;
-            float x = -INFINITY;
-            if (off >= 0) {
-                x = 0;
-                const uint16_t *k = c.k + off + (size_t)h * c.head_stride;
-                for (int e = 0; e < D; ++e) x = fmaf(q[e], from16(k[e], c.bf16), x);
-                x *= d.scale;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 5, ln = lane & 31;
+    const int h = blockIdx.x % c.n_kv;
+    int s, rt, part;
+    const int per = prompt_per<ROWS, TS>(J);
+    const PromptSeq q = prompt_find<ROWS, TS>(J, per, true, blockIdx.x / c.n_kv, s, rt, part);
+    if (s < 0) return;
+    const int G = d.G, rows = q.nt * G, rows_here = min(ROWS, rows - rt * ROWS), ahead = q.n - q.nt;   // slots before the tokens
+    // tiles of the row tile's last token, and this part's
+    const int tiles = (max(0, ahead + (rt * ROWS + rows_here - 1) / G + 1) + TS - 1) / TS;
+    const int t0 = (int)((int64_t)tiles * part / q.parts), t1 = (int)((int64_t)tiles * (part + 1) / q.parts);
+    const uint16_t *kp = c.k + (size_t)h * c.head_stride, *vp = c.v + (size_t)h * c.head_stride;
+    const uint32_t ss = (uint32_t)c.slot_stride;
+    const int td = max(0, ahead + rt * ROWS / G + 1) / TS;   // the first tile that some row sees in part only
+
+    // ---- K and V of stage t to LDS: straight there where all of the wave's rows are in use and have a page, else through
+    // registers, rows that are not there as zeros
+    constexpr int RWV = 64 / PC, RP = WAVES * RWV, PASS = TS / RP;   // rows of a wave and of the workgroup in a pass
+    constexpr int STAGE = TS * ROW;                                  // bytes of a stage's K; its V follows
+    static_assert(PASS >= 1 && TS % RP == 0 && RWV <= 16, "passes");
+    // 16-byte pieces of a row lie at p ^ fk(row) (K), p ^ fv(row) (V), so that a read's rows are in other banks
+    auto fk = [](int row) { return PC < 16 ? row >> 1 & 7 : row & 15; };
+    auto fv = [](int row) { return PC < 16 ? (row >> 1 & 1) << 2 : (row & 3) << 2; };
+    char *const lds = (char *)sh4;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
+    const int rl = lane / PC, pl = lane % PC;
+    int lo = 0, hi = 0;
+    auto load = [&](int t) {
+        constexpr int CH = 64 / PASS;   // stages whose row offsets the lanes hold
+        const int st = t - t0;
+        if (st % CH == 0) {
+            const int slot = TS * (t + lane / PASS) + (lane % PASS) * RP + wave * RWV;
+            int64_t off = -1;
+            if (t + lane / PASS < t1 && slot < q.n) off = slot_offset(c, s, slot & ~15);
+            lo = (int)off, hi = (int)(off >> 32);
+        }
+        const int buf = (st % kStages) * 2 * STAGE;
+        bool direct = true;
+        int64_t off[PASS];
+#pragma unroll
+        for (int p = 0; p < PASS; ++p) {
+            const int r0 = p * RP + wave * RWV, from = st % CH * PASS + p;
+            off[p] = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, from) << 32 | (uint32_t)__builtin_amdgcn_readlane(lo, from));
+            direct = direct && off[p] >= 0 && TS * t + r0 + RWV <= q.n;
+            if (lane == 0 && r0 % 16 == 0) paged[st % 8][r0 / 16] = off[p] >= 0;
+        }
+        if (direct) {
+#pragma unroll
+            for (int p = 0; p < PASS; ++p) {
+                const uint32_t to = lds0 + buf + (p * RP + wave * RWV) * ROW;
+                const int r15 = (p * RP + wave * RWV + rl) & 15;   // the lane's row; its bytes from the 16 slots' first:
+                load_lds(kp + off[p], 2 * (r15 * ss + 8 * (pl ^ fk(r15))), to);
+                load_lds(vp + off[p], 2 * (r15 * ss + 8 * (pl ^ fv(r15))), to + STAGE);
             }
-            at[t] = off;
-            const float mx = fmaxf(m, across(x, true)), f = mx == -INFINITY ? 1.0f : expf(m - mx);
-            p[t] = x == -INFINITY ? 0.0f : expf(x - mx);
-            l = l * f + across(p[t], false);
-            o *= f;
-            m = mx;
-            if (t < D)
-                for (int k = 0; k < min(256, see - j0); ++k)
-                    if (at[k] >= 0) o = fmaf(p[k], from16(c.v[at[k] + (size_t)h * c.head_stride + t], c.bf16), o);
+            return;
         }
-        const size_t to = (size_t)(first + i) * J.ldo + (size_t)head * J.hso + t;
-        const float r = l == 0.0f ? 0.0f : o / l;
-        if (t < D) {
-            if (J.out_dtype == P8X_F32) ((float *)J.out)[to] = r;
-            else ((uint16_t *)J.out)[to] = to16(r, J.out_dtype == P8X_BF16);
+        __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the stages before have arrived
+#pragma unroll 1
+        for (int p = 0; p < PASS; ++p) {
+            const int r = p * RP + wave * RWV + rl, from = st % CH * PASS + p;
+            const int64_t offs = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, from) << 32 | (uint32_t)__builtin_amdgcn_readlane(lo, from));
+            uint4v k = {0, 0, 0, 0}, v = {0, 0, 0, 0};
+            if (offs >= 0 && TS * t + r < q.n) {
+                const size_t at = (size_t)offs + (size_t)(r % 16) * ss + 8 * pl;
+                k = *(const uint4v *)(kp + at);
+                v = *(const uint4v *)(vp + at);
+            }
+            *(uint4v *)(lds + buf + r * ROW + (pl ^ fk(r)) * 16) = k;
+            *(uint4v *)(lds + buf + STAGE + r * ROW + (pl ^ fv(r)) * 16) = v;
         }
-        if (t == 0 && J.lse) J.lse[(size_t)(first + i) * c.n_kv * d.G + head] = l == 0.0f ? -INFINITY : m + logf(l);
+    };
+    // Waits until stage t has arrived; the one two before it is no longer read then, and its place takes stage t + kStages - 2. Loads
+    // come back in order, 2 PASS of each stage: the younger one may be on its way (a stage through registers has waited for all
+    // before it; other loads make the wait longer, never shorter).
+    int loaded = t0;
+    auto arrive = [&](int t) {
+        if (t + 1 < t1 && loaded > t + 1) __asm__ volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * PASS) : "memory");
+        else __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (t >= td && t < t1) {   // some of the slots may be hidden from some rows: infinities and NaN among the wave's values
+            bool any = false;
+#pragma unroll 1
+            for (int p = 0; p < PASS; ++p) {
+                const int r = p * RP + wave * RWV + rl;
+                uint4v *at = (uint4v *)(lds + ((t - t0) % kStages) * 2 * STAGE + STAGE + r * ROW + pl * 16);
+                uint4v v = *at;
+                bool has = false;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    uint32_t w = v[e];
+                    has |= take_odd<BF>(w);
+                    v[e] = w;
+                }
+                const uint64_t by = __ballot(has);
+                if (by) *at = v;
+                if (pl == 0) odd_row[(t - t0) % 8][r] = (by >> (rl * PC) & (PC == 64 ? ~0ull : (1ull << PC) - 1)) != 0;
+                any |= by != 0;
+            }
+            if (lane == 0) any_odd[(t - t0) % 8][wave] = any;
+        }
+        __syncthreads();
+#pragma unroll 1
+        for (; loaded < min(t1, t + kStages - 1); ++loaded) load(loaded);
+    };
+    if (t0 < t1) {
+#pragma unroll 1
+        for (; loaded < min(t1, t0 + 2); ++loaded) load(loaded);
+    }
+
+    // ---- the wave's rows: queries, last slot that each sees
+    uint4v qf[NR][QP][C];
+    float16v o[NR][DT];
+    float m[NR], l[NR], c2[NR];
+    int lim[NR];
+    const int row0 = rt * ROWS + wave * 32 * NR, wrows = min(32 * NR, rows - row0);   // of the wave (0 or less: none)
+    const int last = ahead + (row0 + max(wrows, 1) - 1) / G, least = ahead + row0 / G;   // slots of the wave's last and first token
+    const int tw = wrows > 0 ? min(t1, (max(0, last + 1) + TS - 1) / TS) : t0;
+#pragma unroll
+    for (int a = 0; a < NR; ++a) {
+        const int r = row0 + 32 * a + ln, i = min(r, rows - 1) / G;
+        const bool on = r < rows;   // the others have queries of zeros and see what the last one does
+        lim[a] = ahead + i;
+        m[a] = -INFINITY;
+        l[a] = 0.0f;
+        c2[a] = fabsf(d.scale) * kLog2e;
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[a][t][e] = 0.0f;
+        const size_t at = on ? (size_t)(q.first + i) * d.ld_q + (size_t)(h * G + r - i * G) * d.hs_q + 8 * g : 0;
+        if constexpr (QF) {
+            // fp16 parts need the row scaled to 2^13 (the lane 32 apart holds the other half of it)
+            const float *p = (const float *)d.q + at;
+            float f[C][8], mx = 0.0f;
+#pragma unroll
+            for (int k = 0; k < C; ++k) {
+                const float4v x = on ? *(const float4v *)(p + 16 * k) : float4v{0, 0, 0, 0}, y = on ? *(const float4v *)(p + 16 * k + 4) : float4v{0, 0, 0, 0};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    f[k][e] = x[e], f[k][e + 4] = y[e];
+                    mx = fmaxf(mx, fmaxf(fabsf(x[e]), fabsf(y[e])));
+                }
+            }
+            float s1 = d.scale < 0 ? -1.0f : 1.0f, s2 = 1.0f;
+            if constexpr (!BF) {
+                mx = fmaxf(mx, __shfl_xor(mx, 32));
+                const int ex = mx > 0.0f && mx < INFINITY ? 13 - (int)((__builtin_bit_cast(uint32_t, mx) >> 23) - 127) : 0;
+                const int e1 = min(ex, 100);   // in two steps: 2^ex may be beyond f32
+                s1 *= ldexpf(1.0f, e1), s2 = ldexpf(1.0f, ex - e1);
+                c2[a] = ldexpf(c2[a], -ex);
+            }
+#pragma unroll
+            for (int k = 0; k < C; ++k) {
+                uint4v w[QP];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[k][e] = f[k][e] * s1 * s2;
+                split8<BF, QP>(f[k], w);
+#pragma unroll
+                for (int n = 0; n < QP; ++n) qf[a][n][k] = w[n];
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < C; ++k) {
+                uint4v w = on ? *(const uint4v *)((const uint16_t *)d.q + at + 16 * k) : uint4v{0, 0, 0, 0};
+                if (d.scale < 0) w ^= uint4v{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};   // its sign goes into the queries
+                qf[a][0][k] = w;
+            }
+        }
+        c2[a] = fmaxf(c2[a], 0x1p-149f);   // of a scale of 0, or one that underflows: hidden scores, -inf, stay so
+    }
+
+    const int k_at = ln * ROW + ((g ^ fk(ln)) * 16);   // pieces 2 c + g: c only flips higher bits
+    const int tl = lane & 15, v_row = 4 * g + (tl >> 2), v_at = v_row * ROW + ((((lane >> 4 & 1) * 2 + (tl >> 1 & 1)) ^ fv(v_row)) * 16) + 8 * (tl & 1);
+    auto place = [&](int t) { return lds + ((t - t0) % kStages) * 2 * STAGE; };
+    auto qk = [&](const char *k, float16v (&x)[NR][SUB]) {
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) {
+#pragma unroll
+            for (int a = 0; a < NR; ++a)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[a][u][e] = 0.0f;
+#pragma unroll
+            for (int n = 0; n < C; ++n) {
+                const uint4v kf = *(const uint4v *)(k + (k_at ^ 32 * n) + 32 * u * ROW);
+#pragma unroll
+                for (int p = QP - 1; p >= 0; --p)   // small parts first
+#pragma unroll
+                    for (int a = 0; a < NR; ++a) x[a][u] = mfma32<BF>(kf, qf[a][p][n], x[a][u]);
+            }
+        }
+    };
+    // scores to weights, in parts; returns the lane's sum of them
+    auto weights = [&](const float16v (&x)[SUB], float c2, float m, uint4v (&p)[KS][PP]) {
+        const float base = (m == -INFINITY ? 0.0f : m) - kBias;
+        float sum = 0;
+#pragma unroll
+        for (int u = 0; u < SUB; ++u)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                float f[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    f[e] = __builtin_amdgcn_exp2f(fmaf(x[u][8 * half + e], c2, -base));
+                    sum += f[e];
+                }
+                uint4v w[PP];
+                split8<BF, PP>(f, w);
+#pragma unroll
+                for (int n = 0; n < PP; ++n) p[2 * u + half][n] = w[n];
+            }
+        return sum;
+    };
+    bool settled = false;   // every row has a reference
+    auto softmax = [&](float16v (&x)[NR][SUB], uint4v (&p)[NR][KS][PP]) {
+        float sum[NR];
+        bool bad = !settled;
+#pragma unroll
+        for (int a = 0; a < NR; ++a) {
+            sum[a] = weights(x[a], c2[a], m[a], p[a]);
+            bad |= !(sum[a] <= __builtin_exp2f(kUp + kBias));
+            if (!BF) bad |= sum[a] < __builtin_exp2f(kBias - kLow);
+        }
+        if (__any(bad)) {
+            settled = true;
+#pragma unroll
+            for (int a = 0; a < NR; ++a) {
+                float v = -INFINITY;
+#pragma unroll
+                for (int u = 0; u < SUB; ++u)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) v = fmaxf(v, x[a][u][e]);
+                v = fmaxf(v, __shfl_xor(v, 32)) * c2[a];   // log2 of the tile's largest (-inf: the row sees none of it)
+                float to = m[a];
+                if (v > m[a] && (m[a] == -INFINITY || !(sum[a] <= __builtin_exp2f(kUp + kBias)))) {
+                    to = v;
+                } else if (!BF && v < m[a] - kDown && v > -INFINITY) {
+                    const float ls = l[a] + __shfl_xor(l[a], 32);
+                    to = fmaxf(v, fminf(m[a], m[a] - (kRoom - __log2f(ls))));
+                }
+                to = fmaxf(to, __shfl_xor(to, 32));   // where one of the row's two lanes moves up so does the other
+                const float al = m[a] == -INFINITY || to == m[a] ? 1.0f : __builtin_amdgcn_exp2f(m[a] - to);
+                m[a] = to;
+                settled = settled && !__any(to == -INFINITY);
+                l[a] *= al;
+#pragma unroll
+                for (int t = 0; t < DT; ++t) o[a][t] *= al;
+                sum[a] = weights(x[a], c2[a], m[a], p[a]);
+            }
+        }
+#pragma unroll
+        for (int a = 0; a < NR; ++a) l[a] += sum[a];
+    };
+    // hides what a row does not see: later tokens' slots, those without a page
+    auto hide = [&](int t, float16v (&x)[NR][SUB]) {
+        int pg[KS];
+#pragma unroll
+        for (int k = 0; k < KS; ++k) pg[k] = __builtin_amdgcn_readfirstlane(paged[(t - t0) % 8][k]);
+#pragma unroll
+        for (int a = 0; a < NR; ++a) {
+            const int see = lim[a] - TS * t - 4 * g;
+#pragma unroll
+            for (int u = 0; u < SUB; ++u)
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const int upto = pg[2 * u + half] ? see : -1;
+#pragma unroll
+                    for (int e = 8 * half; e < 8 * half + 8; ++e) x[a][u][e] = 32 * u + 8 * (e / 4) + e % 4 > upto ? -INFINITY : x[a][u][e];
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+        }
+    };
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    auto vt = [&](const char *v, int t, int ks) {   // V^T operand: elements 32 t .., slots 16 ks ..
+        uint2v e[2];
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+            e[half] = __builtin_bit_cast(uint2v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)(v + (v_at ^ 64 * t) + (16 * ks + 8 * half) * ROW)));
+        return uint4v{e[0][0], e[0][1], e[1][0], e[1][1]};
+    };
+    auto pv = [&](const char *v, const uint4v (&p)[NR][KS][PP]) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int t = 0; t < DT; ++t) {
+                const uint4v e = vt(v, t, ks);
+#pragma unroll
+                for (int n = PP - 1; n >= 0; --n)
+#pragma unroll
+                    for (int a = 0; a < NR; ++a) o[a][t] = mfma32<BF>(e, p[a][ks][n], o[a][t]);
+            }
+    };
+    // Adds the odd values of a stage's slots, which are zeros there, to the rows that see them.
+    auto add_odd = [&](int t) {
+        for (int j = 0; j < TS; ++j) {
+            if (!__builtin_amdgcn_readfirstlane(odd_row[(t - t0) % 8][j])) continue;
+            const int slot = TS * t + j;
+            const uint16_t *p = vp + slot_offset(c, s, slot) + 4 * g;
+#pragma unroll
+            for (int k = 0; k < DT; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint2v w = *(const uint2v *)(p + 32 * k + 8 * i);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t word = e < 2 ? w[0] : w[1];
+                        const float v = e & 1 ? part_hi<BF>(word) : part_lo<BF>(word);
+#pragma unroll
+                        for (int a = 0; a < NR; ++a)
+                            o[a][k][4 * i + e] += !(v - v == 0.0f) && slot <= lim[a] ? v : 0.0f;
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+        }
+    };
+
+    float16v x[NR][SUB];
+    uint4v p[NR][KS][PP];
+    auto phase_s = [&](int t) {
+        int pages = 1;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) pages &= paged[(t - t0) % 8][k];
+        if (TS * t + TS - 1 > least || !__builtin_amdgcn_readfirstlane(pages)) hide(t, x);
+        softmax(x, p);
+    };
+    auto phase_m = [&](int t) {
+        pv(place(t) + STAGE, p);
+        qk(place(min(t + 1, tw - 1)), x);   // (of the last tile once more: not used)
+        if constexpr (QP == 1) {   // operands from LDS some products ahead, no more of them than registers
+            constexpr int AHEAD = 4, NV = KS * DT, NK = SUB * C;
+            __builtin_amdgcn_sched_group_barrier(0x100, 2 * AHEAD, 0);
+#pragma unroll
+            for (int i = 0; i < NV + NK; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x8, NR, 0);
+                if (i + AHEAD < NV) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+                else if (i + AHEAD < NV + NK) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (t >= td) {
+            int any = 0;
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) any |= any_odd[(t - t0) % 8][w];
+            if (__builtin_amdgcn_readfirstlane(any)) add_odd(t);
+        }
+    };
+    if (t0 < t1) {
+        arrive(t0);
+        if (t0 < tw) qk(place(t0), x);
+        // With two waves a SIMD of the compute unit, one makes weights while the other multiplies: the second four waves are half a
+        // turn behind, and a barrier follows each half. Stages arrive at the first's middles.
+        const int grp = PING ? wave >> 2 : 0;
+        if (grp) arrive(t0 + 1);
+        auto halves = [&](int n) {   // the barrier after half n
+            if (!PING && (n & 1)) return;
+            if ((n & 1) ^ grp) __syncthreads();
+            else arrive(t0 + 1 + ((n + grp) >> 1));
+        };
+        int t = t0;
+#pragma unroll 1
+        for (; t < tw; ++t) {
+            phase_s(t);
+            halves(2 * (t - t0));
+            phase_m(t);
+            halves(2 * (t - t0) + 1);
+        }
+#pragma unroll 1
+        for (int n = 2 * (t - t0); n < 2 * (t1 - t0) + (PING && !grp); ++n) halves(n);
+    }
+
+    float *rec = J.part + (size_t)blockIdx.x * ROWS * (D + 2);
+#pragma unroll
+    for (int a = 0; a < NR; ++a) {
+        const int r = row0 + 32 * a + ln;
+        l[a] += __shfl_xor(l[a], 32);
+        if (r >= rows) continue;
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float4v v{o[a][t][4 * i], o[a][t][4 * i + 1], o[a][t][4 * i + 2], o[a][t][4 * i + 3]};
+                const int e = 32 * t + 8 * i + 4 * g;
+                if (q.parts == 1) {
+                    store_out<D>(J, q.first, h, r, e, v, m[a], l[a], kBias);
+                } else {
+                    *(float4v *)(rec + (size_t)(r - rt * ROWS) * D + e) = v;
+                    if (e == 0) *(float2 *)(rec + (size_t)ROWS * D + 2 * (r - rt * ROWS)) = make_float2(m[a], l[a]);
+                }
+            }
     }
 }
 
-size_t attn_prompt_workspace(const KvDev &, const DraftDev &, int) { return 0; }
+// The records of split segments: a thread four elements of a row, over all parts in order.
+template <int D, int ROWS>
+__global__ __launch_bounds__(256) void k_prompt_join(PromptJob J) {
+    constexpr int TS = tile_slots(D);
+    const KvDev &c = J.c;
+    const float bias = c.bf16 ? 0.0f : 7.0f;
+    const int h = blockIdx.x % c.n_kv, x = blockIdx.x / c.n_kv;
+    const int per = prompt_per<ROWS, TS>(J);
+    int s, rt, part;
+    const PromptSeq q = prompt_find<ROWS, TS>(J, per, false, x, s, rt, part);
+    if (s < 0 || q.parts < 2) return;
+    // the workgroups of the segment's parts: those of the sequences before, then of the longer row tiles
+    int before = 0;
+    for (int s0 = 0; s0 < s; s0 += 64) {
+        const PromptSeq p = prompt_seq<ROWS, TS>(J, s0 + (threadIdx.x & 63), per);
+        before += wave_total(s0 + (int)(threadIdx.x & 63) < s ? p.rts * p.parts : 0);
+    }
+    const int b0 = before + (q.rts - 1 - rt) * q.parts;
+    const int rows = min(ROWS, q.nt * J.d.G - rt * ROWS);
+    for (int i = blockIdx.y * 256 + threadIdx.x; i < rows * (D / 4); i += gridDim.y * 256) {
+        const int r = i / (D / 4), e = i % (D / 4) * 4;
+        float4v v = {0, 0, 0, 0};
+        float m = -INFINITY, l = 0.0f;
+        for (int b = 0; b < q.parts; ++b) {
+            const float *rec = J.part + (size_t)((b0 + b) * c.n_kv + h) * ROWS * (D + 2);
+            const float2 ml = *(const float2 *)(rec + (size_t)ROWS * D + 2 * r);
+            const float4v w = *(const float4v *)(rec + (size_t)r * D + e);
+            if (ml.x == -INFINITY) continue;   // a part that the row sees nothing of
+            const float mn = fmaxf(m, ml.x), f0 = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn), f1 = __builtin_amdgcn_exp2f(ml.x - mn);
+            v = m == -INFINITY ? w * f1 : v * f0 + w * f1;
+            l = l * f0 + ml.y * f1;
+            m = mn;
+        }
+        store_out<D>(J, q.first, h, rt * ROWS + r, e, v, m, l, bias);
+    }
+}
 
-int launch_attn_prompt(const KvDev &c, const DraftDev &d, int D, void *out, int out_dtype, size_t ldo, size_t hso, float *lse, void *, size_t, hipStream_t st) {
-    const PromptJob J{c, d, out, ldo, hso, out_dtype, lse, D};
-    k_prompt_simple<<<dim3(std::min(d.max_tokens, 65535), c.n_kv * d.G, c.n_seq), 256, 0, st>>>(J);
+// Rows of a workgroup: 8 waves of 32 rows; 4 waves where that leaves compute units without one, and where rows of 256 elements
+// or queries of several parts take more than 256 registers a lane.
+struct PromptPlan { int waves, rows, segs, heads_wg; size_t rec_bytes; };
+static PromptPlan prompt_plan(const KvDev &c, const DraftDev &d, int D) {
+    PromptPlan p;
+    auto segs = [&](int rows) {   // of a head: row tiles of all sequences, at most
+        const int64_t each = ((int64_t)d.max_tokens * d.G + rows - 1) / rows, all = (int64_t)d.n_tokens * d.G / rows + std::min(c.n_seq, d.n_tokens);
+        return std::min(each * c.n_seq, all);
+    };
+    p.waves = D == 256 || d.q_f32 || segs(256) * c.n_kv < num_cus() ? 4 : 8;
+    p.rows = 32 * p.waves;
+    const int64_t n = segs(p.rows);
+    p.segs = (int)std::min<int64_t>(n, INT32_MAX);
+    p.heads_wg = num_cus() / c.n_kv;   // when they are split
+    p.rec_bytes = 4 * (size_t)p.rows * (D + 2);
+    return p;
+}
+
+size_t attn_prompt_workspace(const KvDev &c, const DraftDev &d, int D) {
+    const PromptPlan p = prompt_plan(c, d, D);
+    return p.heads_wg >= 2 * p.segs ? (size_t)p.heads_wg * c.n_kv * p.rec_bytes : 0;
+}
+
+template <int D, bool BF, bool QF, int WAVES>
+static int prompt_run(const PromptJob &J, int segs, hipStream_t st) {
+    constexpr int lds = kStages * 2 * tile_slots(D) * 2 * D, ROWS = 32 * WAVES;
+    static OncePerDevice once;
+    if (int rc = allow_lds(once, (const void *)k_prompt<D, BF, QF, 1, WAVES>, lds, "p8x_attn_prompt LDS")) return rc;
+    k_prompt<D, BF, QF, 1, WAVES><<<J.heads_wg * J.c.n_kv, 64 * WAVES, lds, st>>>(J);
+    if (J.split) k_prompt_join<D, ROWS><<<dim3(segs * J.c.n_kv, 8), 256, 0, st>>>(J);
     return hip_check(hipGetLastError(), "p8x_attn_prompt launch");
+}
+
+template <int D, bool BF>
+static int prompt_types(const PromptJob &J, const PromptPlan &p, hipStream_t st) {
+    if (J.d.q_f32) return prompt_run<D, BF, true, 4>(J, p.segs, st);
+    if constexpr (D < 256) {
+        if (p.waves == 8) return prompt_run<D, BF, false, 8>(J, p.segs, st);
+    }
+    return prompt_run<D, BF, false, 4>(J, p.segs, st);
+}
+
+int launch_attn_prompt(const KvDev &c, const DraftDev &d, int D, void *out, int out_dtype, size_t ldo, size_t hso, float *lse, void *ws, size_t ws_bytes,
+                       hipStream_t st) {
+    if (c.slot_stride >= (1u << 26)) return set_error(P8X_ERR_UNSUPPORTED, "p8x_attn_prompt: slot_stride %zu (below 2^26)", c.slot_stride);
+    const PromptPlan p = prompt_plan(c, d, D);
+    if ((int64_t)p.segs * c.n_kv > INT32_MAX || (int64_t)d.max_tokens * d.G > INT32_MAX)
+        return set_error(P8X_ERR_UNSUPPORTED, "p8x_attn_prompt: %d row tiles of %d heads, %d tokens of %d heads", p.segs, c.n_kv, d.max_tokens, d.G);
+    PromptJob J{c, d, out, ldo, hso, out_dtype, lse, (float *)ws, p.segs, 0, 4};
+    const int room = (int)std::min<size_t>(p.heads_wg, ws_bytes / p.rec_bytes / c.n_kv);
+    if (room >= 2 * p.segs) J.split = 1, J.heads_wg = room;
+    if (D == 64) return c.bf16 ? prompt_types<64, true>(J, p, st) : prompt_types<64, false>(J, p, st);
+    if (D == 128) return c.bf16 ? prompt_types<128, true>(J, p, st) : prompt_types<128, false>(J, p, st);
+    return c.bf16 ? prompt_types<256, true>(J, p, st) : prompt_types<256, false>(J, p, st);
 }
 
 }  // namespace p8x

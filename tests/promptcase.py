@@ -35,29 +35,30 @@ class Prompt(Case):
             n, nt = self.lens[s], self.toks[s]
             there = np.array([self.there(s, j) for j in range(n)], bool)
             for h in range(self.kv):
-                k, v = (np.array([from_bits(self.row(p, s, j)[h], self.cache) if there[j] else np.zeros(self.D) for j in range(n)]).reshape(n, self.D)
+                k, v = (from_bits(np.array([self.row(p, s, j)[h] if there[j] else np.zeros(self.D, np.uint16) for j in range(n)], np.uint16).reshape(n, self.D), self.cache)
                         for p in (self.kb, self.vb))
-                for i in range(nt):
-                    end = max(0, n - nt + i + 1)
-                    see = np.flatnonzero(there[:end])
-                    tok = self.first[s] + i
-                    for head in range(h * self.G, (h + 1) * self.G):
-                        if not len(see):
-                            continue
-                        q = from_bits(self.qb[tok, head], self.qt)
-                        x = self.scale * (k[see] @ q)
-                        m = x.max()
-                        z = m + np.log(np.exp(x - m).sum())
-                        w = np.exp(x - z)
-                        vs = v[see]
-                        lse[tok, head], out[tok, head] = z, w @ vs
-                        a = w @ np.abs(vs)
-                        qk = abs(self.scale) * (np.abs(k[see]) @ np.abs(q)).max()
-                        es = ((self.D + 8) * 2.0 ** -24 + (2.0 ** -21 if f32 else 0)) * qk + 2.0 ** -22 * np.abs(x).max() + 2.0 ** -21
-                        sums = (len(see) + 64) * 2.0 ** -24
-                        err = a * (uw + 2 * es + 2 * sums) * 1.01 + floor * 64 * np.abs(vs).max()
-                        tol[tok, head] = err + half_ulp(self.out_t) * (np.abs(out[tok, head]) + err) + (2.0 ** -25 if self.out_t == F16 else 0)
-                        ltol[tok, head] = es + sums + 2.0 ** -22 * (1 + abs(z)) + floor * 64 * 0
+                if not n or not nt:
+                    continue
+                toks = slice(self.first[s], self.first[s] + nt)
+                # [nt][slots] whether a token sees a slot
+                see = there & (np.arange(n) <= (n - nt + np.arange(nt))[:, None])
+                some = see.any(1)
+                for head in range(h * self.G, (h + 1) * self.G):
+                    q = from_bits(self.qb[toks, head], self.qt)
+                    x = np.where(see, self.scale * (q @ k.T), -np.inf)
+                    m = np.where(some, x.max(1), 0.0)
+                    z = m + np.log(np.maximum(np.exp(x - m[:, None]).sum(1), 1e-300))
+                    w = np.exp(x - z[:, None]) * some[:, None]
+                    lse[toks, head] = np.where(some, z, -np.inf)
+                    out[toks, head] = w @ v
+                    a = w @ np.abs(v)
+                    qk = abs(self.scale) * np.where(see, np.abs(q) @ np.abs(k).T, 0.0).max(1)
+                    big = np.where(see, np.abs(x), 0.0).max(1)
+                    es = ((self.D + 8) * 2.0 ** -24 + (2.0 ** -21 if f32 else 0)) * qk + 2.0 ** -22 * big + 2.0 ** -21
+                    sums = (see.sum(1) + 64) * 2.0 ** -24
+                    err = a * (uw + 2 * es + 2 * sums)[:, None] * 1.01 + floor * 64 * np.abs(v).max()
+                    tol[toks, head] = err + half_ulp(self.out_t) * (np.abs(out[toks, head]) + err) + (2.0 ** -25 if self.out_t == F16 else 0)
+                    ltol[toks, head] = es + sums + 2.0 ** -22 * (1 + np.abs(z))
         return out, lse, tol, ltol
 
     def run(self, workspace=None, lse=True, stream=None, call=None):
