@@ -34,7 +34,8 @@ __device__ __forceinline__ float16v mfma32(uint4v a, uint4v b, float16v c) {
 // by its moving down
 constexpr float kUp = 8.0f, kRoom = 64.0f;
 constexpr int kStages = 4;   // in LDS: two in use (K of the next tile, V of this one), the others on their way
-__host__ __device__ constexpr int tile_slots(int D) { return D == 256 ? 32 : 64; }
+// slots of a tile: fewer where the operands of 64 do not fit the registers
+__host__ __device__ constexpr int tile_slots(int D, bool bf, bool qf) { return D == 256 || (D == 128 && bf && qf) ? 32 : 64; }
 
 struct PromptJob {
     KvDev c;
@@ -128,8 +129,8 @@ __device__ __forceinline__ void store_out(const PromptJob &J, int first, int h, 
 }
 
 template <int D, bool BF, bool QF, int NR, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void k_prompt(PromptJob J) {
-    constexpr int TS = tile_slots(D), SUB = TS / 32, C = D / 16, DT = D / 32, KS = TS / 16, PC = D / 8, ROW = 2 * D, ROWS = 32 * NR * WAVES;
+__global__ __launch_bounds__(64 * WAVES, QF && D == 256 ? 1 : 2) void k_prompt(PromptJob J) {
+    constexpr int TS = tile_slots(D, BF, QF), SUB = TS / 32, C = D / 16, DT = D / 32, KS = TS / 16, PC = D / 8, ROW = 2 * D, ROWS = 32 * NR * WAVES;
     constexpr int QP = QF ? (BF ? 3 : 2) : 1, PP = QP;
     constexpr float kBias = BF ? 0.0f : 7.0f;
     // (fp16) log2 of a lane's sum of weights below which the tile's largest is looked up, and of that one below which m moves down
@@ -149,7 +150,8 @@ __global__ __launch_bounds__(64 * WAVES) void k_prompt(PromptJob J) {
     const int G = d.G, rows = q.nt * G, rows_here = min(ROWS, rows - rt * ROWS), ahead = q.n - q.nt;   // slots before the tokens
     // tiles of the row tile's last token, and this part's
     const int tiles = (max(0, ahead + (rt * ROWS + rows_here - 1) / G + 1) + TS - 1) / TS;
-    const int t0 = (int)((int64_t)tiles * part / q.parts), t1 = (int)((int64_t)tiles * (part + 1) / q.parts);
+    const int share = q.parts == 1 ? tiles : tiles / q.parts, more = tiles - share * q.parts;
+    const int t0 = part * share + min(part, more), t1 = t0 + share + (part < more);
     const uint16_t *kp = c.k + (size_t)h * c.head_stride, *vp = c.v + (size_t)h * c.head_stride;
     const uint32_t ss = (uint32_t)c.slot_stride;
     const int td = max(0, ahead + rt * ROWS / G + 1) / TS;   // the first tile that some row sees in part only
@@ -314,20 +316,21 @@ __global__ __launch_bounds__(64 * WAVES) void k_prompt(PromptJob J) {
     auto place = [&](int t) { return lds + ((t - t0) % kStages) * 2 * STAGE; };
     auto qk = [&](const char *k, float16v (&x)[NR][SUB]) {
 #pragma unroll
-        for (int u = 0; u < SUB; ++u) {
+        for (int a = 0; a < NR; ++a)
 #pragma unroll
-            for (int a = 0; a < NR; ++a)
+            for (int u = 0; u < SUB; ++u)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) x[a][u][e] = 0.0f;
 #pragma unroll
-            for (int n = 0; n < C; ++n) {
+        for (int n = 0; n < C; ++n)
+#pragma unroll
+            for (int u = 0; u < SUB; ++u) {   // (sums in turn: a product waits for the one before on its own)
                 const uint4v kf = *(const uint4v *)(k + (k_at ^ 32 * n) + 32 * u * ROW);
 #pragma unroll
                 for (int p = QP - 1; p >= 0; --p)   // small parts first
 #pragma unroll
                     for (int a = 0; a < NR; ++a) x[a][u] = mfma32<BF>(kf, qf[a][p][n], x[a][u]);
             }
-        }
     };
     // scores to weights, in parts; returns the lane's sum of them
     auto weights = [&](const float16v (&x)[SUB], float c2, float m, uint4v (&p)[KS][PP]) {
@@ -354,13 +357,19 @@ __global__ __launch_bounds__(64 * WAVES) void k_prompt(PromptJob J) {
     auto softmax = [&](float16v (&x)[NR][SUB], uint4v (&p)[NR][KS][PP]) {
         float sum[NR];
         bool bad = !settled;
+        if (settled) {
 #pragma unroll
-        for (int a = 0; a < NR; ++a) {
-            sum[a] = weights(x[a], c2[a], m[a], p[a]);
-            bad |= !(sum[a] <= __builtin_exp2f(kUp + kBias));
-            if (!BF) bad |= sum[a] < __builtin_exp2f(kBias - kLow);
+            for (int a = 0; a < NR; ++a) {
+                sum[a] = weights(x[a], c2[a], m[a], p[a]);
+                bad |= !(sum[a] <= __builtin_exp2f(kUp + kBias));
+                if (!BF) bad |= sum[a] < __builtin_exp2f(kBias - kLow);
+            }
+            bad = __any(bad);
+        } else {
+#pragma unroll
+            for (int a = 0; a < NR; ++a) sum[a] = INFINITY;
         }
-        if (__any(bad)) {
+        if (bad) {
             settled = true;
 #pragma unroll
             for (int a = 0; a < NR; ++a) {
@@ -466,7 +475,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_prompt(PromptJob J) {
         pv(place(t) + STAGE, p);
         qk(place(min(t + 1, tw - 1)), x);   // (of the last tile once more: not used)
         if constexpr (QP == 1) {   // operands from LDS some products ahead, no more of them than registers
-            constexpr int AHEAD = 4, NV = KS * DT, NK = SUB * C;
+            constexpr int AHEAD = D == 256 ? 4 : 8, NV = KS * DT, NK = SUB * C;
             __builtin_amdgcn_sched_group_barrier(0x100, 2 * AHEAD, 0);
 #pragma unroll
             for (int i = 0; i < NV + NK; ++i) {
@@ -530,9 +539,8 @@ __global__ __launch_bounds__(64 * WAVES) void k_prompt(PromptJob J) {
 }
 
 // The records of split segments: a thread four elements of a row, over all parts in order.
-template <int D, int ROWS>
+template <int D, int TS, int ROWS>
 __global__ __launch_bounds__(256) void k_prompt_join(PromptJob J) {
-    constexpr int TS = tile_slots(D);
     const KvDev &c = J.c;
     const float bias = c.bf16 ? 0.0f : 7.0f;
     const int h = blockIdx.x % c.n_kv, x = blockIdx.x / c.n_kv;
@@ -575,7 +583,7 @@ static PromptPlan prompt_plan(const KvDev &c, const DraftDev &d, int D) {
         const int64_t each = ((int64_t)d.max_tokens * d.G + rows - 1) / rows, all = (int64_t)d.n_tokens * d.G / rows + std::min(c.n_seq, d.n_tokens);
         return std::min(each * c.n_seq, all);
     };
-    p.waves = D == 256 || d.q_f32 || segs(256) * c.n_kv < num_cus() ? 4 : 8;
+    p.waves = (D == 256 && d.q_f32) || segs(256) * c.n_kv < num_cus() ? 4 : 8;
     p.rows = 32 * p.waves;
     const int64_t n = segs(p.rows);
     p.segs = (int)std::min<int64_t>(n, INT32_MAX);
@@ -591,21 +599,21 @@ size_t attn_prompt_workspace(const KvDev &c, const DraftDev &d, int D) {
 
 template <int D, bool BF, bool QF, int WAVES>
 static int prompt_run(const PromptJob &J, int segs, hipStream_t st) {
-    constexpr int lds = kStages * 2 * tile_slots(D) * 2 * D, ROWS = 32 * WAVES;
+    constexpr int TS = tile_slots(D, BF, QF), lds = kStages * 2 * TS * 2 * D, ROWS = 32 * WAVES;
     static OncePerDevice once;
     if (int rc = allow_lds(once, (const void *)k_prompt<D, BF, QF, 1, WAVES>, lds, "p8x_attn_prompt LDS")) return rc;
     k_prompt<D, BF, QF, 1, WAVES><<<J.heads_wg * J.c.n_kv, 64 * WAVES, lds, st>>>(J);
-    if (J.split) k_prompt_join<D, ROWS><<<dim3(segs * J.c.n_kv, 8), 256, 0, st>>>(J);
+    if (J.split) k_prompt_join<D, TS, ROWS><<<dim3(segs * J.c.n_kv, 8), 256, 0, st>>>(J);
     return hip_check(hipGetLastError(), "p8x_attn_prompt launch");
 }
 
 template <int D, bool BF>
 static int prompt_types(const PromptJob &J, const PromptPlan &p, hipStream_t st) {
-    if (J.d.q_f32) return prompt_run<D, BF, true, 4>(J, p.segs, st);
     if constexpr (D < 256) {
-        if (p.waves == 8) return prompt_run<D, BF, false, 8>(J, p.segs, st);
+        if (J.d.q_f32 && p.waves == 8) return prompt_run<D, BF, true, 8>(J, p.segs, st);
     }
-    return prompt_run<D, BF, false, 4>(J, p.segs, st);
+    if (J.d.q_f32) return prompt_run<D, BF, true, 4>(J, p.segs, st);
+    return p.waves == 8 ? prompt_run<D, BF, false, 8>(J, p.segs, st) : prompt_run<D, BF, false, 4>(J, p.segs, st);
 }
 
 int launch_attn_prompt(const KvDev &c, const DraftDev &d, int D, void *out, int out_dtype, size_t ldo, size_t hso, float *lse, void *ws, size_t ws_bytes,
