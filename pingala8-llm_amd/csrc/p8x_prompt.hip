@@ -137,7 +137,6 @@ __global__ __launch_bounds__(64 * WAVES, QF && D == 256 ? 1 : 2) void k_prompt(P
     constexpr float kLow = QF ? 5.0f : 10.0f, kDown = 10.0f;
     extern __shared__ float4v sh4[];
     constexpr bool PING = WAVES == 8;
-    __shared__ int paged[8][KS];   // whether a stage's 16 slots have a page
     __shared__ int odd_row[8][TS], any_odd[8][WAVES];   // slots with infinities or NaN among their values, of stages that some rows see in part; whether a wave found any
     const KvDev &c = J.c;
     const DraftDev &d = J.d;
@@ -167,44 +166,55 @@ __global__ __launch_bounds__(64 * WAVES, QF && D == 256 ? 1 : 2) void k_prompt(P
     char *const lds = (char *)sh4;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
     const int rl = lane / PC, pl = lane % PC;
-    int lo = 0, hi = 0;
-    auto load = [&](int t) {
-        constexpr int CH = 64 / PASS;   // stages whose row offsets the lanes hold
-        const int st = t - t0;
-        if (st % CH == 0) {
-            const int slot = TS * (t + lane / PASS) + (lane % PASS) * RP + wave * RWV;
-            int64_t off = -1;
-            if (t + lane / PASS < t1 && slot < q.n) off = slot_offset(c, s, slot & ~15);
-            lo = (int)off, hi = (int)(off >> 32);
-        }
-        const int buf = (st % kStages) * 2 * STAGE;
-        bool direct = true;
-        int64_t off[PASS];
+    uint32_t kl[2], vl[2];   // the lane's bytes from its 16 slots' first
 #pragma unroll
-        for (int p = 0; p < PASS; ++p) {
-            const int r0 = p * RP + wave * RWV, from = st % CH * PASS + p;
-            off[p] = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, from) << 32 | (uint32_t)__builtin_amdgcn_readlane(lo, from));
-            direct = direct && off[p] >= 0 && TS * t + r0 + RWV <= q.n;
-            if (lane == 0 && r0 % 16 == 0) paged[st % 8][r0 / 16] = off[p] >= 0;
-        }
+    for (int p = 0; p < (RP % 16 ? 2 : 1); ++p) {
+        const int r15 = (p * RP + wave * RWV + rl) & 15;
+        kl[p] = 2 * (r15 * ss + 8 * (pl ^ fk(r15)));
+        vl[p] = 2 * (r15 * ss + 8 * (pl ^ fv(r15)));
+    }
+    // Of CH stages from c0 on, the lanes hold where their groups of 16 slots lie; bit KS i + k: group k of stage c0 + i has a page
+    constexpr int CH = 64 / KS;
+    int lo = 0, hi = 0, c0 = 0;
+    uint64_t here = 0, before = 0;   // of these stages, of the CH before them
+    auto pages = [&](int st) {
+        const int slot = TS * (t0 + st + lane / KS) + 16 * (lane % KS);
+        int64_t off = -1;
+        if (t0 + st + lane / KS < t1 && slot < q.n) off = slot_offset(c, s, slot);
+        lo = (int)off, hi = (int)(off >> 32), c0 = st;
+        before = here;
+        here = __ballot(off >= 0);
+    };
+    auto group = [&](int st, int p) {   // where the 16 slots of the wave's rows of a pass lie
+        const int from = (st - c0) * KS + (p * RP + wave * RWV) / 16;
+        return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, from) << 32 | (uint32_t)__builtin_amdgcn_readlane(lo, from));
+    };
+    auto load_direct = [&](int t, int i) {   // load i of 2 PASS
+        const int p = i / 2;
+        const uint32_t to = lds0 + (uint32_t)(t - t0) % kStages * 2 * STAGE + (p * RP + wave * RWV) * ROW;
+        const int64_t off = group(t - t0, p);
+        if (i % 2) load_lds(vp + off, vl[RP % 16 ? p & 1 : 0], to + STAGE);
+        else load_lds(kp + off, kl[RP % 16 ? p & 1 : 0], to);
+    };
+    auto load = [&](int t) {
+        if ((t - t0) % CH == 0) pages(t - t0);
+        bool direct = true;
+#pragma unroll
+        for (int p = 0; p < PASS; ++p) direct = direct && group(t - t0, p) >= 0 && TS * t + p * RP + wave * RWV + RWV <= q.n;
         if (direct) {
 #pragma unroll
-            for (int p = 0; p < PASS; ++p) {
-                const uint32_t to = lds0 + buf + (p * RP + wave * RWV) * ROW;
-                const int r15 = (p * RP + wave * RWV + rl) & 15;   // the lane's row; its bytes from the 16 slots' first:
-                load_lds(kp + off[p], 2 * (r15 * ss + 8 * (pl ^ fk(r15))), to);
-                load_lds(vp + off[p], 2 * (r15 * ss + 8 * (pl ^ fv(r15))), to + STAGE);
-            }
+            for (int i = 0; i < 2 * PASS; ++i) load_direct(t, i);
             return;
         }
+        const uint32_t buf = (uint32_t)(t - t0) % kStages * 2 * STAGE;
         __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the stages before have arrived
 #pragma unroll 1
         for (int p = 0; p < PASS; ++p) {
-            const int r = p * RP + wave * RWV + rl, from = st % CH * PASS + p;
-            const int64_t offs = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, from) << 32 | (uint32_t)__builtin_amdgcn_readlane(lo, from));
+            const int r = p * RP + wave * RWV + rl;
+            const int64_t off = group(t - t0, p);
             uint4v k = {0, 0, 0, 0}, v = {0, 0, 0, 0};
-            if (offs >= 0 && TS * t + r < q.n) {
-                const size_t at = (size_t)offs + (size_t)(r % 16) * ss + 8 * pl;
+            if (off >= 0 && TS * t + r < q.n) {
+                const size_t at = (size_t)off + (size_t)(r % 16) * ss + 8 * pl;
                 k = *(const uint4v *)(kp + at);
                 v = *(const uint4v *)(vp + at);
             }
@@ -212,19 +222,22 @@ __global__ __launch_bounds__(64 * WAVES, QF && D == 256 ? 1 : 2) void k_prompt(P
             *(uint4v *)(lds + buf + STAGE + r * ROW + (pl ^ fv(r)) * 16) = v;
         }
     };
-    // Waits until stage t has arrived; the one two before it is no longer read then, and its place takes stage t + kStages - 2. Loads
-    // come back in order, 2 PASS of each stage: the younger one may be on its way (a stage through registers has waited for all
-    // before it; other loads make the wait longer, never shorter).
+    // which groups of tile t have a page
+    auto present = [&](int t) { return (uint32_t)(t - t0 >= c0 ? here >> (t - t0 - c0) * KS : before >> (t - t0 - c0 + CH) * KS) & ((1u << KS) - 1); };
+    // Waits until the wave's part of stage t has arrived; a barrier then tells of the others'. Loads come back in order, 2 PASS of
+    // each stage: younger stages may be on their way (a stage through registers has waited for all before it; other loads make
+    // the wait longer, never shorter).
     int loaded = t0;
     auto arrive = [&](int t) {
-        if (t + 1 < t1 && loaded > t + 1) __asm__ volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * PASS) : "memory");
+        if (loaded > t + 2) __asm__ volatile("s_waitcnt vmcnt(%0)" ::"n"(4 * PASS) : "memory");
+        else if (loaded > t + 1) __asm__ volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * PASS) : "memory");
         else __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
         if (t >= td && t < t1) {   // some of the slots may be hidden from some rows: infinities and NaN among the wave's values
             bool any = false;
 #pragma unroll 1
             for (int p = 0; p < PASS; ++p) {
                 const int r = p * RP + wave * RWV + rl;
-                uint4v *at = (uint4v *)(lds + ((t - t0) % kStages) * 2 * STAGE + STAGE + r * ROW + pl * 16);
+                uint4v *at = (uint4v *)(lds + (uint32_t)(t - t0) % kStages * 2 * STAGE + STAGE + r * ROW + pl * 16);
                 uint4v v = *at;
                 bool has = false;
 #pragma unroll
@@ -235,19 +248,16 @@ __global__ __launch_bounds__(64 * WAVES, QF && D == 256 ? 1 : 2) void k_prompt(P
                 }
                 const uint64_t by = __ballot(has);
                 if (by) *at = v;
-                if (pl == 0) odd_row[(t - t0) % 8][r] = (by >> (rl * PC) & (PC == 64 ? ~0ull : (1ull << PC) - 1)) != 0;
+                if (pl == 0) odd_row[(uint32_t)(t - t0) % 8][r] = (by >> (rl * PC) & (PC == 64 ? ~0ull : (1ull << PC) - 1)) != 0;
                 any |= by != 0;
             }
-            if (lane == 0) any_odd[(t - t0) % 8][wave] = any;
+            if (lane == 0) any_odd[(uint32_t)(t - t0) % 8][wave] = any;
         }
         __syncthreads();
-#pragma unroll 1
-        for (; loaded < min(t1, t + kStages - 1); ++loaded) load(loaded);
     };
-    if (t0 < t1) {
+    const int grp = PING ? wave >> 2 : 0, next = 2 + grp;   // a turn loads the stage so many behind its own
 #pragma unroll 1
-        for (; loaded < min(t1, t0 + 2); ++loaded) load(loaded);
-    }
+    for (; loaded < min(t1, t0 + next); ++loaded) load(loaded);
 
     // ---- the wave's rows: queries, last slot that each sees
     uint4v qf[NR][QP][C];
@@ -313,7 +323,7 @@ __global__ __launch_bounds__(64 * WAVES, QF && D == 256 ? 1 : 2) void k_prompt(P
 
     const int k_at = ln * ROW + ((g ^ fk(ln)) * 16);   // pieces 2 c + g: c only flips higher bits
     const int tl = lane & 15, v_row = 4 * g + (tl >> 2), v_at = v_row * ROW + ((((lane >> 4 & 1) * 2 + (tl >> 1 & 1)) ^ fv(v_row)) * 16) + 8 * (tl & 1);
-    auto place = [&](int t) { return lds + ((t - t0) % kStages) * 2 * STAGE; };
+    auto place = [&](int t) { return lds + (uint32_t)(t - t0) % kStages * 2 * STAGE; };
     auto qk = [&](const char *k, float16v (&x)[NR][SUB]) {
 #pragma unroll
         for (int a = 0; a < NR; ++a)
@@ -400,10 +410,7 @@ __global__ __launch_bounds__(64 * WAVES, QF && D == 256 ? 1 : 2) void k_prompt(P
         for (int a = 0; a < NR; ++a) l[a] += sum[a];
     };
     // hides what a row does not see: later tokens' slots, those without a page
-    auto hide = [&](int t, float16v (&x)[NR][SUB]) {
-        int pg[KS];
-#pragma unroll
-        for (int k = 0; k < KS; ++k) pg[k] = __builtin_amdgcn_readfirstlane(paged[(t - t0) % 8][k]);
+    auto hide = [&](int t, uint32_t pg, float16v (&x)[NR][SUB]) {
 #pragma unroll
         for (int a = 0; a < NR; ++a) {
             const int see = lim[a] - TS * t - 4 * g;
@@ -411,7 +418,7 @@ __global__ __launch_bounds__(64 * WAVES, QF && D == 256 ? 1 : 2) void k_prompt(P
             for (int u = 0; u < SUB; ++u)
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    const int upto = pg[2 * u + half] ? see : -1;
+                    const int upto = pg >> (2 * u + half) & 1 ? see : -1;
 #pragma unroll
                     for (int e = 8 * half; e < 8 * half + 8; ++e) x[a][u][e] = 32 * u + 8 * (e / 4) + e % 4 > upto ? -INFINITY : x[a][u][e];
                     __builtin_amdgcn_sched_barrier(0);
@@ -426,12 +433,14 @@ __global__ __launch_bounds__(64 * WAVES, QF && D == 256 ? 1 : 2) void k_prompt(P
             e[half] = __builtin_bit_cast(uint2v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)(v + (v_at ^ 64 * t) + (16 * ks + 8 * half) * ROW)));
         return uint4v{e[0][0], e[0][1], e[1][0], e[1][1]};
     };
+    constexpr int AHEAD = 4, EARLY = 4;   // operands that are read ahead of their products; of V before the barrier in front of them
+    uint4v first[EARLY];
     auto pv = [&](const char *v, const uint4v (&p)[NR][KS][PP]) {
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
             for (int t = 0; t < DT; ++t) {
-                const uint4v e = vt(v, t, ks);
+                const uint4v e = ks * DT + t < EARLY ? first[ks * DT + t] : vt(v, t, ks);
 #pragma unroll
                 for (int n = PP - 1; n >= 0; --n)
 #pragma unroll
@@ -441,7 +450,7 @@ __global__ __launch_bounds__(64 * WAVES, QF && D == 256 ? 1 : 2) void k_prompt(P
     // Adds the odd values of a stage's slots, which are zeros there, to the rows that see them.
     auto add_odd = [&](int t) {
         for (int j = 0; j < TS; ++j) {
-            if (!__builtin_amdgcn_readfirstlane(odd_row[(t - t0) % 8][j])) continue;
+            if (!__builtin_amdgcn_readfirstlane(odd_row[(uint32_t)(t - t0) % 8][j])) continue;
             const int slot = TS * t + j;
             const uint16_t *p = vp + slot_offset(c, s, slot) + 4 * g;
 #pragma unroll
@@ -464,19 +473,19 @@ __global__ __launch_bounds__(64 * WAVES, QF && D == 256 ? 1 : 2) void k_prompt(P
 
     float16v x[NR][SUB];
     uint4v p[NR][KS][PP];
-    auto phase_s = [&](int t) {
-        int pages = 1;
-#pragma unroll
-        for (int k = 0; k < KS; ++k) pages &= paged[(t - t0) % 8][k];
-        if (TS * t + TS - 1 > least || !__builtin_amdgcn_readfirstlane(pages)) hide(t, x);
+    auto weigh = [&](int t) {
         softmax(x, p);
+#pragma unroll
+        for (int i = 0; i < EARLY; ++i) first[i] = vt(place(t) + STAGE, i % DT, i / DT);
     };
-    auto phase_m = [&](int t) {
+    // products of the tile's weights and values, then the scores of the next
+    auto multiply = [&](int t, int next) {
+        __builtin_amdgcn_s_setprio(1);
         pv(place(t) + STAGE, p);
-        qk(place(min(t + 1, tw - 1)), x);   // (of the last tile once more: not used)
+        qk(place(next), x);
         if constexpr (QP == 1) {   // operands from LDS some products ahead, no more of them than registers
-            constexpr int AHEAD = D == 256 ? 4 : 8, NV = KS * DT, NK = SUB * C;
-            __builtin_amdgcn_sched_group_barrier(0x100, 2 * AHEAD, 0);
+            constexpr int NV = KS * DT, NK = SUB * C;
+            __builtin_amdgcn_sched_group_barrier(0x100, 2 * (AHEAD - EARLY), 0);
 #pragma unroll
             for (int i = 0; i < NV + NK; ++i) {
                 __builtin_amdgcn_sched_group_barrier(0x8, NR, 0);
@@ -485,35 +494,71 @@ __global__ __launch_bounds__(64 * WAVES, QF && D == 256 ? 1 : 2) void k_prompt(P
             }
         }
         __builtin_amdgcn_sched_barrier(0);
-        if (t >= td) {
-            int any = 0;
-#pragma unroll
-            for (int w = 0; w < WAVES; ++w) any |= any_odd[(t - t0) % 8][w];
-            if (__builtin_amdgcn_readfirstlane(any)) add_odd(t);
-        }
+        __builtin_amdgcn_s_setprio(0);
+    };
+    // A turn is weights, then products, with a barrier after each where two waves share a SIMD: there the second four waves are
+    // half a turn behind, so that one of the two makes weights while the other multiplies. At the barrier in the middle of
+    // turn t of the first four, which is at the end of turn t - 1 of the others, stage t + 1 has arrived and t - 1 is no longer
+    // read: its place takes stage t + 3 at the next turn that begins, t + 1 of the first four and t of the others.
+    auto start = [&](int t) {
+        if (t + next < t1) load(t + next), loaded = t + next + 1;
+    };
+    auto middle = [&](int t) {
+        if (grp) __syncthreads();
+        else arrive(t + 1);
+    };
+    auto end = [&](int t) {
+        if (!PING) return;
+        if (grp) arrive(t + 2);
+        else __syncthreads();
     };
     if (t0 < t1) {
         arrive(t0);
         if (t0 < tw) qk(place(t0), x);
-        // With two waves a SIMD of the compute unit, one makes weights while the other multiplies: the second four waves are half a
-        // turn behind, and a barrier follows each half. Stages arrive at the first's middles.
-        const int grp = PING ? wave >> 2 : 0;
         if (grp) arrive(t0 + 1);
-        auto halves = [&](int n) {   // the barrier after half n
-            if (!PING && (n & 1)) return;
-            if ((n & 1) ^ grp) __syncthreads();
-            else arrive(t0 + 1 + ((n + grp) >> 1));
-        };
         int t = t0;
 #pragma unroll 1
-        for (; t < tw; ++t) {
-            phase_s(t);
-            halves(2 * (t - t0));
-            phase_m(t);
-            halves(2 * (t - t0) + 1);
+        while (t < tw) {
+            start(t);
+            const uint32_t pg = present(t);
+            if (TS * t + TS - 1 > least || pg != (1u << KS) - 1) hide(t, pg, x);
+            weigh(t);
+            middle(t);
+            multiply(t, min(t + 1, tw - 1));   // (of the last tile its own scores once more: not used)
+            if (t >= td) {
+                int any = 0;
+#pragma unroll
+                for (int w = 0; w < WAVES; ++w) any |= any_odd[(uint32_t)(t - t0) % 8][w];
+                if (__builtin_amdgcn_readfirstlane(any)) add_odd(t);
+            }
+            end(t);
+            ++t;
+            // The turns without any of that: all rows have a reference and see all of the tile, pages are there, and there is a stage
+            // that goes straight to LDS with each.
+            if (!settled || (t - t0 < c0 && ~before)) continue;
+            const int run = min(min(td - 2, min(t1, q.n / TS) - next), t0 + c0 - next + (~here ? __builtin_ctzll(~here) : 64) / KS);
+#pragma unroll 1
+            for (; t < run; ++t) {
+#pragma unroll
+                for (int i = 0; i < 2 * PASS; ++i) load_direct(t + next, i);
+                loaded = t + next + 1;
+                weigh(t);
+                __asm__ volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * PASS) : "memory");
+                __syncthreads();
+                multiply(t, t + 1);
+                if constexpr (PING) {
+                    __asm__ volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * PASS) : "memory");
+                    __syncthreads();
+                }
+            }
         }
 #pragma unroll 1
-        for (int n = 2 * (t - t0); n < 2 * (t1 - t0) + (PING && !grp); ++n) halves(n);
+        for (; t < t1; ++t) {
+            start(t);
+            middle(t);
+            end(t);
+        }
+        if (PING && !grp) __syncthreads();
     }
 
     float *rec = J.part + (size_t)blockIdx.x * ROWS * (D + 2);
