@@ -44,11 +44,11 @@ struct PromptJob {
     float *lse;
     float *part;   // a record of each workgroup of a split segment: rows x D sums, then rows x (m, l)
     int heads_wg;  // workgroups of a key/value head
-    int split, least;   // segments may be split over workgroups, into parts of at least so many tiles
+    int split;     // segments may be split over workgroups
 };
 
-// the sequences' share of a head's workgroups: sequence s has rts row tiles (segments) of at most `tiles` tiles of slots, each
-// cut into `parts`
+// A sequence's share of a head's workgroups: it has rts row tiles (segments) of at most `tiles` tiles of slots, each cut into
+// `parts`.
 struct PromptSeq { int nt, n, first, rts, tiles, parts; };
 
 __device__ __forceinline__ int wave_total(int v) {
@@ -68,21 +68,37 @@ __device__ __forceinline__ PromptSeq prompt_seq(const PromptJob &J, int s, int p
     return q;
 }
 
-// tiles of a part, the least that fits a head's workgroups (0: segments whole)
+// Tiles of a part, the least that fits a head's workgroups (0: segments whole). Records and their join cost what kJoinTiles tiles do:
+// where no segment would get shorter by more, they stay whole (512 tokens in two parts 26.2 us, whole 25.6; 16 tiles in 2 to 8 parts, one
+// token, 24.0 to 19.7).
+constexpr int kJoinTiles = 6;
 template <int ROWS, int TS>
 __device__ __forceinline__ int prompt_per(const PromptJob &J) {
     if (!J.split) return 0;
     const int lane = threadIdx.x & 63;
-    auto over = [&](auto f) {   // f(sequence) summed
-        int t = 0;
-        for (int s0 = 0; s0 < J.c.n_seq; s0 += 64) t += wave_total(f(s0 + lane));
-        return t;
-    };
-    const int tiles = over([&](int s) { const PromptSeq q = prompt_seq<ROWS, TS>(J, s, 0); return q.rts * q.tiles; });
-    int per = max(J.least, (tiles + J.heads_wg - 1) / J.heads_wg);
-    // (there are at least twice as many workgroups as segments: twice the first `per` always fits)
-    while (over([&](int s) { const PromptSeq q = prompt_seq<ROWS, TS>(J, s, per); return q.rts * q.parts; }) > J.heads_wg) per += (per + 7) / 8;
-    return per;
+    int most = 0, per;
+    if (J.c.n_seq == 1) {
+        const PromptSeq q = prompt_seq<ROWS, TS>(J, 0, 0);
+        if (q.rts == 0) return 0;
+        const int parts = J.heads_wg / q.rts;
+        most = q.tiles, per = max(1, (q.tiles + parts - 1) / parts);
+    } else {
+        auto over = [&](auto f) {   // f(sequence) summed
+            int t = 0;
+            for (int s0 = 0; s0 < J.c.n_seq; s0 += 64) t += wave_total(f(s0 + lane));
+            return t;
+        };
+        const int tiles = over([&](int s) {
+            const PromptSeq q = prompt_seq<ROWS, TS>(J, s, 0);
+            most = max(most, q.rts ? q.tiles : 0);
+            return q.rts * q.tiles;
+        });
+        for (int o = 32; o; o >>= 1) most = max(most, __shfl_xor(most, o));
+        per = max(1, (tiles + J.heads_wg - 1) / J.heads_wg);
+        // (there are at least twice as many workgroups as segments: twice the first `per` always fits)
+        while (over([&](int s) { const PromptSeq q = prompt_seq<ROWS, TS>(J, s, per); return q.rts * q.parts; }) > J.heads_wg) per += (per + 7) / 8;
+    }
+    return __builtin_amdgcn_readfirstlane(most - per <= kJoinTiles ? 0 : per);
 }
 
 // The segment x (of a head's, all sequences' in a row; `part` of it when they are counted in parts): its sequence's numbers, s = -1
@@ -90,30 +106,38 @@ __device__ __forceinline__ int prompt_per(const PromptJob &J) {
 template <int ROWS, int TS>
 __device__ __forceinline__ PromptSeq prompt_find(const PromptJob &J, int per, bool in_parts, int x, int &s, int &rt, int &part) {
     const int lane = threadIdx.x & 63;
-    int base = 0;
-    s = -1, rt = part = 0;
     PromptSeq r{};
-    for (int s0 = 0; s0 < J.c.n_seq; s0 += 64) {
-        const PromptSeq q = prompt_seq<ROWS, TS>(J, s0 + lane, per);
-        const int v = q.rts * (in_parts ? q.parts : 1);
-        int y = v;
-        for (int o = 1; o < 64; o <<= 1) {
-            const int z = __shfl_up(y, o);
-            if (lane >= o) y += z;
+    int i = x;   // among the sequence's
+    s = -1, rt = part = 0;
+    if (J.c.n_seq == 1) {
+        r = prompt_seq<ROWS, TS>(J, 0, per);
+        if (x < r.rts * (in_parts ? r.parts : 1)) s = 0;
+    } else {
+        for (int s0 = 0, base = 0; s0 < J.c.n_seq && s < 0; s0 += 64) {
+            const PromptSeq q = prompt_seq<ROWS, TS>(J, s0 + lane, per);
+            const int v = q.rts * (in_parts ? q.parts : 1);
+            int y = v;
+            for (int o = 1; o < 64; o <<= 1) {
+                const int z = __shfl_up(y, o);
+                if (lane >= o) y += z;
+            }
+            const uint64_t in = __ballot(base + y > x);
+            if (in) {
+                const int f = __ffsll((unsigned long long)in) - 1;
+                auto of = [&](int a) { return __builtin_amdgcn_readlane(a, f); };
+                r = PromptSeq{of(q.nt), of(q.n), of(q.first), of(q.rts), of(q.tiles), of(q.parts)};
+                s = s0 + f;
+                i = x - base - of(y - v);
+            }
+            base += __builtin_amdgcn_readlane(y, 63);
         }
-        const uint64_t in = __ballot(base + y > x);
-        if (in) {
-            const int f = __ffsll((unsigned long long)in) - 1;
-            auto of = [&](int a) { return __builtin_amdgcn_readlane(a, f); };
-            r = PromptSeq{of(q.nt), of(q.n), of(q.first), of(q.rts), of(q.tiles), of(q.parts)};
-            s = s0 + f;
-            const int i = x - base - of(y - v);
-            part = in_parts ? i % r.parts : 0;
-            rt = r.rts - 1 - (in_parts ? i / r.parts : i);   // the longest first
-            return r;
-        }
-        base += __builtin_amdgcn_readlane(y, 63);
     }
+    if (s < 0) return r;
+    if (in_parts && r.parts > 1) {
+        part = i % r.parts;
+        i /= r.parts;
+    }
+    rt = r.rts - 1 - i;   // the longest first
     return r;
 }
 
@@ -619,27 +643,34 @@ __global__ __launch_bounds__(256) void k_prompt_join(PromptJob J) {
     }
 }
 
-// Rows of a workgroup: 8 waves of 32 rows; 4 waves where that leaves compute units without one, and where rows of 256 elements
-// or queries of several parts take more than 256 registers a lane.
-struct PromptPlan { int waves, rows, segs, heads_wg; size_t rec_bytes; };
+// Rows of a workgroup: 8 waves of 32 rows, two a SIMD; 4 waves where too few compute units would get such a workgroup (but half of
+// them will do where the context is long and segments are cut in two), and where rows of 256 elements and queries of several
+// parts together take more than 256 registers a lane. Segments are split where a head has at most half as many as workgroups for
+// it. (Equal shares of all tiles in a row, cut anywhere, balance better but read K and V at as many places at once as there are
+// workgroups, which the L2s do not hold: 95 against 72 us at 2048 tokens, 1086 against 604 at 2 x 8190 slots of 256 elements.)
+struct PromptPlan { int waves, rows, segs, heads_wg; bool split; size_t rec_bytes; };
 static PromptPlan prompt_plan(const KvDev &c, const DraftDev &d, int D) {
     PromptPlan p;
     auto segs = [&](int rows) {   // of a head: row tiles of all sequences, at most
         const int64_t each = ((int64_t)d.max_tokens * d.G + rows - 1) / rows, all = (int64_t)d.n_tokens * d.G / rows + std::min(c.n_seq, d.n_tokens);
         return std::min(each * c.n_seq, all);
     };
-    p.waves = (D == 256 && d.q_f32) || segs(256) * c.n_kv < num_cus() ? 4 : 8;
+    const int cus = num_cus(), tiles = c.max_len / tile_slots(D, c.bf16, d.q_f32) + 1;
+    p.waves = (D == 256 && d.q_f32) || segs(256) * c.n_kv < (tiles > 32 ? cus / 2 : cus) ? 4 : 8;
     p.rows = 32 * p.waves;
     const int64_t n = segs(p.rows);
     p.segs = (int)std::min<int64_t>(n, INT32_MAX);
-    p.heads_wg = num_cus() / c.n_kv;   // when they are split
+    // Several sequences of few rows, whose records are small: parts in three rounds, so that long and short ones even out (24
+    // sequences of one token and 400 to 4000 slots, 8 heads of 128: whole 97 us, so 80).
+    p.heads_wg = cus / c.n_kv * (c.n_seq > 1 && (int64_t)d.max_tokens * d.G <= 64 ? 3 : 1);
+    p.split = p.heads_wg >= 2 * n && tiles > kJoinTiles + 1;
     p.rec_bytes = 4 * (size_t)p.rows * (D + 2);
     return p;
 }
 
 size_t attn_prompt_workspace(const KvDev &c, const DraftDev &d, int D) {
     const PromptPlan p = prompt_plan(c, d, D);
-    return p.heads_wg >= 2 * p.segs ? (size_t)p.heads_wg * c.n_kv * p.rec_bytes : 0;
+    return p.split ? (size_t)p.heads_wg * c.n_kv * p.rec_bytes : 0;
 }
 
 template <int D, bool BF, bool QF, int WAVES>
@@ -667,9 +698,9 @@ int launch_attn_prompt(const KvDev &c, const DraftDev &d, int D, void *out, int 
     const PromptPlan p = prompt_plan(c, d, D);
     if ((int64_t)p.segs * c.n_kv > INT32_MAX || (int64_t)d.max_tokens * d.G > INT32_MAX)
         return set_error(P8X_ERR_UNSUPPORTED, "p8x_attn_prompt: %d row tiles of %d heads, %d tokens of %d heads", p.segs, c.n_kv, d.max_tokens, d.G);
-    PromptJob J{c, d, out, ldo, hso, out_dtype, lse, (float *)ws, p.segs, 0, 4};
+    PromptJob J{c, d, out, ldo, hso, out_dtype, lse, (float *)ws, p.segs, 0};
     const int room = (int)std::min<size_t>(p.heads_wg, ws_bytes / p.rec_bytes / c.n_kv);
-    if (room >= 2 * p.segs) J.split = 1, J.heads_wg = room;
+    if (p.split && room >= 2 * p.segs) J.split = 1, J.heads_wg = room;
     if (D == 64) return c.bf16 ? prompt_types<64, true>(J, p, st) : prompt_types<64, false>(J, p, st);
     if (D == 128) return c.bf16 ? prompt_types<128, true>(J, p, st) : prompt_types<128, false>(J, p, st);
     return c.bf16 ? prompt_types<256, true>(J, p, st) : prompt_types<256, false>(J, p, st);
