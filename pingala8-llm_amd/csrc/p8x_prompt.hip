@@ -51,8 +51,13 @@ struct PromptJob {
 // `parts`.
 struct PromptSeq { int nt, n, first, rts, tiles, parts; };
 
-__device__ __forceinline__ int wave_total(int v) {
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+// sum and largest of what the first n lanes have (n at most 64; the others 0)
+__device__ __forceinline__ int first_total(int v, int n) {
+    for (int o = 1; o < min(n, 64); o <<= 1) v += __shfl_xor(v, o);
+    return __builtin_amdgcn_readfirstlane(v);
+}
+__device__ __forceinline__ int first_most(int v, int n) {
+    for (int o = 1; o < min(n, 64); o <<= 1) v = max(v, __shfl_xor(v, o));
     return __builtin_amdgcn_readfirstlane(v);
 }
 
@@ -85,7 +90,7 @@ __device__ __forceinline__ int prompt_per(const PromptJob &J) {
     } else {
         auto over = [&](auto f) {   // f(sequence) summed
             int t = 0;
-            for (int s0 = 0; s0 < J.c.n_seq; s0 += 64) t += wave_total(f(s0 + lane));
+            for (int s0 = 0; s0 < J.c.n_seq; s0 += 64) t += first_total(f(s0 + lane), J.c.n_seq);
             return t;
         };
         const int tiles = over([&](int s) {
@@ -93,12 +98,12 @@ __device__ __forceinline__ int prompt_per(const PromptJob &J) {
             most = max(most, q.rts ? q.tiles : 0);
             return q.rts * q.tiles;
         });
-        for (int o = 32; o; o >>= 1) most = max(most, __shfl_xor(most, o));
+        most = first_most(most, J.c.n_seq);
         per = max(1, (tiles + J.heads_wg - 1) / J.heads_wg);
         // (there are at least twice as many workgroups as segments: twice the first `per` always fits)
         while (over([&](int s) { const PromptSeq q = prompt_seq<ROWS, TS>(J, s, per); return q.rts * q.parts; }) > J.heads_wg) per += (per + 7) / 8;
     }
-    return __builtin_amdgcn_readfirstlane(most - per <= kJoinTiles ? 0 : per);
+    return most - per <= kJoinTiles ? 0 : per;
 }
 
 // The segment x (of a head's, all sequences' in a row; `part` of it when they are counted in parts): its sequence's numbers, s = -1
@@ -117,7 +122,7 @@ __device__ __forceinline__ PromptSeq prompt_find(const PromptJob &J, int per, bo
             const PromptSeq q = prompt_seq<ROWS, TS>(J, s0 + lane, per);
             const int v = q.rts * (in_parts ? q.parts : 1);
             int y = v;
-            for (int o = 1; o < 64; o <<= 1) {
+            for (int o = 1; o < min(J.c.n_seq, 64); o <<= 1) {   // (lanes behind the last sequence add nothing)
                 const int z = __shfl_up(y, o);
                 if (lane >= o) y += z;
             }
@@ -129,7 +134,7 @@ __device__ __forceinline__ PromptSeq prompt_find(const PromptJob &J, int per, bo
                 s = s0 + f;
                 i = x - base - of(y - v);
             }
-            base += __builtin_amdgcn_readlane(y, 63);
+            base += __builtin_amdgcn_readlane(y, min(J.c.n_seq - s0, 64) - 1);
         }
     }
     if (s < 0) return r;
@@ -621,7 +626,7 @@ __global__ __launch_bounds__(256) void k_prompt_join(PromptJob J) {
     int before = 0;
     for (int s0 = 0; s0 < s; s0 += 64) {
         const PromptSeq p = prompt_seq<ROWS, TS>(J, s0 + (threadIdx.x & 63), per);
-        before += wave_total(s0 + (int)(threadIdx.x & 63) < s ? p.rts * p.parts : 0);
+        before += first_total(s0 + (int)(threadIdx.x & 63) < s ? p.rts * p.parts : 0, J.c.n_seq);
     }
     const int b0 = before + (q.rts - 1 - rt) * q.parts;
     const int rows = min(ROWS, q.nt * J.d.G - rt * ROWS);
@@ -643,9 +648,9 @@ __global__ __launch_bounds__(256) void k_prompt_join(PromptJob J) {
     }
 }
 
-// Rows of a workgroup: 8 waves of 32 rows, two a SIMD; 4 waves where too few compute units would get such a workgroup (but half of
-// them will do where the context is long and segments are cut in two), and where rows of 256 elements and queries of several
-// parts together take more than 256 registers a lane. Segments are split where a head has at most half as many as workgroups for
+// Rows of a workgroup: 8 waves of 32 rows, two a SIMD; 4 waves where sequences have no more rows than those, where contexts are short and too
+// few compute units would get a workgroup of 8 (long ones are cut: 2 x 325 tokens of 8 heads a group over 49909 slots 533 us with 4,
+// %W8 with 8), and where rows of 256 elements and queries of several parts together take more than 256 registers a lane. Segments are split where a head has at most half as many as workgroups for
 // it. (Equal shares of all tiles in a row, cut anywhere, balance better but read K and V at as many places at once as there are
 // workgroups, which the L2s do not hold: 95 against 72 us at 2048 tokens, 1086 against 604 at 2 x 8190 slots of 256 elements.)
 struct PromptPlan { int waves, rows, segs, heads_wg; bool split; size_t rec_bytes; };
@@ -656,7 +661,7 @@ static PromptPlan prompt_plan(const KvDev &c, const DraftDev &d, int D) {
         return std::min(each * c.n_seq, all);
     };
     const int cus = num_cus(), tiles = c.max_len / tile_slots(D, c.bf16, d.q_f32) + 1;
-    p.waves = (D == 256 && d.q_f32) || segs(256) * c.n_kv < (tiles > 32 ? cus / 2 : cus) ? 4 : 8;
+    p.waves = (D == 256 && d.q_f32) || (int64_t)d.max_tokens * d.G <= 128 || (tiles <= 32 && segs(256) * c.n_kv < cus) ? 4 : 8;
     p.rows = 32 * p.waves;
     const int64_t n = segs(p.rows);
     p.segs = (int)std::min<int64_t>(n, INT32_MAX);
@@ -679,7 +684,10 @@ static int prompt_run(const PromptJob &J, int segs, hipStream_t st) {
     static OncePerDevice once;
     if (int rc = allow_lds(once, (const void *)k_prompt<D, BF, QF, 1, WAVES>, lds, "p8x_attn_prompt LDS")) return rc;
     k_prompt<D, BF, QF, 1, WAVES><<<J.heads_wg * J.c.n_kv, 64 * WAVES, lds, st>>>(J);
-    if (J.split) k_prompt_join<D, TS, ROWS><<<dim3(segs * J.c.n_kv, 8), 256, 0, st>>>(J);
+    if (J.split) {   // a pass of 256 threads for a row tile's pieces, up to 8 of them side by side
+        const int64_t pieces = std::min<int64_t>(ROWS, (int64_t)J.d.max_tokens * J.d.G) * (D / 4);
+        k_prompt_join<D, TS, ROWS><<<dim3(segs * J.c.n_kv, (unsigned)std::min<int64_t>(8, (pieces + 255) / 256)), 256, 0, st>>>(J);
+    }
     return hip_check(hipGetLastError(), "p8x_attn_prompt launch");
 }
 

@@ -1,13 +1,13 @@
 """Greedy decoding with drafted tokens on a cache of bounded size: the calls between the linears as a decode step uses them.
 
-A transformer with random Pingala-8 weights (each layer: norm -> q, k, v -> attention of the drafted tokens -> o -> norm ->
-gate, up, silu -> down; norms before and after each block, no rotary embedding) decodes one sequence. Every step runs a small
+A transformer with random Pingala-8 weights (each layer: norm -> q, k, v, with --rope-base rotated by their positions -> attention of
+the drafted tokens -> o -> norm -> gate, up, silu -> down; norms before and after each block) decodes one sequence. Every step runs a small
 tree of tokens -- the last one and guesses of what follows, looked up from earlier occurrences -- through all layers at
-once (p8x_norm_residual, p8x_mul_mat_vec, p8x_attn_tree), keeps the path that the model itself would have taken, adds what it
+once (p8x_norm_residual, p8x_mul_mat_vec, p8x_rope, p8x_attn_tree), keeps the path that the model itself would have taken, adds what it
 attended to to the slots' scores (p8x_kv_score), stores its keys and values (p8x_kv_append) and cuts the cache to its budget
 (p8x_kv_evict: the first positions, the last ones and the highest scores stay).
 
-    python -m p8x.tree_decode [--layers 4] [--tokens 96] [--budget 64] [--drafts 8]
+    python -m p8x.tree_decode [--layers 4] [--tokens 96] [--budget 64] [--drafts 8] [--rope-base 10000]
 
 prints tokens, steps and milliseconds a step (calls enqueued one by one; the host chooses between steps).
 """
@@ -22,9 +22,9 @@ MAX_COLUMNS = 8   # of p8x_mul_mat_vec: tokens of a step
 
 
 class Model:
-    """random weights: hidden and ffn multiples of 256, vocabulary a multiple of 32"""
+    """random weights: hidden and ffn multiples of 256, vocabulary a multiple of 32; rope_base 0: positions are not rotated in"""
 
-    def __init__(self, layers=4, hidden=512, heads=4, kv=2, head_dim=128, ffn=1024, vocab=512, seed=0):
+    def __init__(self, layers=4, hidden=512, heads=4, kv=2, head_dim=128, ffn=1024, vocab=512, seed=0, rope_base=0.0):
         self.hidden, self.heads, self.kv, self.D, self.ffn, self.vocab = hidden, heads, kv, head_dim, ffn, vocab
         rng = np.random.default_rng(seed)
         self.embedding = rng.standard_normal((vocab, hidden)).astype(np.float32)
@@ -39,6 +39,10 @@ class Model:
                        for _ in range(layers)]
         self.head = linears(hidden, head=vocab)["head"]
         self.one = p8x.DeviceBuffer.from_numpy(np.ones(hidden, np.float32))
+        self.rotation = None
+        if rope_base:
+            freq, amplitude = p8x.rope_frequencies(head_dim, rope_base)
+            self.rotation = p8x.Rotation(head_dim, p8x.DeviceBuffer.from_numpy(freq), amplitude=amplitude)
         # a norm that puts the products of random weights to the size that the next step expects
         self.half = p8x.DeviceBuffer.from_numpy(np.full(hidden, 0.5, np.float32))
 
@@ -84,7 +88,9 @@ class Decoder:
             at = L["qkv"].addr
             d = dict(n_tokens=n, max_tokens=n, first=self.first, q=at, k=at + 4 * m.heads * m.D, v=at + 4 * (m.heads + m.kv) * m.D, ld_q=self.ld,
                      ld_kv=self.ld, mask=self.mask, n_heads=m.heads, scale=m.D ** -0.5)
-            out.append(dict(attn=p8x.AttnTree(L["cache"], self.act, lse=L["lse"], **d),
+            rope = None if m.rotation is None else p8x.Rope(m.rotation, n, m.D, self.at, n_heads=m.heads, q=at, ld_q=self.ld, n_kv=m.kv,
+                                                            k=d["k"], ld_k=self.ld)   # in place
+            out.append(dict(rope=rope, attn=p8x.AttnTree(L["cache"], self.act, lse=L["lse"], **d),
                             score=p8x.KvScore(L["cache"], L["lse"], L["score"], accept=self.accept, decay=self.decay, **d),
                             append=p8x.KvAppend(L["cache"], accept=self.accept, at=self.at, pos=L["pos"], len_out=L["len"], **d)))
         return dict(layers=out, start=self._norm(n), add=self._norm(n, self.y))
@@ -109,6 +115,8 @@ class Decoder:
             at = L["qkv"].addr
             for name, off in (("q", 0), ("k", m.heads * m.D), ("v", (m.heads + m.kv) * m.D)):
                 w[name].mul_mat_vec_dev(self.x, at + 4 * off, n, ldy=self.ld, stream=stream)
+            if call["rope"]:
+                call["rope"].run(stream)
             call["attn"].run(stream)
             w["o"].mul_mat_vec_dev(self.act, self.y, n, stream=stream)
             c["add"].run(stream)
@@ -184,8 +192,9 @@ def main():
     ap = argparse.ArgumentParser(description=__doc__.split("\n")[0])
     for name, value in dict(layers=4, hidden=512, heads=4, kv=2, head_dim=128, ffn=1024, vocab=512, tokens=96, budget=64, drafts=8, seed=0).items():
         ap.add_argument("--" + name.replace("_", "-"), type=int, default=value)
+    ap.add_argument("--rope-base", type=float, default=0.0)
     a = ap.parse_args()
-    model = Model(a.layers, a.hidden, a.heads, a.kv, a.head_dim, a.ffn, a.vocab, a.seed)
+    model = Model(a.layers, a.hidden, a.heads, a.kv, a.head_dim, a.ffn, a.vocab, a.seed, a.rope_base)
     prompt = np.random.default_rng(a.seed).integers(0, a.vocab, 20).tolist()
     for drafts in (1, a.drafts):
         d = Decoder(model, a.budget)
