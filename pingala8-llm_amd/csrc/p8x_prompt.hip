@@ -119,7 +119,20 @@ __device__ __forceinline__ PromptSeq prompt_find(const PromptJob &J, int per, bo
         if (x < r.rts * (in_parts ? r.parts : 1)) s = 0;
     } else {
         for (int s0 = 0, base = 0; s0 < J.c.n_seq && s < 0; s0 += 64) {
-            const PromptSeq q = prompt_seq<ROWS, TS>(J, s0 + lane, per);
+            PromptSeq q = prompt_seq<ROWS, TS>(J, s0 + lane, per);
+            int id = s0 + lane;
+            if (!per && J.c.n_seq <= 64) {   // whole segments: those of the longest sequence first (16 of 400 to 4400 slots 165 us, in their order 195)
+                const int mine = q.rts ? q.tiles : 0;
+                int at = 0;
+                for (int j = 0; j < J.c.n_seq; ++j) {
+                    const int its = __builtin_amdgcn_readlane(mine, j);
+                    at += its > mine || (its == mine && j < lane);
+                }
+                if (lane >= J.c.n_seq) at = lane;
+                auto to = [&](int a) { return __builtin_amdgcn_ds_permute(4 * at, a); };
+                q = PromptSeq{to(q.nt), to(q.n), to(q.first), to(q.rts), to(q.tiles), to(q.parts)};
+                id = to(lane);
+            }
             const int v = q.rts * (in_parts ? q.parts : 1);
             int y = v;
             for (int o = 1; o < min(J.c.n_seq, 64); o <<= 1) {   // (lanes behind the last sequence add nothing)
@@ -131,7 +144,7 @@ __device__ __forceinline__ PromptSeq prompt_find(const PromptJob &J, int per, bo
                 const int f = __ffsll((unsigned long long)in) - 1;
                 auto of = [&](int a) { return __builtin_amdgcn_readlane(a, f); };
                 r = PromptSeq{of(q.nt), of(q.n), of(q.first), of(q.rts), of(q.tiles), of(q.parts)};
-                s = s0 + f;
+                s = of(id);
                 i = x - base - of(y - v);
             }
             base += __builtin_amdgcn_readlane(y, min(J.c.n_seq - s0, 64) - 1);
@@ -650,7 +663,7 @@ __global__ __launch_bounds__(256) void k_prompt_join(PromptJob J) {
 
 // Rows of a workgroup: 8 waves of 32 rows, two a SIMD; 4 waves where sequences have no more rows than those, where contexts are short and too
 // few compute units would get a workgroup of 8 (long ones are cut: 2 x 325 tokens of 8 heads a group over 49909 slots 533 us with 4,
-// %W8 with 8), and where rows of 256 elements and queries of several parts together take more than 256 registers a lane. Segments are split where a head has at most half as many as workgroups for
+// 386 with 8), and where rows of 256 elements and queries of several parts together take more than 256 registers a lane. Segments are split where a head has at most half as many as workgroups for
 // it. (Equal shares of all tiles in a row, cut anywhere, balance better but read K and V at as many places at once as there are
 // workgroups, which the L2s do not hold: 95 against 72 us at 2048 tokens, 1086 against 604 at 2 x 8190 slots of 256 elements.)
 struct PromptPlan { int waves, rows, segs, heads_wg; bool split; size_t rec_bytes; };
