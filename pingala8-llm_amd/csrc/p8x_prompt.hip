@@ -538,26 +538,25 @@ __global__ __launch_bounds__(64 * WAVES, QF && D == 256 ? 1 : 2) void k_prompt(P
         __builtin_amdgcn_sched_barrier(0);
         __builtin_amdgcn_s_setprio(0);
     };
-    // A turn is weights, then products, with a barrier after each where two waves share a SIMD: there the second four waves are
-    // half a turn behind, so that one of the two makes weights while the other multiplies. At the barrier in the middle of
-    // turn t of the first four, which is at the end of turn t - 1 of the others, stage t + 1 has arrived and t - 1 is no longer
-    // read: its place takes stage t + 3 at the next turn that begins, t + 1 of the first four and t of the others.
+    // A turn is weights, then products. One barrier a turn: at that of turn t stage t + 1 has arrived and t - 1 is no longer read. Where
+    // two waves share a SIMD it lies between weights and products for the first four waves and before the weights for the
+    // others, so that from one barrier to the next one of the two multiplies first and then makes weights, the other the other
+    // way round. The place of stage t - 1 takes stage t + 3 with the weights that follow the barrier, those of turn t + 1 of the first
+    // four waves and of turn t of the others.
     auto start = [&](int t) {
+        if (grp) arrive(t + 1);
         if (t + next < t1) load(t + next), loaded = t + next + 1;
     };
     auto middle = [&](int t) {
-        if (grp) __syncthreads();
-        else arrive(t + 1);
+        if (!grp) arrive(t + 1);
     };
-    auto end = [&](int t) {
-        if (!PING) return;
-        if (grp) arrive(t + 2);
-        else __syncthreads();
+    auto arrive_full = [&]() {
+        __asm__ volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * PASS) : "memory");
+        __syncthreads();
     };
     if (t0 < t1) {
         arrive(t0);
         if (t0 < tw) qk(place(t0), x);
-        if (grp) arrive(t0 + 1);
         int t = t0;
 #pragma unroll 1
         while (t < tw) {
@@ -573,7 +572,6 @@ __global__ __launch_bounds__(64 * WAVES, QF && D == 256 ? 1 : 2) void k_prompt(P
                 for (int w = 0; w < WAVES; ++w) any |= any_odd[(uint32_t)(t - t0) % 8][w];
                 if (__builtin_amdgcn_readfirstlane(any)) add_odd(t);
             }
-            end(t);
             ++t;
             // The turns without any of that: all rows have a reference and see all of the tile, pages are there, and there is a stage
             // that goes straight to LDS with each.
@@ -581,26 +579,20 @@ __global__ __launch_bounds__(64 * WAVES, QF && D == 256 ? 1 : 2) void k_prompt(P
             const int run = min(min(td - 2, min(t1, q.n / TS) - next), t0 + c0 - next + (~here ? __builtin_ctzll(~here) : 64) / KS);
 #pragma unroll 1
             for (; t < run; ++t) {
+                if (grp) arrive_full();
 #pragma unroll
                 for (int i = 0; i < 2 * PASS; ++i) load_direct(t + next, i);
                 loaded = t + next + 1;
                 weigh(t);
-                __asm__ volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * PASS) : "memory");
-                __syncthreads();
+                if (!grp) arrive_full();
                 multiply(t, t + 1);
-                if constexpr (PING) {
-                    __asm__ volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * PASS) : "memory");
-                    __syncthreads();
-                }
             }
         }
 #pragma unroll 1
         for (; t < t1; ++t) {
             start(t);
             middle(t);
-            end(t);
         }
-        if (PING && !grp) __syncthreads();
     }
 
     float *rec = J.part + (size_t)blockIdx.x * ROWS * (D + 2);
