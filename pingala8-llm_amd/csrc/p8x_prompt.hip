@@ -34,8 +34,8 @@ __device__ __forceinline__ float16v mfma32(uint4v a, uint4v b, float16v c) {
 // by its moving down
 constexpr float kUp = 8.0f, kRoom = 64.0f;
 constexpr int kStages = 4;   // in LDS: two in use (K of the next tile, V of this one), the others on their way
-// slots of a tile: fewer where the operands of 64 do not fit the registers
-__host__ __device__ constexpr int tile_slots(int D, bool bf, bool qf) { return D == 256 || (D == 128 && bf && qf) ? 32 : 64; }
+// slots of a tile: fewer where the operands of 64 do not fit the registers, or two rings of stages LDS
+__host__ __device__ constexpr int tile_slots(int D, bool bf, bool qf, bool halves) { return D == 256 || (D == 128 && ((bf && qf) || halves)) ? 32 : 64; }
 
 struct PromptJob {
     KvDev c;
@@ -52,9 +52,9 @@ struct PromptJob {
 struct PromptSeq { int nt, n, first, rts, tiles, parts; };
 
 // sum and largest of what the first n lanes have (n at most 64; the others 0)
-__device__ __forceinline__ int first_total(int v, int n) {
+__device__ __forceinline__ float first_total(float v, int n) {
     for (int o = 1; o < min(n, 64); o <<= 1) v += __shfl_xor(v, o);
-    return __builtin_amdgcn_readfirstlane(v);
+    return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v)));
 }
 __device__ __forceinline__ int first_most(int v, int n) {
     for (int o = 1; o < min(n, 64); o <<= 1) v = max(v, __shfl_xor(v, o));
@@ -73,37 +73,39 @@ __device__ __forceinline__ PromptSeq prompt_seq(const PromptJob &J, int s, int p
     return q;
 }
 
-// Tiles of a part, the least that fits a head's workgroups (0: segments whole). Records and their join cost what kJoinTiles tiles do:
-// where no segment would get shorter by more, they stay whole (512 tokens in two parts 26.2 us, whole 25.6; 16 tiles in 2 to 8 parts, one
-// token, 24.0 to 19.7).
-constexpr int kJoinTiles = 6;
-template <int ROWS, int TS>
+// Tiles of a part: as few as a head's workgroups allow, but the join costs what kRecord slots do for each record that it reads, so
+// that a longest segment of n slots is done first in parts of about sqrt(n * kRecord). Where no segment would get shorter by more
+// than kJoin, 0: they stay whole, and nothing is joined. COST: what a slot takes against one of 128 elements.
+constexpr int kRecord = 32, kLeast = 128, kJoin = 384;
+__host__ __device__ constexpr int slot_cost(int D) { return D == 256 ? 2 : 1; }
+template <int COST, int ROWS, int TS>
 __device__ __forceinline__ int prompt_per(const PromptJob &J) {
     if (!J.split) return 0;
     const int lane = threadIdx.x & 63;
+    auto least = [](int tiles) { return max(max(2, kLeast / COST / TS), (int)(__builtin_amdgcn_sqrtf((float)tiles * kRecord / COST / TS) + 0.5f)); };
     int most = 0, per;
     if (J.c.n_seq == 1) {
         const PromptSeq q = prompt_seq<ROWS, TS>(J, 0, 0);
         if (q.rts == 0) return 0;
         const int parts = J.heads_wg / q.rts;
-        most = q.tiles, per = max(1, (q.tiles + parts - 1) / parts);
+        most = q.tiles, per = max(least(most), (q.tiles + parts - 1) / parts);
     } else {
-        auto over = [&](auto f) {   // f(sequence) summed
-            int t = 0;
+        auto over = [&](auto f) {   // f(sequence) summed; in f32: products of long sequences pass 31 bits
+            float t = 0.0f;
             for (int s0 = 0; s0 < J.c.n_seq; s0 += 64) t += first_total(f(s0 + lane), J.c.n_seq);
             return t;
         };
-        const int tiles = over([&](int s) {
+        const float tiles = over([&](int s) {
             const PromptSeq q = prompt_seq<ROWS, TS>(J, s, 0);
             most = max(most, q.rts ? q.tiles : 0);
-            return q.rts * q.tiles;
+            return (float)q.rts * (float)q.tiles;
         });
         most = first_most(most, J.c.n_seq);
-        per = max(1, (tiles + J.heads_wg - 1) / J.heads_wg);
+        per = max(least(most), (int)(tiles / (float)J.heads_wg) + 1);
         // (there are at least twice as many workgroups as segments: twice the first `per` always fits)
-        while (over([&](int s) { const PromptSeq q = prompt_seq<ROWS, TS>(J, s, per); return q.rts * q.parts; }) > J.heads_wg) per += (per + 7) / 8;
+        while (over([&](int s) { const PromptSeq q = prompt_seq<ROWS, TS>(J, s, per); return (float)q.rts * (float)q.parts; }) > (float)J.heads_wg) per += (per + 7) / 8;
     }
-    return most - per <= kJoinTiles ? 0 : per;
+    return most - per <= kJoin / COST / TS ? 0 : per;
 }
 
 // The segment x (of a head's, all sequences' in a row; `part` of it when they are counted in parts): its sequence's numbers, s = -1
@@ -170,48 +172,55 @@ __device__ __forceinline__ void store_out(const PromptJob &J, int first, int h, 
     if (e == 0 && J.lse) J.lse[(size_t)(first + i) * J.c.n_kv * G + head] = l == 0.0f ? -INFINITY : (m - bias + __log2f(l)) * kLn2;
 }
 
-template <int D, bool BF, bool QF, int NR, int WAVES>
+// HALVES: the second four waves have the rows of the first, over the second half of the tiles, in a ring of stages of their own; the sums
+// of both meet in LDS at the end.
+template <int D, bool BF, bool QF, int NR, int WAVES, bool HALVES>
 __global__ __launch_bounds__(64 * WAVES, QF && D == 256 ? 1 : 2) void k_prompt(PromptJob J) {
-    constexpr int TS = tile_slots(D, BF, QF), SUB = TS / 32, C = D / 16, DT = D / 32, KS = TS / 16, PC = D / 8, ROW = 2 * D, ROWS = 32 * NR * WAVES;
+    constexpr int TS = tile_slots(D, BF, QF, HALVES), GW = HALVES ? WAVES / 2 : WAVES, SUB = TS / 32, C = D / 16, DT = D / 32, KS = TS / 16, PC = D / 8, ROW = 2 * D, ROWS = 32 * NR * GW;
     constexpr int QP = QF ? (BF ? 3 : 2) : 1, PP = QP;
     constexpr float kBias = BF ? 0.0f : 7.0f;
     // (fp16) log2 of a lane's sum of weights below which the tile's largest is looked up, and of that one below which m moves down
     constexpr float kLow = QF ? 5.0f : 10.0f, kDown = 10.0f;
     extern __shared__ float4v sh4[];
     constexpr bool PING = WAVES == 8;
-    __shared__ int odd_row[8][TS], any_odd[8][WAVES];   // slots with infinities or NaN among their values, of stages that some rows see in part; whether a wave found any
+    __shared__ int odd_rows[HALVES ? 2 : 1][8][TS], any_odds[HALVES ? 2 : 1][8][GW];   // slots with infinities or NaN among their values, of stages that some rows see in part; whether a wave found any
     const KvDev &c = J.c;
     const DraftDev &d = J.d;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 5, ln = lane & 31;
     const int h = blockIdx.x % c.n_kv;
     int s, rt, part;
-    const int per = prompt_per<ROWS, TS>(J);
+    const int per = prompt_per<slot_cost(D), ROWS, TS>(J);
     const PromptSeq q = prompt_find<ROWS, TS>(J, per, true, blockIdx.x / c.n_kv, s, rt, part);
     if (s < 0) return;
     const int G = d.G, rows = q.nt * G, rows_here = min(ROWS, rows - rt * ROWS), ahead = q.n - q.nt;   // slots before the tokens
     // tiles of the row tile's last token, and this part's
     const int tiles = (max(0, ahead + (rt * ROWS + rows_here - 1) / G + 1) + TS - 1) / TS;
     const int share = q.parts == 1 ? tiles : tiles / q.parts, more = tiles - share * q.parts;
-    const int t0 = part * share + min(part, more), t1 = t0 + share + (part < more);
+    const int p0 = part * share + min(part, more), p1 = p0 + share + (part < more), turns = HALVES ? (p1 - p0 + 1) / 2 : p1 - p0;
+    // the waves' half, and their number in it
+    const int half = HALVES ? wave >> 2 : 0, gw = HALVES ? wave & 3 : wave;
+    const int t0 = half ? p0 + turns : p0, t1 = half ? p1 : p0 + turns;
+    auto &odd_row = odd_rows[half];
+    auto &any_odd = any_odds[half];
     const uint16_t *kp = c.k + (size_t)h * c.head_stride, *vp = c.v + (size_t)h * c.head_stride;
     const uint32_t ss = (uint32_t)c.slot_stride;
     const int td = max(0, ahead + rt * ROWS / G + 1) / TS;   // the first tile that some row sees in part only
 
     // ---- K and V of stage t to LDS: straight there where all of the wave's rows are in use and have a page, else through
     // registers, rows that are not there as zeros
-    constexpr int RWV = 64 / PC, RP = WAVES * RWV, PASS = TS / RP;   // rows of a wave and of the workgroup in a pass
+    constexpr int RWV = 64 / PC, RP = GW * RWV, PASS = TS / RP;   // rows of a wave and of the workgroup in a pass
     constexpr int STAGE = TS * ROW;                                  // bytes of a stage's K; its V follows
     static_assert(PASS >= 1 && TS % RP == 0 && RWV <= 16, "passes");
     // 16-byte pieces of a row lie at p ^ fk(row) (K), p ^ fv(row) (V), so that a read's rows are in other banks
     auto fk = [](int row) { return PC < 16 ? row >> 1 & 7 : row & 15; };
     auto fv = [](int row) { return PC < 16 ? (row >> 1 & 1) << 2 : (row & 3) << 2; };
-    char *const lds = (char *)sh4;
+    char *const lds = (char *)sh4 + half * kStages * 2 * STAGE;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
     const int rl = lane / PC, pl = lane % PC;
     uint32_t kl[2], vl[2];   // the lane's bytes from its 16 slots' first
 #pragma unroll
     for (int p = 0; p < (RP % 16 ? 2 : 1); ++p) {
-        const int r15 = (p * RP + wave * RWV + rl) & 15;
+        const int r15 = (p * RP + gw * RWV + rl) & 15;
         kl[p] = 2 * (r15 * ss + 8 * (pl ^ fk(r15)));
         vl[p] = 2 * (r15 * ss + 8 * (pl ^ fv(r15)));
     }
@@ -228,12 +237,12 @@ __global__ __launch_bounds__(64 * WAVES, QF && D == 256 ? 1 : 2) void k_prompt(P
         here = __ballot(off >= 0);
     };
     auto group = [&](int st, int p) {   // where the 16 slots of the wave's rows of a pass lie
-        const int from = (st - c0) * KS + (p * RP + wave * RWV) / 16;
+        const int from = (st - c0) * KS + (p * RP + gw * RWV) / 16;
         return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, from) << 32 | (uint32_t)__builtin_amdgcn_readlane(lo, from));
     };
     auto load_direct = [&](int t, int i) {   // load i of 2 PASS
         const int p = i / 2;
-        const uint32_t to = lds0 + (uint32_t)(t - t0) % kStages * 2 * STAGE + (p * RP + wave * RWV) * ROW;
+        const uint32_t to = lds0 + (uint32_t)(t - t0) % kStages * 2 * STAGE + (p * RP + gw * RWV) * ROW;
         const int64_t off = group(t - t0, p);
         if (i % 2) load_lds(vp + off, vl[RP % 16 ? p & 1 : 0], to + STAGE);
         else load_lds(kp + off, kl[RP % 16 ? p & 1 : 0], to);
@@ -242,7 +251,7 @@ __global__ __launch_bounds__(64 * WAVES, QF && D == 256 ? 1 : 2) void k_prompt(P
         if ((t - t0) % CH == 0) pages(t - t0);
         bool direct = true;
 #pragma unroll
-        for (int p = 0; p < PASS; ++p) direct = direct && group(t - t0, p) >= 0 && TS * t + p * RP + wave * RWV + RWV <= q.n;
+        for (int p = 0; p < PASS; ++p) direct = direct && group(t - t0, p) >= 0 && TS * t + p * RP + gw * RWV + RWV <= q.n;
         if (direct) {
 #pragma unroll
             for (int i = 0; i < 2 * PASS; ++i) load_direct(t, i);
@@ -252,7 +261,7 @@ __global__ __launch_bounds__(64 * WAVES, QF && D == 256 ? 1 : 2) void k_prompt(P
         __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the stages before have arrived
 #pragma unroll 1
         for (int p = 0; p < PASS; ++p) {
-            const int r = p * RP + wave * RWV + rl;
+            const int r = p * RP + gw * RWV + rl;
             const int64_t off = group(t - t0, p);
             uint4v k = {0, 0, 0, 0}, v = {0, 0, 0, 0};
             if (off >= 0 && TS * t + r < q.n) {
@@ -278,7 +287,7 @@ __global__ __launch_bounds__(64 * WAVES, QF && D == 256 ? 1 : 2) void k_prompt(P
             bool any = false;
 #pragma unroll 1
             for (int p = 0; p < PASS; ++p) {
-                const int r = p * RP + wave * RWV + rl;
+                const int r = p * RP + gw * RWV + rl;
                 uint4v *at = (uint4v *)(lds + (uint32_t)(t - t0) % kStages * 2 * STAGE + STAGE + r * ROW + pl * 16);
                 uint4v v = *at;
                 bool has = false;
@@ -293,7 +302,7 @@ __global__ __launch_bounds__(64 * WAVES, QF && D == 256 ? 1 : 2) void k_prompt(P
                 if (pl == 0) odd_row[(uint32_t)(t - t0) % 8][r] = (by >> (rl * PC) & (PC == 64 ? ~0ull : (1ull << PC) - 1)) != 0;
                 any |= by != 0;
             }
-            if (lane == 0) any_odd[(uint32_t)(t - t0) % 8][wave] = any;
+            if (lane == 0) any_odd[(uint32_t)(t - t0) % 8][gw] = any;
         }
         __syncthreads();
     };
@@ -306,7 +315,7 @@ __global__ __launch_bounds__(64 * WAVES, QF && D == 256 ? 1 : 2) void k_prompt(P
     float16v o[NR][DT];
     float m[NR], l[NR], c2[NR];
     int lim[NR];
-    const int row0 = rt * ROWS + wave * 32 * NR, wrows = min(32 * NR, rows - row0);   // of the wave (0 or less: none)
+    const int row0 = rt * ROWS + gw * 32 * NR, wrows = min(32 * NR, rows - row0);   // of the wave (0 or less: none)
     const int last = ahead + (row0 + max(wrows, 1) - 1) / G, least = ahead + row0 / G;   // slots of the wave's last and first token
     const int tw = wrows > 0 ? min(t1, (max(0, last + 1) + TS - 1) / TS) : t0;
 #pragma unroll
@@ -554,7 +563,7 @@ __global__ __launch_bounds__(64 * WAVES, QF && D == 256 ? 1 : 2) void k_prompt(P
         __asm__ volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * PASS) : "memory");
         __syncthreads();
     };
-    if (t0 < t1) {
+    if (p0 < p1) {
         arrive(t0);
         if (t0 < tw) qk(place(t0), x);
         int t = t0;
@@ -569,7 +578,7 @@ __global__ __launch_bounds__(64 * WAVES, QF && D == 256 ? 1 : 2) void k_prompt(P
             if (t >= td) {
                 int any = 0;
 #pragma unroll
-                for (int w = 0; w < WAVES; ++w) any |= any_odd[(uint32_t)(t - t0) % 8][w];
+                for (int w = 0; w < GW; ++w) any |= any_odd[(uint32_t)(t - t0) % 8][w];
                 if (__builtin_amdgcn_readfirstlane(any)) add_odd(t);
             }
             ++t;
@@ -593,13 +602,50 @@ __global__ __launch_bounds__(64 * WAVES, QF && D == 256 ? 1 : 2) void k_prompt(P
             start(t);
             middle(t);
         }
+        if constexpr (HALVES) {
+            for (int k = t1 - t0; k <= turns; ++k) __syncthreads();   // as many as the other half's, and one: LDS is free
+#pragma unroll
+            for (int a = 0; a < NR; ++a) l[a] += __shfl_xor(l[a], 32);
+            // a lane's sums lie in the same places in both
+            float4v *po = sh4 + (size_t)gw * NR * DT * 4 * 64 + lane;
+            float2 *pm = (float2 *)(sh4 + (size_t)GW * NR * DT * 4 * 64) + (size_t)gw * NR * 64 + lane;
+            if (half) {
+#pragma unroll
+                for (int a = 0; a < NR; ++a) {
+#pragma unroll
+                    for (int t = 0; t < DT; ++t)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) po[((a * DT + t) * 4 + i) * 64] = float4v{o[a][t][4 * i], o[a][t][4 * i + 1], o[a][t][4 * i + 2], o[a][t][4 * i + 3]};
+                    pm[a * 64] = make_float2(m[a], l[a]);
+                }
+            }
+            __syncthreads();
+            if (half) return;
+#pragma unroll
+            for (int a = 0; a < NR; ++a) {
+                const float2 ml = pm[a * 64];
+                const float mn = fmaxf(m[a], ml.x), f0 = m[a] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[a] - mn), f1 = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - mn);
+                m[a] = mn;
+                l[a] = l[a] * f0 + ml.y * f1;
+#pragma unroll
+                for (int t = 0; t < DT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float4v w = po[((a * DT + t) * 4 + i) * 64];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[a][t][4 * i + e] = o[a][t][4 * i + e] * f0 + w[e] * f1;
+                    }
+            }
+        }
     }
+    if constexpr (HALVES)
+        if (half) return;
 
     float *rec = J.part + (size_t)blockIdx.x * ROWS * (D + 2);
 #pragma unroll
     for (int a = 0; a < NR; ++a) {
         const int r = row0 + 32 * a + ln;
-        l[a] += __shfl_xor(l[a], 32);
+        if constexpr (!HALVES) l[a] += __shfl_xor(l[a], 32);
         if (r >= rows) continue;
 #pragma unroll
         for (int t = 0; t < DT; ++t)
@@ -618,12 +664,12 @@ __global__ __launch_bounds__(64 * WAVES, QF && D == 256 ? 1 : 2) void k_prompt(P
 }
 
 // The records of split segments: a thread four elements of a row, over all parts in order.
-template <int D, int TS, int ROWS>
+template <int D, int TS, int ROWS, int COST>
 __global__ __launch_bounds__(256) void k_prompt_join(PromptJob J) {
     const KvDev &c = J.c;
     const float bias = c.bf16 ? 0.0f : 7.0f;
     const int h = blockIdx.x % c.n_kv, x = blockIdx.x / c.n_kv;
-    const int per = prompt_per<ROWS, TS>(J);
+    const int per = prompt_per<COST, ROWS, TS>(J);
     int s, rt, part;
     const PromptSeq q = prompt_find<ROWS, TS>(J, per, false, x, s, rt, part);
     if (s < 0 || q.parts < 2) return;
@@ -653,27 +699,29 @@ __global__ __launch_bounds__(256) void k_prompt_join(PromptJob J) {
     }
 }
 
-// Rows of a workgroup: 8 waves of 32 rows, two a SIMD; 4 waves where sequences have no more rows than those, where contexts are short and too
-// few compute units would get a workgroup of 8 (long ones are cut: 2 x 325 tokens of 8 heads a group over 49909 slots 533 us with 4,
-// 386 with 8), and where rows of 256 elements and queries of several parts together take more than 256 registers a lane. Segments are split where a head has at most half as many as workgroups for
-// it. (Equal shares of all tiles in a row, cut anywhere, balance better but read K and V at as many places at once as there are
-// workgroups, which the L2s do not hold: 95 against 72 us at 2048 tokens, 1086 against 604 at 2 x 8190 slots of 256 elements.)
-struct PromptPlan { int waves, rows, segs, heads_wg; bool split; size_t rec_bytes; };
+// Rows of a workgroup: 256, or 128 where sequences have no more rows than those, where contexts are short and too few compute units
+// would get a workgroup of 256 (long ones are cut: 2 x 325 tokens of 8 heads a group over 49909 slots 533 us with 128, 386 with
+// 256), and where rows of 256 elements and queries of several parts together take more than 256 registers a lane. Segments are split
+// where a head has at most half as many as workgroups for it. (Equal shares of all tiles in a row, cut anywhere, balance better but
+// read K and V at as many places at once as there are workgroups, which the L2s do not hold: 95 against 72 us at 2048 tokens, 1086
+// against 604 at 2 x 8190 slots of 256 elements.)
+struct PromptPlan { int rows, segs, heads_wg; bool split; size_t rec_bytes; };
 static PromptPlan prompt_plan(const KvDev &c, const DraftDev &d, int D) {
     PromptPlan p;
     auto segs = [&](int rows) {   // of a head: row tiles of all sequences, at most
         const int64_t each = ((int64_t)d.max_tokens * d.G + rows - 1) / rows, all = (int64_t)d.n_tokens * d.G / rows + std::min(c.n_seq, d.n_tokens);
         return std::min(each * c.n_seq, all);
     };
-    const int cus = num_cus(), tiles = c.max_len / tile_slots(D, c.bf16, d.q_f32) + 1;
-    p.waves = (D == 256 && d.q_f32) || (int64_t)d.max_tokens * d.G <= 128 || (tiles <= 32 && segs(256) * c.n_kv < cus) ? 4 : 8;
-    p.rows = 32 * p.waves;
+    const int cus = num_cus();
+    p.rows = (D == 256 && d.q_f32) || (int64_t)d.max_tokens * d.G <= 128 || (c.max_len < 2048 && segs(256) * c.n_kv < cus) ? 128 : 256;
     const int64_t n = segs(p.rows);
     p.segs = (int)std::min<int64_t>(n, INT32_MAX);
-    // Several sequences of few rows, whose records are small: parts in three rounds, so that long and short ones even out (24
-    // sequences of one token and 400 to 4000 slots, 8 heads of 128: whole 97 us, so 80).
-    p.heads_wg = cus / c.n_kv * (c.n_seq > 1 && (int64_t)d.max_tokens * d.G <= 64 ? 3 : 1);
-    p.split = p.heads_wg >= 2 * n && tiles > kJoinTiles + 1;
+    // A round of the compute units; of rows whose records are small two, where one is too few to cut all segments, so that long and
+    // short ones even out (24 sequences of one token and 400 to 4000 slots, 8 heads of 128: whole 97 us, so 64; 8 of 1600 to 16000
+    // slots in one round 66, in two 76, in three 90), or where a compute unit has room for two workgroups (64 elements: 35 to 28).
+    p.heads_wg = cus / c.n_kv;
+    if ((D == 64 || p.heads_wg < 2 * n) && (int64_t)d.max_tokens * d.G <= 64) p.heads_wg *= 2;
+    p.split = p.heads_wg >= 2 * n && c.max_len > (kJoin + kLeast) / slot_cost(D);
     p.rec_bytes = 4 * (size_t)p.rows * (D + 2);
     return p;
 }
@@ -683,26 +731,30 @@ size_t attn_prompt_workspace(const KvDev &c, const DraftDev &d, int D) {
     return p.split ? (size_t)p.heads_wg * c.n_kv * p.rec_bytes : 0;
 }
 
-template <int D, bool BF, bool QF, int WAVES>
+template <int D, bool BF, bool QF, int WAVES, bool HALVES>
 static int prompt_run(const PromptJob &J, int segs, hipStream_t st) {
-    constexpr int TS = tile_slots(D, BF, QF), lds = kStages * 2 * TS * 2 * D, ROWS = 32 * WAVES;
+    constexpr int TS = tile_slots(D, BF, QF, HALVES), lds = (HALVES ? 2 : 1) * kStages * 2 * TS * 2 * D, ROWS = 32 * (HALVES ? WAVES / 2 : WAVES);
     static OncePerDevice once;
-    if (int rc = allow_lds(once, (const void *)k_prompt<D, BF, QF, 1, WAVES>, lds, "p8x_attn_prompt LDS")) return rc;
-    k_prompt<D, BF, QF, 1, WAVES><<<J.heads_wg * J.c.n_kv, 64 * WAVES, lds, st>>>(J);
+    if (int rc = allow_lds(once, (const void *)k_prompt<D, BF, QF, 1, WAVES, HALVES>, lds, "p8x_attn_prompt LDS")) return rc;
+    k_prompt<D, BF, QF, 1, WAVES, HALVES><<<J.heads_wg * J.c.n_kv, 64 * WAVES, lds, st>>>(J);
     if (J.split) {   // a pass of 256 threads for a row tile's pieces, up to 8 of them side by side
         const int64_t pieces = std::min<int64_t>(ROWS, (int64_t)J.d.max_tokens * J.d.G) * (D / 4);
-        k_prompt_join<D, TS, ROWS><<<dim3(segs * J.c.n_kv, (unsigned)std::min<int64_t>(8, (pieces + 255) / 256)), 256, 0, st>>>(J);
+        k_prompt_join<D, TS, ROWS, slot_cost(D)><<<dim3(segs * J.c.n_kv, (unsigned)std::min<int64_t>(8, (pieces + 255) / 256)), 256, 0, st>>>(J);
     }
     return hip_check(hipGetLastError(), "p8x_attn_prompt launch");
 }
 
+template <int D, bool BF, bool QF>
+static int prompt_form(const PromptJob &J, const PromptPlan &p, hipStream_t st) {
+    if constexpr (D == 256 && QF) return prompt_run<D, BF, QF, 4, false>(J, p.segs, st);
+    else if (p.rows == 256) return prompt_run<D, BF, QF, 8, false>(J, p.segs, st);
+    else if constexpr (D != 128) return prompt_run<D, BF, QF, 4, false>(J, p.segs, st);
+    else return prompt_run<D, BF, QF, 8, true>(J, p.segs, st);
+}
+
 template <int D, bool BF>
 static int prompt_types(const PromptJob &J, const PromptPlan &p, hipStream_t st) {
-    if constexpr (D < 256) {
-        if (J.d.q_f32 && p.waves == 8) return prompt_run<D, BF, true, 8>(J, p.segs, st);
-    }
-    if (J.d.q_f32) return prompt_run<D, BF, true, 4>(J, p.segs, st);
-    return p.waves == 8 ? prompt_run<D, BF, false, 8>(J, p.segs, st) : prompt_run<D, BF, false, 4>(J, p.segs, st);
+    return J.d.q_f32 ? prompt_form<D, BF, true>(J, p, st) : prompt_form<D, BF, false>(J, p, st);
 }
 
 int launch_attn_prompt(const KvDev &c, const DraftDev &d, int D, void *out, int out_dtype, size_t ldo, size_t hso, float *lse, void *ws, size_t ws_bytes,
