@@ -102,8 +102,9 @@ __device__ __forceinline__ int prompt_per(const PromptJob &J) {
         });
         most = first_most(most, J.c.n_seq);
         per = max(least(most), (int)(tiles / (float)J.heads_wg) + 1);
-        // (there are at least twice as many workgroups as segments: twice the first `per` always fits)
-        while (over([&](int s) { const PromptSeq q = prompt_seq<ROWS, TS>(J, s, per); return (float)q.rts * (float)q.parts; }) > (float)J.heads_wg) per += (per + 7) / 8;
+        // (there are at least twice as many workgroups as segments: twice the first `per` fits, or, of sequences that overlap in
+        // `first` and so may have more segments than that, none)
+        while (per < most && over([&](int s) { const PromptSeq q = prompt_seq<ROWS, TS>(J, s, per); return (float)q.rts * (float)q.parts; }) > (float)J.heads_wg) per += (per + 7) / 8;
     }
     return most - per <= kJoin / COST / TS ? 0 : per;
 }

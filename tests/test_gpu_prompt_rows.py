@@ -80,3 +80,16 @@ def test_sink(cache, depth):
     # weights of e^-depth / (1 + 299 e^-depth), held to u of themselves behind the sink's tile; sums of at most 300 terms
     tol = (u + 400 * 2.0 ** -23 + 2.0 ** -15) * 236 * np.exp(-float(depth)) * 5.0 + u * np.abs(ref) + (2.0 ** -25 if cache == F16 else 0)
     assert (np.abs(got - ref) <= tol).all()
+
+
+def test_sequences_that_overlap():
+    # `first` goes up and down: every other sequence has the same token, which makes more segments than any workspace is meant for
+    S = 81
+    c = Prompt([900] * S, [1] + [0] * (S - 1), cache=F16, q=F16, heads=32, kv=8, page=64, seed=130)
+    c.pages[:] = c.pages[0]
+    want = c.causal()
+    c.first = np.array([i % 2 for i in range(S + 1)], np.int32)
+    out, lse = c.run()
+    # a workgroup writes the whole of a row or nothing of it
+    assert (np.abs(from_bits(out[:1], F16) - want[0][:1]) <= want[2][:1]).all()
+    assert (np.abs(lse[:1] - want[1][:1]) <= want[3][:1]).all()
