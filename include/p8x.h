@@ -413,7 +413,7 @@ typedef struct p8x_heads {
  * head_dim a multiple of 8, 8 .. 256. */
 int p8x_rope(const p8x_rotation *r, int n_tokens, int head_dim, const int32_t *pos, const p8x_heads *q, const p8x_heads *k, void *stream);
 
-/* p8x_kv_append of all tokens (the fields of d that it reads, any number of tokens) with their keys rotated on the way, and
+/* p8x_kv_append of all tokens (the fields of d that it reads, up to 2^30 tokens a sequence) with their keys rotated on the way, and
  * their queries q (NULL: none) rotated to q->out: one pass over the products of a layer. Positions are at[token] (NULL: the slot that the
  * token takes), and are stored to pos (NULL: not stored). Tokens past max_len are dropped (their queries are rotated). Rows of q->out of no sequence
  * are left as they are. */
@@ -422,8 +422,8 @@ int p8x_kv_append_rope(const p8x_kv_cache *c, const p8x_drafts *d, const p8x_rot
 
 /* Causal attention of new tokens that are in the cache already (p8x_kv_append_rope, p8x_kv_append; c->len counts them): of the nt
  * tokens of a sequence of n slots, token i sees slots 0 .. n - nt + i. out = softmax(scale q k) v, lse [n_tokens][n_heads] = log of the
- * sum of exp (NULL: not stored). Any number of tokens a sequence; of d first, n_tokens, max_tokens, q and scale are read, mask is
- * NULL. P8X_F32 queries are multiplied and weighed in f32 accuracy (as sums of 16-bit parts), to out of any type; 16-bit ones as they are, with
+ * sum of exp (NULL: not stored). Up to 2^30 tokens a sequence, in
+ * all (n_tokens n_heads / n_kv / 128 + n_seq) n_kv below 2^23; of d first, n_tokens, max_tokens, q and scale are read, mask is NULL. P8X_F32 queries are multiplied and weighed in f32 accuracy (as sums of 16-bit parts), to out of any type; 16-bit ones as they are, with
  * weights rounded to the cache's type, to out of either 16-bit type. Sums are f32. A token that sees no slot (no page, a length below nt), or only scores
  * of -inf, gets 0 and lse -inf; what a token does not see does not reach it, be it infinite or NaN; what it sees of them reaches it as infinities or NaN.
  * A weight is held to half a step of its type, or on a P8X_F16 cache to 2^-17 (P8X_F32 queries: 2^-22) of the largest weight of its row

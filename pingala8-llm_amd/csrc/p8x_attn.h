@@ -98,15 +98,6 @@ __device__ __forceinline__ void load_lds(const uint16_t *base, uint32_t off, uin
     __asm__ volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0" : "=&s"(m0) : "v"(off), "s"(base), "s"(to) : "memory");
 }
 
-// The same of two bases, one after the other. (The wait states before the first are for a base that a VALU instruction wrote, the
-// one before the second for M0.)
-__device__ __forceinline__ void load_lds2(const uint16_t *base0, uint32_t off0, uint32_t to0, const uint16_t *base1, uint32_t off1, uint32_t to1) {
-    uint32_t m0;
-    __asm__ volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %5\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %3\n\t"
-                     "s_mov_b32 m0, %6\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %4\n\ts_mov_b32 m0, %0"
-                     : "=&s"(m0) : "v"(off0), "v"(off1), "s"(base0), "s"(base1), "s"(to0), "s"(to1) : "memory");
-}
-
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 // 8 elements of a draft row as the cache holds them

@@ -2,6 +2,7 @@
 // checks, and the structs of p8x.h as kernel arguments.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include "p8x_kv.h"
@@ -69,6 +70,8 @@ int check_drafts(const char *fn, const p8x_kv_cache *c, const p8x_drafts *d, boo
     }
     return P8X_OK;
 }
+
+constexpr int kMostTokens = 1 << 30;   // of a sequence: slots are counted in 31 bits
 
 // the rotation of heads of D elements
 int check_rotation(const char *fn, const p8x_rotation *r, int D, TurnDev &o) {
@@ -241,7 +244,7 @@ int p8x_kv_append_rope(const p8x_kv_cache *c, const p8x_drafts *d, const p8x_rot
     TurnDev turn;
     HeadsDev h;
     int rc = check_cache(fn, c, k);
-    if (!rc) rc = check_drafts(fn, c, d, true, true, false, 0, t);
+    if (!rc) rc = check_drafts(fn, c, d, true, true, false, kMostTokens, t);
     if (!rc) rc = check_rotation(fn, r, c->head_dim, turn);
     if (!rc) rc = check_heads(fn, q, c->head_dim, h);
     if (rc) return rc;
@@ -254,11 +257,14 @@ int p8x_attn_prompt(const p8x_kv_cache *c, const p8x_drafts *d, void *out, int o
     KvDev k;
     DraftDev q;
     int rc = check_cache(fn, c, k);
-    if (!rc) rc = check_drafts(fn, c, d, false, false, true, 0, q);
+    if (!rc) rc = check_drafts(fn, c, d, false, false, true, kMostTokens, q);
     if (rc) return rc;
     if (d->mask) return set_error(P8X_ERR_ARG, "%s: a mask (its tokens see all before them)", fn);
     if (!is_float(out_dtype)) return set_error(P8X_ERR_ARG, "%s: out dtype %d", fn, out_dtype);
     if (!d->n_tokens || !d->max_tokens) return P8X_OK;
+    // row tiles of 128 at least, 512 threads each: a launch has less than 2^32 (and rows of a sequence stay below 2^31)
+    if (((int64_t)d->n_tokens * q.G / 128 + std::min(c->n_seq, d->n_tokens)) * c->n_kv >= 1 << 23)
+        return set_error(P8X_ERR_UNSUPPORTED, "%s: %d tokens of %d sequences, %d heads (row tiles of 128: below 2^23)", fn, d->n_tokens, c->n_seq, d->n_heads);
     if (out_dtype == P8X_F32 && d->q_dtype != P8X_F32) return set_error(P8X_ERR_UNSUPPORTED, "%s: f32 out of 16-bit queries", fn);
     const size_t hs = head_stride_out ? head_stride_out : (size_t)c->head_dim;
     if (!out || !rows_ok(out, out_dtype, ld_out, hs, d->n_heads, c->head_dim))

@@ -716,7 +716,7 @@ static PromptPlan prompt_plan(const KvDev &c, const DraftDev &d, int D) {
     const int cus = num_cus();
     p.rows = (D == 256 && d.q_f32) || (int64_t)d.max_tokens * d.G <= 128 || (c.max_len < 2048 && segs(256) * c.n_kv < cus) ? 128 : 256;
     const int64_t n = segs(p.rows);
-    p.segs = (int)std::min<int64_t>(n, INT32_MAX);
+    p.segs = (int)n;
     // A round of the compute units; of rows whose records are small two, where one is too few to cut all segments, so that long and
     // short ones even out (24 sequences of one token and 400 to 4000 slots, 8 heads of 128: whole 97 us, so 64; 8 of 1600 to 16000
     // slots in one round 66, in two 76, in three 90), or where a compute unit has room for two workgroups (64 elements: 35 to 28).
@@ -762,8 +762,6 @@ int launch_attn_prompt(const KvDev &c, const DraftDev &d, int D, void *out, int 
                        hipStream_t st) {
     if (c.slot_stride >= (1u << 26)) return set_error(P8X_ERR_UNSUPPORTED, "p8x_attn_prompt: slot_stride %zu (below 2^26)", c.slot_stride);
     const PromptPlan p = prompt_plan(c, d, D);
-    if ((int64_t)p.segs * c.n_kv > INT32_MAX || (int64_t)d.max_tokens * d.G > INT32_MAX)
-        return set_error(P8X_ERR_UNSUPPORTED, "p8x_attn_prompt: %d row tiles of %d heads, %d tokens of %d heads", p.segs, c.n_kv, d.max_tokens, d.G);
     PromptJob J{c, d, out, ldo, hso, out_dtype, lse, (float *)ws, p.segs, 0};
     const int room = (int)std::min<size_t>(p.heads_wg, ws_bytes / p.rec_bytes / c.n_kv);
     if (p.split && room >= 2 * p.segs) J.split = 1, J.heads_wg = room;

@@ -143,3 +143,9 @@ def test_bad_workspace():
 def test_no_tokens_is_no_work():
     prompt(n_tokens=0, q=None, out=None).run()
     prompt(max_tokens=0, q=None, out=None).run()
+
+
+def test_more_tokens_than_are_counted():
+    refused(append(d=tokens(max_tokens=(1 << 30) + 1)))
+    refused(prompt(max_tokens=(1 << 30) + 1))
+    refused(prompt(n_tokens=1 << 29))
