@@ -18,10 +18,10 @@
 // What bounds it: the matrix units, at the clock that the card's power leaves. 8190 tokens of 32 heads on 8 of 128 elements, fp16: 550
 // GFLOP in 556 us, 988 TFLOP/s, where a large library product reaches 1191; K, V and queries together would take 20 us from HBM. The matrix
 // units are busy for 51% of the cycles (63% with f32 queries, which have twice the products to an exponential), the clock is about
-// 1.85 GHz meanwhile. Rows of 256 elements, bf16: 471 GFLOP in 534 us, 882 TFLOP/s; f32 queries, fp16 cache, 999 tokens over 16000 slots: 254
-// GFLOP, products of two parts, in 500 us, 1015 TFLOP/s counting both. What else was tried at 8190 tokens: operands of LDS eight
+// 1.85 GHz meanwhile. Rows of 256 elements, bf16: 471 GFLOP in 537 us, 877 TFLOP/s; f32 queries, fp16 cache, 999 tokens over 16000 slots: 254
+// GFLOP, products of two parts, in 497 us, 1022 TFLOP/s counting both. What else was tried at 8190 tokens: operands of LDS eight
 // products ahead instead of four (slower: reads in flight beyond about eight delay each other), two barriers a turn (605 against
-// 541 us for 256 elements), the loads among the products (nothing). Few rows are bound by what is done in turn, 12 us at least: the
+// 541 us for 256 elements), the loads among the products (nothing). Few rows are bound by what is done in turn, 10 us at least: the
 // tables, the first K, the products of a tile, the sums.
 #include <hip/hip_runtime.h>
 
@@ -171,7 +171,9 @@ __device__ __forceinline__ PromptSeq prompt_find(const PromptJob &J, int per, bo
     return r;
 }
 
-template <int D>
+__device__ __forceinline__ float lse_of(float m, float l, float bias) { return l == 0.0f ? -INFINITY : (m - bias + __log2f(l)) * kLn2; }
+
+// four elements of the result, from the joined sums
 __device__ __forceinline__ void store_out(const PromptJob &J, int first, int h, int row, int e, float4v v, float m, float l, float bias) {
     const int G = J.d.G, i = row / G, head = h * G + row - i * G;
     v *= l == 0.0f ? 0.0f : 1.0f / l;
@@ -179,7 +181,7 @@ __device__ __forceinline__ void store_out(const PromptJob &J, int first, int h, 
     if (J.out_dtype == P8X_F32) *(float4v *)((float *)J.out + at) = v;
     else if (J.out_dtype == P8X_BF16) *(uint2v *)((uint16_t *)J.out + at) = uint2v{pack2<true>(v[0], v[1]), pack2<true>(v[2], v[3])};
     else *(uint2v *)((uint16_t *)J.out + at) = uint2v{pack2<false>(v[0], v[1]), pack2<false>(v[2], v[3])};
-    if (e == 0 && J.lse) J.lse[(size_t)(first + i) * J.c.n_kv * G + head] = l == 0.0f ? -INFINITY : (m - bias + __log2f(l)) * kLn2;
+    if (e == 0 && J.lse) J.lse[(size_t)(first + i) * J.c.n_kv * G + head] = lse_of(m, l, bias);
 }
 
 // HALVES: the second four waves have the rows of the first, over the second half of the tiles, in a ring of stages of their own; the sums
@@ -651,25 +653,35 @@ __global__ __launch_bounds__(64 * WAVES, QF && D == 256 ? 1 : 2) void k_prompt(P
     if constexpr (HALVES)
         if (half) return;
 
-    float *rec = J.part + (size_t)blockIdx.x * ROWS * (D + 2);
+    // (the cases around the pieces, not in each: what is fetched and run once a workgroup took 3 us of the 20.4 of 512 tokens otherwise, 1.7 so)
 #pragma unroll
     for (int a = 0; a < NR; ++a) {
         const int r = row0 + 32 * a + ln;
         if constexpr (!HALVES) l[a] += __shfl_xor(l[a], 32);
         if (r >= rows) continue;
+        auto pieces = [&](auto f) {   // f(element, four sums from there)
 #pragma unroll
-        for (int t = 0; t < DT; ++t)
+            for (int t = 0; t < DT; ++t)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float4v v{o[a][t][4 * i], o[a][t][4 * i + 1], o[a][t][4 * i + 2], o[a][t][4 * i + 3]};
-                const int e = 32 * t + 8 * i + 4 * g;
-                if (q.parts == 1) {
-                    store_out<D>(J, q.first, h, r, e, v, m[a], l[a], kBias);
-                } else {
-                    *(float4v *)(rec + (size_t)(r - rt * ROWS) * D + e) = v;
-                    if (e == 0) *(float2 *)(rec + (size_t)ROWS * D + 2 * (r - rt * ROWS)) = make_float2(m[a], l[a]);
-                }
-            }
+                for (int i = 0; i < 4; ++i) f(32 * t + 8 * i + 4 * g, float4v{o[a][t][4 * i], o[a][t][4 * i + 1], o[a][t][4 * i + 2], o[a][t][4 * i + 3]});
+        };
+        if (q.parts > 1) {
+            float *rec = J.part + (size_t)blockIdx.x * ROWS * (D + 2) + (size_t)(r - rt * ROWS) * D;
+            if (g == 0) *(float2 *)(J.part + (size_t)blockIdx.x * ROWS * (D + 2) + (size_t)ROWS * D + 2 * (r - rt * ROWS)) = make_float2(m[a], l[a]);
+            pieces([&](int e, float4v v) { *(float4v *)(rec + e) = v; });
+            continue;
+        }
+        const int i = r / G, head = h * G + r - i * G;
+        const float by = l[a] == 0.0f ? 0.0f : 1.0f / l[a];
+        const size_t at = (size_t)(q.first + i) * J.ldo + (size_t)head * J.hso;
+        if (g == 0 && J.lse) J.lse[(size_t)(q.first + i) * c.n_kv * G + head] = lse_of(m[a], l[a], kBias);
+        if (J.out_dtype == P8X_BF16) {
+            pieces([&](int e, float4v v) { v *= by; *(uint2v *)((uint16_t *)J.out + at + e) = uint2v{pack2<true>(v[0], v[1]), pack2<true>(v[2], v[3])}; });
+        } else if (!QF || J.out_dtype == P8X_F16) {
+            pieces([&](int e, float4v v) { v *= by; *(uint2v *)((uint16_t *)J.out + at + e) = uint2v{pack2<false>(v[0], v[1]), pack2<false>(v[2], v[3])}; });
+        } else {
+            pieces([&](int e, float4v v) { *(float4v *)((float *)J.out + at + e) = v * by; });
+        }
     }
 }
 
@@ -705,7 +717,7 @@ __global__ __launch_bounds__(256) void k_prompt_join(PromptJob J) {
             l = l * f0 + ml.y * f1;
             m = mn;
         }
-        store_out<D>(J, q.first, h, rt * ROWS + r, e, v, m, l, bias);
+        store_out(J, q.first, h, rt * ROWS + r, e, v, m, l, bias);
     }
 }
 

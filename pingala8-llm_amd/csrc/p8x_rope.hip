@@ -8,8 +8,8 @@
 // cosine by their series over an eighth of a turn either way, once for all heads of a wave.
 //
 // What bounds it: HBM where rows are many, the launch where they are few. 1500 tokens of 48 normed heads of 128, f32 to bf16, 55 MB: 13.4
-// us, 4.1 TB/s, where a large copy reaches 4.9; appended (16 bits throughout, 37 MB) 12.0 us, 3.1 TB/s: half the bytes a
-// wave for the same angles, page lookup and norm. One token of 40 heads 3.7 us, 24 tokens of 48 appended 4.8.
+// us, 4.1 TB/s, where a large copy reaches 4.9; appended (16 bits throughout, 37 MB) 12.0 us: some 6 of it is what one round of waves does in
+// turn, lengths, pages, rows, stores. One token of 40 heads 3.7 us, 24 tokens of 48 appended 4.8.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
