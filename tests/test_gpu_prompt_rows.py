@@ -93,3 +93,26 @@ def test_sequences_that_overlap():
     # a workgroup writes the whole of a row or nothing of it
     assert (np.abs(from_bits(out[:1], F16) - want[0][:1]) <= want[2][:1]).all()
     assert (np.abs(lse[:1] - want[1][:1]) <= want[3][:1]).all()
+
+
+@pytest.mark.parametrize("cache,q", [(F16, F16), (BF16, F32)])
+@pytest.mark.parametrize("toks", [1, 5, 32])
+@pytest.mark.parametrize("n", [32, 33, 64, 65, 96, 97, 129, 544, 545, 897, 1500])
+def test_halves_and_parts_end_anywhere(n, toks, cache, q):
+    # 128 rows: two halves of the slots, each of none, one or more tiles, whole or in parts
+    c = Prompt([n], [min(n, toks)], cache=cache, q=q, heads=16, kv=4, page=32, seed=140 + n)
+    c.check(*c.run())
+
+
+@pytest.mark.parametrize("n", [70, 700])
+@pytest.mark.parametrize("what", [np.inf, np.nan])
+def test_odd_values_and_missing_pages_in_the_second_half(what, n):
+    c = Prompt([n, n - 3], [30, 1], cache=BF16, q=BF16, heads=16, kv=4, page=16, seed=150)
+    c.pages[0, (n - 40) // 16] = -1
+    clean = c.causal()
+    for j in (n - 1, n - 9):   # the last tokens', hidden from those before
+        c.row(c.vb, 0, j)[:, 3] = to_bits(np.float32(what), BF16)
+    got = from_bits(c.run()[0], BF16)
+    ok = np.abs(got - clean[0]) <= clean[2]
+    assert ok[:30 - 9].all() and ok[:31, :, :3].all() and ok[:31, :, 4:].all() and ok[30].all()
+    assert not np.isfinite(got[30 - 9:30, :, 3]).any()
