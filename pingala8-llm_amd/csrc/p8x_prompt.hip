@@ -1,7 +1,7 @@
 // p8x_prompt.hip -- causal attention of new tokens over the cache that holds them (p8x_attn_prompt).
 //
 // Rows: the (token, head of the group) pairs of a sequence and key/value head, token-major, so that the rows of a workgroup
-// end at about the same slot and share K and V. A wave has 32 NR rows; tiles of 64 slots (32 where 64 do not fit) come to LDS
+// end at about the same slot and share K and V. A wave has 32 rows; tiles of 64 slots (32 where 64 do not fit) come to LDS
 // asynchronously, once for the workgroup, in a ring of stages. Products on v_mfma_f32_32x32x16, transposed throughout so that
 // nothing passes through LDS between the two:
 //   S^T [slot][row] = K Q^T: A = K (lane m = lane % 32 is the slot, 8 elements at 8 (lane / 32)), B = Q, kept in registers; of its
@@ -186,9 +186,9 @@ __device__ __forceinline__ void store_out(const PromptJob &J, int first, int h, 
 
 // HALVES: the second four waves have the rows of the first, over the second half of the tiles, in a ring of stages of their own; the sums
 // of both meet in LDS at the end.
-template <int D, bool BF, bool QF, int NR, int WAVES, bool HALVES>
+template <int D, bool BF, bool QF, int WAVES, bool HALVES>
 __global__ __launch_bounds__(64 * WAVES, QF && D == 256 ? 1 : 2) void k_prompt(PromptJob J) {
-    constexpr int TS = tile_slots(D, BF, QF, HALVES), GW = HALVES ? WAVES / 2 : WAVES, SUB = TS / 32, C = D / 16, DT = D / 32, KS = TS / 16, PC = D / 8, ROW = 2 * D, ROWS = 32 * NR * GW;
+    constexpr int TS = tile_slots(D, BF, QF, HALVES), GW = HALVES ? WAVES / 2 : WAVES, SUB = TS / 32, C = D / 16, DT = D / 32, KS = TS / 16, PC = D / 8, ROW = 2 * D, ROWS = 32 * GW;
     constexpr int QP = QF ? (BF ? 3 : 2) : 1, PP = QP;
     constexpr float kBias = BF ? 0.0f : 7.0f;
     // (fp16) log2 of a lane's sum of weights below which the tile's largest is looked up, and of that one below which m moves down
@@ -323,25 +323,24 @@ __global__ __launch_bounds__(64 * WAVES, QF && D == 256 ? 1 : 2) void k_prompt(P
     for (; loaded < min(t1, t0 + next); ++loaded) load(loaded);
 
     // ---- the wave's rows: queries, last slot that each sees
-    uint4v qf[NR][QP][C];
-    float16v o[NR][DT];
-    float m[NR], l[NR], c2[NR];
-    int lim[NR];
-    const int row0 = rt * ROWS + gw * 32 * NR, wrows = min(32 * NR, rows - row0);   // of the wave (0 or less: none)
+    uint4v qf[QP][C];
+    float16v o[DT];
+    float m, l, c2;
+    int lim;
+    const int row0 = rt * ROWS + gw * 32, wrows = min(32, rows - row0);   // of the wave (0 or less: none)
     const int last = ahead + (row0 + max(wrows, 1) - 1) / G, least = ahead + row0 / G;   // slots of the wave's last and first token
     const int tw = wrows > 0 ? min(t1, (max(0, last + 1) + TS - 1) / TS) : t0;
-#pragma unroll
-    for (int a = 0; a < NR; ++a) {
-        const int r = row0 + 32 * a + ln, i = min(r, rows - 1) / G;
+    {
+        const int r = row0 + ln, i = min(r, rows - 1) / G;
         const bool on = r < rows;   // the others have queries of zeros and see what the last one does
-        lim[a] = ahead + i;
-        m[a] = -INFINITY;
-        l[a] = 0.0f;
-        c2[a] = fabsf(d.scale) * kLog2e;
+        lim = ahead + i;
+        m = -INFINITY;
+        l = 0.0f;
+        c2 = fabsf(d.scale) * kLog2e;
 #pragma unroll
         for (int t = 0; t < DT; ++t)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) o[a][t][e] = 0.0f;
+            for (int e = 0; e < 16; ++e) o[t][e] = 0.0f;
         const size_t at = on ? (size_t)(q.first + i) * d.ld_q + (size_t)(h * G + r - i * G) * d.hs_q + 8 * g : 0;
         if constexpr (QF) {
             // fp16 parts need the row scaled to 2^13 (the lane 32 apart holds the other half of it)
@@ -362,7 +361,7 @@ __global__ __launch_bounds__(64 * WAVES, QF && D == 256 ? 1 : 2) void k_prompt(P
                 const int ex = mx > 0.0f && mx < INFINITY ? 13 - (int)((__builtin_bit_cast(uint32_t, mx) >> 23) - 127) : 0;
                 const int e1 = min(ex, 100);   // in two steps: 2^ex may be beyond f32
                 s1 *= ldexpf(1.0f, e1), s2 = ldexpf(1.0f, ex - e1);
-                c2[a] = ldexpf(c2[a], -ex);
+                c2 = ldexpf(c2, -ex);
             }
 #pragma unroll
             for (int k = 0; k < C; ++k) {
@@ -371,29 +370,27 @@ __global__ __launch_bounds__(64 * WAVES, QF && D == 256 ? 1 : 2) void k_prompt(P
                 for (int e = 0; e < 8; ++e) f[k][e] = f[k][e] * s1 * s2;
                 split8<BF, QP>(f[k], w);
 #pragma unroll
-                for (int n = 0; n < QP; ++n) qf[a][n][k] = w[n];
+                for (int n = 0; n < QP; ++n) qf[n][k] = w[n];
             }
         } else {
 #pragma unroll
             for (int k = 0; k < C; ++k) {
                 uint4v w = on ? *(const uint4v *)((const uint16_t *)d.q + at + 16 * k) : uint4v{0, 0, 0, 0};
                 if (d.scale < 0) w ^= uint4v{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};   // its sign goes into the queries
-                qf[a][0][k] = w;
+                qf[0][k] = w;
             }
         }
-        c2[a] = fmaxf(c2[a], 0x1p-149f);   // of a scale of 0, or one that underflows: hidden scores, -inf, stay so
+        c2 = fmaxf(c2, 0x1p-149f);   // of a scale of 0, or one that underflows: hidden scores, -inf, stay so
     }
 
     const int k_at = ln * ROW + ((g ^ fk(ln)) * 16);   // pieces 2 c + g: c only flips higher bits
     const int tl = lane & 15, v_row = 4 * g + (tl >> 2), v_at = v_row * ROW + ((((lane >> 4 & 1) * 2 + (tl >> 1 & 1)) ^ fv(v_row)) * 16) + 8 * (tl & 1);
     auto place = [&](int t) { return lds + (uint32_t)(t - t0) % kStages * 2 * STAGE; };
-    auto qk = [&](const char *k, float16v (&x)[NR][SUB]) {
+    auto qk = [&](const char *k, float16v (&x)[SUB]) {
 #pragma unroll
-        for (int a = 0; a < NR; ++a)
+        for (int u = 0; u < SUB; ++u)
 #pragma unroll
-            for (int u = 0; u < SUB; ++u)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) x[a][u][e] = 0.0f;
+            for (int e = 0; e < 16; ++e) x[u][e] = 0.0f;
 #pragma unroll
         for (int n = 0; n < C; ++n)
 #pragma unroll
@@ -401,8 +398,7 @@ __global__ __launch_bounds__(64 * WAVES, QF && D == 256 ? 1 : 2) void k_prompt(P
                 const uint4v kf = *(const uint4v *)(k + (k_at ^ 32 * n) + 32 * u * ROW);
 #pragma unroll
                 for (int p = QP - 1; p >= 0; --p)   // small parts first
-#pragma unroll
-                    for (int a = 0; a < NR; ++a) x[a][u] = mfma32<BF>(kf, qf[a][p][n], x[a][u]);
+                    x[u] = mfma32<BF>(kf, qf[p][n], x[u]);
             }
     };
     // scores to weights, in parts; returns the lane's sum of them
@@ -427,66 +423,55 @@ __global__ __launch_bounds__(64 * WAVES, QF && D == 256 ? 1 : 2) void k_prompt(P
         return sum;
     };
     bool settled = false;   // every row has a reference
-    auto softmax = [&](float16v (&x)[NR][SUB], uint4v (&p)[NR][KS][PP]) {
-        float sum[NR];
+    auto softmax = [&](float16v (&x)[SUB], uint4v (&p)[KS][PP]) {
+        float sum;
         bool bad = !settled;
         if (settled) {
-#pragma unroll
-            for (int a = 0; a < NR; ++a) {
-                sum[a] = weights(x[a], c2[a], m[a], p[a]);
-                bad |= !(sum[a] <= __builtin_exp2f(kUp + kBias));
-                if (!BF) bad |= sum[a] < __builtin_exp2f(kBias - kLow);
-            }
+            sum = weights(x, c2, m, p);
+            bad |= !(sum <= __builtin_exp2f(kUp + kBias));
+            if (!BF) bad |= sum < __builtin_exp2f(kBias - kLow);
             bad = __any(bad);
         } else {
-#pragma unroll
-            for (int a = 0; a < NR; ++a) sum[a] = INFINITY;
+            sum = INFINITY;
         }
         if (bad) {
             settled = true;
-#pragma unroll
-            for (int a = 0; a < NR; ++a) {
-                float v = -INFINITY;
-#pragma unroll
-                for (int u = 0; u < SUB; ++u)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) v = fmaxf(v, x[a][u][e]);
-                v = fmaxf(v, __shfl_xor(v, 32)) * c2[a];   // log2 of the tile's largest (-inf: the row sees none of it)
-                float to = m[a];
-                if (v > m[a] && (m[a] == -INFINITY || !(sum[a] <= __builtin_exp2f(kUp + kBias)))) {
-                    to = v;
-                } else if (!BF && v < m[a] - kDown && v > -INFINITY) {
-                    const float ls = l[a] + __shfl_xor(l[a], 32);
-                    to = fmaxf(v, fminf(m[a], m[a] - (kRoom - __log2f(ls))));
-                }
-                to = fmaxf(to, __shfl_xor(to, 32));   // where one of the row's two lanes moves up so does the other
-                const float al = m[a] == -INFINITY || to == m[a] ? 1.0f : __builtin_amdgcn_exp2f(m[a] - to);
-                m[a] = to;
-                settled = settled && !__any(to == -INFINITY);
-                l[a] *= al;
-#pragma unroll
-                for (int t = 0; t < DT; ++t) o[a][t] *= al;
-                sum[a] = weights(x[a], c2[a], m[a], p[a]);
-            }
-        }
-#pragma unroll
-        for (int a = 0; a < NR; ++a) l[a] += sum[a];
-    };
-    // hides what a row does not see: later tokens' slots, those without a page
-    auto hide = [&](int t, uint32_t pg, float16v (&x)[NR][SUB]) {
-#pragma unroll
-        for (int a = 0; a < NR; ++a) {
-            const int see = lim[a] - TS * t - 4 * g;
+            float v = -INFINITY;
 #pragma unroll
             for (int u = 0; u < SUB; ++u)
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const int upto = pg >> (2 * u + half) & 1 ? see : -1;
+                for (int e = 0; e < 16; ++e) v = fmaxf(v, x[u][e]);
+            v = fmaxf(v, __shfl_xor(v, 32)) * c2;   // log2 of the tile's largest (-inf: the row sees none of it)
+            float to = m;
+            if (v > m && (m == -INFINITY || !(sum <= __builtin_exp2f(kUp + kBias)))) {
+                to = v;
+            } else if (!BF && v < m - kDown && v > -INFINITY) {
+                const float ls = l + __shfl_xor(l, 32);
+                to = fmaxf(v, fminf(m, m - (kRoom - __log2f(ls))));
+            }
+            to = fmaxf(to, __shfl_xor(to, 32));   // where one of the row's two lanes moves up so does the other
+            const float al = m == -INFINITY || to == m ? 1.0f : __builtin_amdgcn_exp2f(m - to);
+            m = to;
+            settled = settled && !__any(to == -INFINITY);
+            l *= al;
 #pragma unroll
-                    for (int e = 8 * half; e < 8 * half + 8; ++e) x[a][u][e] = 32 * u + 8 * (e / 4) + e % 4 > upto ? -INFINITY : x[a][u][e];
-                    __builtin_amdgcn_sched_barrier(0);
-                }
+            for (int t = 0; t < DT; ++t) o[t] *= al;
+            sum = weights(x, c2, m, p);
         }
+        l += sum;
+    };
+    // hides what a row does not see: later tokens' slots, those without a page
+    auto hide = [&](int t, uint32_t pg, float16v (&x)[SUB]) {
+        const int see = lim - TS * t - 4 * g;
+#pragma unroll
+        for (int u = 0; u < SUB; ++u)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int upto = pg >> (2 * u + half) & 1 ? see : -1;
+#pragma unroll
+                for (int e = 8 * half; e < 8 * half + 8; ++e) x[u][e] = 32 * u + 8 * (e / 4) + e % 4 > upto ? -INFINITY : x[u][e];
+                __builtin_amdgcn_sched_barrier(0);
+            }
     };
     typedef short s4 __attribute__((ext_vector_type(4)));
     auto vt = [&](const char *v, int t, int ks) {   // V^T operand: elements 32 t .., slots 16 ks ..
@@ -498,7 +483,7 @@ __global__ __launch_bounds__(64 * WAVES, QF && D == 256 ? 1 : 2) void k_prompt(P
     };
     constexpr int AHEAD = 4, EARLY = 4;   // operands that are read ahead of their products; of V before the barrier in front of them
     uint4v first[EARLY];
-    auto pv = [&](const char *v, const uint4v (&p)[NR][KS][PP]) {
+    auto pv = [&](const char *v, const uint4v (&p)[KS][PP]) {
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
@@ -506,8 +491,7 @@ __global__ __launch_bounds__(64 * WAVES, QF && D == 256 ? 1 : 2) void k_prompt(P
                 const uint4v e = ks * DT + t < EARLY ? first[ks * DT + t] : vt(v, t, ks);
 #pragma unroll
                 for (int n = PP - 1; n >= 0; --n)
-#pragma unroll
-                    for (int a = 0; a < NR; ++a) o[a][t] = mfma32<BF>(e, p[a][ks][n], o[a][t]);
+                    o[t] = mfma32<BF>(e, p[ks][n], o[t]);
             }
     };
     // Adds the odd values of a stage's slots, which are zeros there, to the rows that see them.
@@ -525,17 +509,15 @@ __global__ __launch_bounds__(64 * WAVES, QF && D == 256 ? 1 : 2) void k_prompt(P
                     for (int e = 0; e < 4; ++e) {
                         const uint32_t word = e < 2 ? w[0] : w[1];
                         const float v = e & 1 ? part_hi<BF>(word) : part_lo<BF>(word);
-#pragma unroll
-                        for (int a = 0; a < NR; ++a)
-                            o[a][k][4 * i + e] += !(v - v == 0.0f) && slot <= lim[a] ? v : 0.0f;
+                        o[k][4 * i + e] += !(v - v == 0.0f) && slot <= lim ? v : 0.0f;
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 }
         }
     };
 
-    float16v x[NR][SUB];
-    uint4v p[NR][KS][PP];
+    float16v x[SUB];
+    uint4v p[KS][PP];
     auto weigh = [&](int t) {
         softmax(x, p);
 #pragma unroll
@@ -551,7 +533,7 @@ __global__ __launch_bounds__(64 * WAVES, QF && D == 256 ? 1 : 2) void k_prompt(P
             __builtin_amdgcn_sched_group_barrier(0x100, 2 * (AHEAD - EARLY), 0);
 #pragma unroll
             for (int i = 0; i < NV + NK; ++i) {
-                __builtin_amdgcn_sched_group_barrier(0x8, NR, 0);
+                __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
                 if (i + AHEAD < NV) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
                 else if (i + AHEAD < NV + NK) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             }
@@ -616,72 +598,62 @@ __global__ __launch_bounds__(64 * WAVES, QF && D == 256 ? 1 : 2) void k_prompt(P
         }
         if constexpr (HALVES) {
             for (int k = t1 - t0; k <= turns; ++k) __syncthreads();   // as many as the other half's, and one: LDS is free
-#pragma unroll
-            for (int a = 0; a < NR; ++a) l[a] += __shfl_xor(l[a], 32);
+            l += __shfl_xor(l, 32);
             // a lane's sums lie in the same places in both
-            float4v *po = sh4 + (size_t)gw * NR * DT * 4 * 64 + lane;
-            float2 *pm = (float2 *)(sh4 + (size_t)GW * NR * DT * 4 * 64) + (size_t)gw * NR * 64 + lane;
+            float4v *po = sh4 + (size_t)gw * DT * 4 * 64 + lane;
+            float2 *pm = (float2 *)(sh4 + (size_t)GW * DT * 4 * 64) + (size_t)gw * 64 + lane;
             if (half) {
-#pragma unroll
-                for (int a = 0; a < NR; ++a) {
-#pragma unroll
-                    for (int t = 0; t < DT; ++t)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) po[((a * DT + t) * 4 + i) * 64] = float4v{o[a][t][4 * i], o[a][t][4 * i + 1], o[a][t][4 * i + 2], o[a][t][4 * i + 3]};
-                    pm[a * 64] = make_float2(m[a], l[a]);
-                }
-            }
-            __syncthreads();
-            if (half) return;
-#pragma unroll
-            for (int a = 0; a < NR; ++a) {
-                const float2 ml = pm[a * 64];
-                const float mn = fmaxf(m[a], ml.x), f0 = m[a] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[a] - mn), f1 = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - mn);
-                m[a] = mn;
-                l[a] = l[a] * f0 + ml.y * f1;
 #pragma unroll
                 for (int t = 0; t < DT; ++t)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float4v w = po[((a * DT + t) * 4 + i) * 64];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) o[a][t][4 * i + e] = o[a][t][4 * i + e] * f0 + w[e] * f1;
-                    }
+                    for (int i = 0; i < 4; ++i) po[(t * 4 + i) * 64] = float4v{o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]};
+                *pm = make_float2(m, l);
             }
+            __syncthreads();
+            if (half) return;
+            const float2 ml = *pm;
+            const float mn = fmaxf(m, ml.x), f0 = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn), f1 = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - mn);
+            m = mn;
+            l = l * f0 + ml.y * f1;
+#pragma unroll
+            for (int t = 0; t < DT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float4v w = po[(t * 4 + i) * 64];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[t][4 * i + e] = o[t][4 * i + e] * f0 + w[e] * f1;
+                }
         }
     }
     if constexpr (HALVES)
         if (half) return;
 
     // (the cases around the pieces, not in each: what is fetched and run once a workgroup took 3 us of the 20.4 of 512 tokens otherwise, 1.7 so)
+    const int r = row0 + ln;
+    if constexpr (!HALVES) l += __shfl_xor(l, 32);
+    if (r >= rows) return;
+    auto pieces = [&](auto f) {   // f(element, four sums from there)
 #pragma unroll
-    for (int a = 0; a < NR; ++a) {
-        const int r = row0 + 32 * a + ln;
-        if constexpr (!HALVES) l[a] += __shfl_xor(l[a], 32);
-        if (r >= rows) continue;
-        auto pieces = [&](auto f) {   // f(element, four sums from there)
+        for (int t = 0; t < DT; ++t)
 #pragma unroll
-            for (int t = 0; t < DT; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) f(32 * t + 8 * i + 4 * g, float4v{o[a][t][4 * i], o[a][t][4 * i + 1], o[a][t][4 * i + 2], o[a][t][4 * i + 3]});
-        };
-        if (q.parts > 1) {
-            float *rec = J.part + (size_t)blockIdx.x * ROWS * (D + 2) + (size_t)(r - rt * ROWS) * D;
-            if (g == 0) *(float2 *)(J.part + (size_t)blockIdx.x * ROWS * (D + 2) + (size_t)ROWS * D + 2 * (r - rt * ROWS)) = make_float2(m[a], l[a]);
-            pieces([&](int e, float4v v) { *(float4v *)(rec + e) = v; });
-            continue;
-        }
-        const int i = r / G, head = h * G + r - i * G;
-        const float by = l[a] == 0.0f ? 0.0f : 1.0f / l[a];
-        const size_t at = (size_t)(q.first + i) * J.ldo + (size_t)head * J.hso;
-        if (g == 0 && J.lse) J.lse[(size_t)(q.first + i) * c.n_kv * G + head] = lse_of(m[a], l[a], kBias);
-        if (J.out_dtype == P8X_BF16) {
-            pieces([&](int e, float4v v) { v *= by; *(uint2v *)((uint16_t *)J.out + at + e) = uint2v{pack2<true>(v[0], v[1]), pack2<true>(v[2], v[3])}; });
-        } else if (!QF || J.out_dtype == P8X_F16) {
-            pieces([&](int e, float4v v) { v *= by; *(uint2v *)((uint16_t *)J.out + at + e) = uint2v{pack2<false>(v[0], v[1]), pack2<false>(v[2], v[3])}; });
-        } else {
-            pieces([&](int e, float4v v) { *(float4v *)((float *)J.out + at + e) = v * by; });
-        }
+            for (int i = 0; i < 4; ++i) f(32 * t + 8 * i + 4 * g, float4v{o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]});
+    };
+    if (q.parts > 1) {
+        float *rec = J.part + (size_t)blockIdx.x * ROWS * (D + 2) + (size_t)(r - rt * ROWS) * D;
+        if (g == 0) *(float2 *)(J.part + (size_t)blockIdx.x * ROWS * (D + 2) + (size_t)ROWS * D + 2 * (r - rt * ROWS)) = make_float2(m, l);
+        pieces([&](int e, float4v v) { *(float4v *)(rec + e) = v; });
+        return;
+    }
+    const int i = r / G, head = h * G + r - i * G;
+    const float by = l == 0.0f ? 0.0f : 1.0f / l;
+    const size_t at = (size_t)(q.first + i) * J.ldo + (size_t)head * J.hso;
+    if (g == 0 && J.lse) J.lse[(size_t)(q.first + i) * c.n_kv * G + head] = lse_of(m, l, kBias);
+    if (J.out_dtype == P8X_BF16) {
+        pieces([&](int e, float4v v) { v *= by; *(uint2v *)((uint16_t *)J.out + at + e) = uint2v{pack2<true>(v[0], v[1]), pack2<true>(v[2], v[3])}; });
+    } else if (!QF || J.out_dtype == P8X_F16) {
+        pieces([&](int e, float4v v) { v *= by; *(uint2v *)((uint16_t *)J.out + at + e) = uint2v{pack2<false>(v[0], v[1]), pack2<false>(v[2], v[3])}; });
+    } else {
+        pieces([&](int e, float4v v) { *(float4v *)((float *)J.out + at + e) = v * by; });
     }
 }
 
@@ -757,8 +729,8 @@ template <int D, bool BF, bool QF, int WAVES, bool HALVES>
 static int prompt_run(const PromptJob &J, int segs, hipStream_t st) {
     constexpr int TS = tile_slots(D, BF, QF, HALVES), lds = (HALVES ? 2 : 1) * kStages * 2 * TS * 2 * D, ROWS = 32 * (HALVES ? WAVES / 2 : WAVES);
     static OncePerDevice once;
-    if (int rc = allow_lds(once, (const void *)k_prompt<D, BF, QF, 1, WAVES, HALVES>, lds, "p8x_attn_prompt LDS")) return rc;
-    k_prompt<D, BF, QF, 1, WAVES, HALVES><<<J.heads_wg * J.c.n_kv, 64 * WAVES, lds, st>>>(J);
+    if (int rc = allow_lds(once, (const void *)k_prompt<D, BF, QF, WAVES, HALVES>, lds, "p8x_attn_prompt LDS")) return rc;
+    k_prompt<D, BF, QF, WAVES, HALVES><<<J.heads_wg * J.c.n_kv, 64 * WAVES, lds, st>>>(J);
     if (J.split) {   // a pass of 256 threads for a row tile's pieces, up to 8 of them side by side
         const int64_t pieces = std::min<int64_t>(ROWS, (int64_t)J.d.max_tokens * J.d.G) * (D / 4);
         k_prompt_join<D, TS, ROWS, slot_cost(D)><<<dim3(segs * J.c.n_kv, (unsigned)std::min<int64_t>(8, (pieces + 255) / 256)), 256, 0, st>>>(J);
