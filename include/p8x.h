@@ -425,7 +425,8 @@ int p8x_kv_append_rope(const p8x_kv_cache *c, const p8x_drafts *d, const p8x_rot
  * sum of exp (NULL: not stored). Up to 2^30 tokens a sequence, in
  * all (n_tokens n_heads / n_kv / 128 + n_seq) n_kv below 2^23; of d first, n_tokens, max_tokens, q and scale are read, mask is NULL. P8X_F32 queries are multiplied and weighed in f32 accuracy (as sums of 16-bit parts), to out of any type; 16-bit ones as they are, with
  * weights rounded to the cache's type, to out of either 16-bit type. Sums are f32. A token that sees no slot (no page, a length below nt), or only scores
- * of -inf, gets 0 and lse -inf; what a token does not see does not reach it, be it infinite or NaN; what it sees of them reaches it as infinities or NaN.
+ * of -inf, gets 0 and lse -inf; what a token does not see does not reach it, be it infinite or NaN; what it sees of them reaches it as infinities or NaN (such a
+ * value also where all its scores are -inf).
  * A weight is held to half a step of its type, or on a P8X_F16 cache to 2^-17 (P8X_F32 queries: 2^-22) of the largest weight of its row
  * in 64 slots where that is more. out overlaps no input; rows of no sequence are left as they are.
  * workspace: device memory, any contents, 16-byte aligned, that splits long contexts of few tokens over workgroups (NULL or too little: fewer

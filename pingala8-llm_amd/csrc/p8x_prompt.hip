@@ -683,9 +683,9 @@ __global__ __launch_bounds__(256) void k_prompt_join(PromptJob J) {
             const float *rec = J.part + (size_t)((b0 + b) * c.n_kv + h) * ROWS * (D + 2);
             const float2 ml = *(const float2 *)(rec + (size_t)ROWS * D + 2 * r);
             const float4v w = *(const float4v *)(rec + (size_t)r * D + e);
-            if (ml.x == -INFINITY) continue;   // a part that the row sees nothing of
-            const float mn = fmaxf(m, ml.x), f0 = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn), f1 = __builtin_amdgcn_exp2f(ml.x - mn);
-            v = m == -INFINITY ? w * f1 : v * f0 + w * f1;
+            // (a part without a reference is not left out: of scores of NaN alone its sums are NaN, and else zeros)
+            const float mn = fmaxf(m, ml.x), mb = mn == -INFINITY ? 0.0f : mn, f0 = __builtin_amdgcn_exp2f(m - mb), f1 = __builtin_amdgcn_exp2f(ml.x - mb);
+            v = v * f0 + w * f1;
             l = l * f0 + ml.y * f1;
             m = mn;
         }
