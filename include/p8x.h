@@ -333,7 +333,7 @@ typedef struct p8x_drafts {
  * lse -inf; what a mask hides does not reach the token, be it infinite or NaN. At most P8X_MAX_DRAFT tokens a sequence.
  * P8X_F32 queries are multiplied in f32 accuracy (as sums of 16-bit parts), 16-bit ones as they are; sums are f32. A weight is
  * held to 2^-17 of itself or better, or, on a P8X_F16 cache, to 2^-19 (P8X_F32 queries: 2^-22) of the largest weight in its 32
- * slots where that is more, however far those are below others. An infinite or NaN key or value reaches the tokens that see it
+ * slots where that is more, however far those are below others, down to 2^-64 (P8X_BF16: 2^-110) of the sum of the row's weights. An infinite or NaN key or value reaches the tokens that see it
  * as infinities or NaN, also where the formula would give an infinity (values) or a weight of 0 (keys). out overlaps no input.
  * workspace: device memory that splits a sequence over workgroups (NULL or too little: fewer of them), zeroed
  * once by the caller before its first use and left zeroed where it has to be, for calls of any shape in turn; calls that
@@ -428,7 +428,7 @@ int p8x_kv_append_rope(const p8x_kv_cache *c, const p8x_drafts *d, const p8x_rot
  * of -inf, gets 0 and lse -inf; what a token does not see does not reach it, be it infinite or NaN; what it sees of them reaches it as infinities or NaN (such a
  * value also where all its scores are -inf).
  * A weight is held to half a step of its type, or on a P8X_F16 cache to 2^-17 (P8X_F32 queries: 2^-22) of the largest weight of its row
- * in 64 slots where that is more. out overlaps no input; rows of no sequence are left as they are.
+ * in 64 slots where that is more, down to 2^-64 (P8X_BF16: 2^-110) of the sum of the row's weights. out overlaps no input; rows of no sequence are left as they are.
  * workspace: device memory, any contents, 16-byte aligned, that splits long contexts of few tokens over workgroups (NULL or too little: fewer
  * of them, or none); calls that may overlap need one each. p8x_attn_prompt_workspace: bytes beyond which more do not help. */
 int p8x_attn_prompt(const p8x_kv_cache *c, const p8x_drafts *d, void *out, int out_dtype, size_t ld_out, size_t head_stride_out, float *lse,

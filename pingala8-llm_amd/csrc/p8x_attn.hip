@@ -14,7 +14,7 @@
 // lanes until the end. Weights enter the product as two 16-bit parts (three for f32 queries on a bf16 cache). bf16 parts have
 // the range of f32: a weight keeps 16 bits or more. fp16 parts end at 2^-24: weights stand there times 2^7, and where the largest
 // of a row's weights in a tile is below 2^-12 (2^-10 for f32 queries), as in a tail beside slots that take nearly all, m
-// moves down to it, which the f32 sums have the range for (up to 2^64: what is further below is below 2^-64 of the result).
+// moves down to it, as far as the f32 sums have the range for (up to 2^64: what is further below is below 2^-64 of the row's sum).
 // So a weight is held to 2^-17 of itself or 2^-19 (2^-22) of the largest of its tile. (Without moving down, weights e^-15 below
 // the largest were off by 1.4e-3 of themselves, at e^-26 by 10%. Moving from 2^-8 on, the usual spread of scores moves it back and
 // forth: 138 to 146 us at 256 rows of 64, 2 x 65535 slots.)

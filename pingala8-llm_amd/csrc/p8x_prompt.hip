@@ -13,7 +13,9 @@
 // reference, the sums are scaled and the weights made again, so that the usual tile needs no maximum and no exchange between lanes.
 // 16-bit queries take weights of one 16-bit part, f32 ones of two (fp16) or three (bf16); sums are of the unrounded weights. fp16
 // parts end at 2^-24: weights stand there times 2^7, and where a tile's largest is below 2^-10, as in a tail beside slots that
-// take nearly all, m moves down to it, for which f32 sums have the range.
+// take nearly all, m moves down to it, as far as f32 sums have the range for: until what was summed stands at 2^64 (kRoom), m 2^57 below it
+// (a weight's 2^7 apart). Steps of 2^-24 there are 2^-88 of the sum so far, and where a much larger score follows, the factor 2^(m - its m)
+// ends at 2^-126: what is below 2^-69 of the row's sum may be lost.
 //
 // What bounds it: the matrix units, at the clock that the card's power leaves. 8190 tokens of 32 heads on 8 of 128 elements, fp16: 550
 // GFLOP in 556 us, 988 TFLOP/s, where a large library product reaches 1191; K, V and queries together would take 20 us from HBM. The matrix
