@@ -178,7 +178,9 @@ static int rope_plan(RopeJob &J, int seqs) {
     J.each = (int)std::min<int64_t>(J.groups, std::max<int64_t>(1, all / (16 * num_cus())));
     while ((int64_t)J.n * ((J.groups + J.each - 1) / J.each) > INT32_MAX) J.each *= 2;
     const int64_t waves = (int64_t)J.n * ((J.groups + J.each - 1) / J.each);
-    return (int)std::min<int64_t>((waves + 3) / 4, 1 << 20);
+    // (workgroups go on with further tokens. Each sequence has as many as the longest may need: 65535 of one token and one of 200000 would
+    // be a launch of 3.3e9, nearly all of which find nothing)
+    return (int)std::min<int64_t>((waves + 3) / 4, std::max(8, (1 << 20) / seqs));
 }
 
 template <bool F32, bool APPEND>
