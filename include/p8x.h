@@ -378,7 +378,7 @@ size_t p8x_kv_evict_workspace(const p8x_kv_cache *c, int budget);
  *   v = x, or x / sqrt(mean(x^2) + eps) w of the whole head (w_q, w_k [head_dim]; NULL: no norm), then
  *   y_a = amplitude (v_a cos t - v_b sin t), y_b = amplitude (v_b cos t + v_a sin t), t = 2 pi p freq[i] / 2^64
  * for the pairs i < n_rot / 2, (a, b) = (i, i + n_rot / 2) (P8X_ROPE_HALF) or (2 i, 2 i + 1) (P8X_ROPE_PAIRS); elements from n_rot on
- * pass as v. freq holds turns a position as fractions of 2^64, so that the angle of any int32 position is exact to 2^-32 of a
+ * pass as v. freq holds turns a position as fractions of 2^64, so that the angle that it gives any int32 position is exact to 2^-32 of a
  * turn. Sums and products in f32. */
 enum { P8X_ROPE_HALF = 0, P8X_ROPE_PAIRS = 1 };
 typedef struct p8x_rotation {
@@ -392,7 +392,8 @@ typedef struct p8x_rotation {
  * `original` length: P8X_ROPE_LINEAR theta / factor; P8X_ROPE_BANDS theta / factor where the pair makes fewer than `low` turns in
  * `original` positions, theta where more than `high`, linear in the turns between; P8X_ROPE_YARN theta / factor from the pair that
  * makes `low` turns on, theta up to the one that makes `high`, linear in the pair's index between (both rounded outwards), and
- * amplitude 0.1 ln(factor) + 1 (for factor > 1; else, and for the other kinds, 1). amplitude may be NULL. */
+ * amplitude 0.1 ln(factor) + 1 (for factor > 1; else, and for the other kinds, 1). amplitude may be NULL. In 64-bit arithmetic: theta is held to
+ * 2^-49 of itself, an angle to 2^-30 of a turn up to position 2^21 / theta, 2^-20 up to the last (theta <= 1). */
 enum { P8X_ROPE_PLAIN = 0, P8X_ROPE_LINEAR = 1, P8X_ROPE_BANDS = 2, P8X_ROPE_YARN = 3 };
 typedef struct p8x_rope_scaling {
     int kind;

@@ -11,20 +11,28 @@
 // Softmax: the weights of a tile are relative to the row's reference m of the tiles before. Their sum, which is needed anyway,
 // tells whether that was good: where it is beyond 2^8 (or NaN, or there is no reference yet) the tile's largest score becomes the
 // reference, the sums are scaled and the weights made again, so that the usual tile needs no maximum and no exchange between lanes.
-// 16-bit queries take weights of one 16-bit part, f32 ones of two (fp16) or three (bf16); sums are of the unrounded weights. fp16
+// 16-bit queries take weights of one 16-bit part: a second would be half as many products again where the matrix units bound the call, for
+// an error beside that of the result's own rounding (together 0.0020 to 0.0023 of the largest for bf16, 0.0016 to 0.0017 by the
+// rounding alone; fp16 0.00027, 0.0002). Callers who need more pass f32 queries, with weights of two parts (fp16) or three (bf16). Sums are
+// f32, of the unrounded weights. fp16
 // parts end at 2^-24: weights stand there times 2^7, and where a tile's largest is below 2^-10, as in a tail beside slots that
 // take nearly all, m moves down to it, as far as f32 sums have the range for: until what was summed stands at 2^64 (kRoom), m 2^57 below it
 // (a weight's 2^7 apart). Steps of 2^-24 there are 2^-88 of the sum so far, and where a much larger score follows, the factor 2^(m - its m)
 // ends at 2^-126: what is below 2^-69 of the row's sum may be lost.
 //
 // What bounds it: the matrix units, at the clock that the card's power leaves. 8190 tokens of 32 heads on 8 of 128 elements, fp16: 550
-// GFLOP in 556 us, 988 TFLOP/s, where a large library product reaches 1191; K, V and queries together would take 20 us from HBM. The matrix
-// units are busy for 51% of the cycles (63% with f32 queries, which have twice the products to an exponential), the clock is about
-// 1.85 GHz meanwhile. Rows of 256 elements, bf16: 471 GFLOP in 537 us, 877 TFLOP/s; f32 queries, fp16 cache, 999 tokens over 16000 slots: 254
-// GFLOP, products of two parts, in 497 us, 1022 TFLOP/s counting both. What else was tried at 8190 tokens: operands of LDS eight
-// products ahead instead of four (slower: reads in flight beyond about eight delay each other), two barriers a turn (605 against
-// 541 us for 256 elements), the loads among the products (nothing). Few rows are bound by what is done in turn, 10 us at least: the
-// tables, the first K, the products of a tile, the sums.
+// GFLOP in 541 to 592 us by card, 930 to 1017 TFLOP/s, where a large library product reaches 1191; K, V and queries together would take 20 us
+// from HBM. The matrix units are busy for 51% of the cycles (63% with f32 queries, which have twice the products to an exponential), the
+// clock is about 1.85 GHz meanwhile. f32 queries, fp16 cache, 999 tokens over 16000 slots: 254 GFLOP, products of two parts, in 497 to 507 us,
+// 1022 to 1000 TFLOP/s counting both; on a bf16 cache, three parts, 590. 4096 tokens of 64 elements, 69 GFLOP: fp16 99 us, bf16 93, f32 queries
+// 159 and 189. Rows of 256 elements, bf16: 471 GFLOP in 537 us, 877 TFLOP/s: segments are as many as compute units, the longest of 320 tiles where
+// the mean is 253, and the registers do not suffice: with 16-bit queries 16 (eight waves) or 19 (four) go to scratch, of which a turn of the
+// steady loop reads none, one or two back and waits for all loads in flight, the ring's too. With f32 queries on bf16 60 do, and a turn reads
+// 13: 2 x 700 tokens over 8190 slots, 16 heads, 1108 us, on fp16 (none) 839, with 16-bit queries 211 to 219. What else was tried at 8190 tokens:
+// operands of LDS eight products ahead instead of four (slower: reads in flight beyond about eight delay each other), two barriers a turn (605
+// against 541 us for 256 elements), the loads among the products (nothing). Few rows are bound by what is done in turn, 10 us at least: the
+// tables, the first K, the products of a tile, the sums. Each workgroup reads `first` and `len` of all sequences to find its own: one token of 256
+// sequences of <= 201 slots 95 us, of 1024 477, of 4096 3.6 ms (floors 25, 98, 392).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -700,7 +708,9 @@ __global__ __launch_bounds__(256) void k_prompt_join(PromptJob J) {
 // 256), and where rows of 256 elements and queries of several parts together take more than 256 registers a lane. Segments are split
 // where a head has at most half as many as workgroups for it. (Equal shares of all tiles in a row, cut anywhere, balance better but
 // read K and V at as many places at once as there are workgroups, which the L2s do not hold: 95 against 72 us at 2048 tokens, 1086
-// against 604 at 2 x 8190 slots of 256 elements.)
+// against 604 at 2 x 8190 slots of 256 elements.) The host knows of a sequence's slots only that they are max_len at most: in a cache with
+// room for 2048 or more, 512 tokens take workgroups of 256 rows and a join that finds nothing to do, 26.5 us instead of 19.3 where max_len is
+// 512; 19 tokens 13.3 instead of 10.9.
 struct PromptPlan { int rows, segs, heads_wg; bool split; size_t rec_bytes; };
 static PromptPlan prompt_plan(const KvDev &c, const DraftDev &d, int D) {
     PromptPlan p;

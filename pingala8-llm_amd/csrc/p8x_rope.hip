@@ -2,14 +2,14 @@
 // (p8x_rope), or with the keys and values going to the cache (p8x_kv_append_rope).
 //
 // A head takes L lanes, 8 elements each: four pairs of it (elements 4 l .. of either half, or 8 l .. as neighbours) or 8
-// elements that pass; a wave takes 64 / L heads of one token at a time, and several such groups in turn, whose rows are all
-// requested before the first is used. The angle of a pair is p freq mod 2^64, a wrapping integer product: its upper 32 bits
+// elements that pass; a wave takes 64 / L heads of one token at a time, and several such groups in turn, two at a time. The angle of a pair is p freq mod 2^64, a wrapping integer product: its upper 32 bits
 // are the turn to 2^-32 whatever the position (as an f32 product, position 131071 would be off by 0.008 radians). Sine and
 // cosine by their series over an eighth of a turn either way, once for all heads of a wave.
 //
 // What bounds it: HBM where rows are many, the launch where they are few. 1500 tokens of 48 normed heads of 128, f32 to bf16, 55 MB: 13.4
-// us, 4.1 TB/s, where a large copy reaches 4.9; appended (16 bits throughout, 37 MB) 12.0 us: some 6 of it is what one round of waves does in
-// turn, lengths, pages, rows, stores. One token of 40 heads 3.7 us, 24 tokens of 48 appended 4.8.
+// us, 4.1 TB/s, where a large copy reaches 4.9; appended (16 bits throughout, 37 MB) 12.0 us: a wave's requests go out in turn (length, position,
+// page, then the rows of one group after those of the other: below). One token of 40 heads 3.3 to 4.1 us, 24 tokens of 48 appended 4.8. A prompt of
+// 8000 tokens appended alone 37 us, beside 255 single tokens 291: each sequence has as many workgroups as the longest.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -61,8 +61,10 @@ __device__ __forceinline__ void store4(void *p, size_t i, int dtype, float4v v) 
     }
 }
 
-// groups of heads whose rows a wave requests together (1500 tokens of 48 heads, and appended: 13.8 and 12.7 us; with 1, 13.5 and 12.9; with 4,
-// where fewer waves fit, 14.6 and 14.9)
+// groups of heads that a wave has in registers together (1500 tokens of 48 heads, and appended: 13.8 and 12.7 us; with 1, 13.5 and 12.9; with 4,
+// 14.6 and 14.9). Only the append of f32 rows has both groups' rows on their way at once: 16-bit rows are converted where they are
+// loaded, and without the append the place of q or k is read from the arguments in memory, so that either waits for one group before it
+// requests the next
 constexpr int kAtOnce = 2;
 
 // F32: of the rows that come in
